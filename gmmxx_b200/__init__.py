@@ -46,6 +46,7 @@ from .api import (
     tied_score_samples_torch_native_chunked,
 )
 from . import cuda_ops  # noqa: F401  (the reference's operator-level surface, gmmxx.cuda_ops)
+from .experts import RowGroups, group_rows, grouped_matmul, grouped_matmul_backward, orthogonalize
 from .interface import GMMXX
 from .large_n import (
     batch_gmm_largeN_cpu,
@@ -103,6 +104,11 @@ __all__ = [
     "large_n_predict_proba_cpu",
     "large_n_score_samples_cpu",
     "cuda_ops",
+    "RowGroups",
+    "group_rows",
+    "grouped_matmul",
+    "grouped_matmul_backward",
+    "orthogonalize",
 ]
 
 # The reference exports its Triton kernels under these names and sets each to

@@ -89,6 +89,17 @@ _SIGNATURES = {
     "gmmxx_label_stats_width": (_I64, [_I32, _I64]),
     "gmmxx_label_stats_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64, _I64]),
     "gmmxx_label_stats": (_I32, [_I32, _P, _I64, _I64, _I64, _I64, _P, _P, _I32, _P, _P, _SZ, _P]),
+    "gmmxx_group_tiles_len": (_I64, [_I64, _I64]),
+    "gmmxx_group_rows_workspace_bytes": (_SZ, [_I64, _I64]),
+    "gmmxx_group_rows": (_I32, [_P, _I32, _I64, _I64, _P, _P, _P, _P, _SZ, _P]),
+    "gmmxx_grouped_matmul_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64, _I64, _I64]),
+    "gmmxx_grouped_matmul": (_I32, [_I32, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I32, _P, _P, _P, _SZ,
+                                    _P]),
+    "gmmxx_grouped_matmul_backward_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64, _I64, _I64]),
+    "gmmxx_grouped_matmul_backward": (_I32, [_I32, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I32, _P, _P,
+                                             _P, _P, _SZ, _P]),
+    "gmmxx_orthogonalize_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64]),
+    "gmmxx_orthogonalize": (_I32, [_I32, _P, _I64, _I64, _I64, _I32, _F, _F, _F, _F, _P, _P, _SZ, _P]),
 }
 
 
@@ -182,3 +193,33 @@ def label_stats_width(mode: int, d: int) -> int:
 
 def label_stats_workspace_bytes(mode: int, b: int, n: int, d: int, k: int) -> int:
     return int(load().gmmxx_label_stats_workspace_bytes(mode, b, n, d, k))
+
+
+def _size(name: str, *args) -> int:
+    """A size the library computes; 0 / -1 means that it refuses the sizes."""
+    lib = load()
+    v = int(getattr(lib, name)(*args))
+    if v <= 0:
+        msg = lib.gmmxx_last_error().decode("utf-8", "replace")
+        raise UnsupportedShape(ERR_UNSUPPORTED, f"{name}: {msg}")
+    return v
+
+
+def group_tiles_len(slots: int, k: int) -> int:
+    return _size("gmmxx_group_tiles_len", slots, k)
+
+
+def group_rows_workspace_bytes(slots: int, k: int) -> int:
+    return _size("gmmxx_group_rows_workspace_bytes", slots, k)
+
+
+def grouped_matmul_workspace_bytes(dt: int, rows: int, top: int, k: int, n_in: int, n_out: int) -> int:
+    return _size("gmmxx_grouped_matmul_workspace_bytes", dt, rows, top, k, n_in, n_out)
+
+
+def grouped_matmul_backward_workspace_bytes(dt: int, rows: int, top: int, k: int, n_in: int, n_out: int) -> int:
+    return _size("gmmxx_grouped_matmul_backward_workspace_bytes", dt, rows, top, k, n_in, n_out)
+
+
+def orthogonalize_workspace_bytes(dt: int, batch: int, m: int, n: int) -> int:
+    return _size("gmmxx_orthogonalize_workspace_bytes", dt, batch, m, n)

@@ -1,0 +1,58 @@
+// experts_api.cuh -- what the routed-product sources share: the row-tile table
+// and the launchers behind the C entry points (experts_capi.cu).
+#pragma once
+
+#include "gmm_common.cuh"
+
+namespace gmmxx {
+namespace experts {
+
+constexpr int kTileRows = 128;   // rows of one tile: the M extent of a tcgen05 tile
+constexpr int kTileHeader = 4;   // tiles[0]: number of tiles
+constexpr int kTileInts = 3;     // per tile: group, first position in the sorted order, rows
+constexpr int64_t kMaxGroups = 32768;
+
+// the routed rows of one call
+struct Groups {
+  const int32_t* order;    // [slots] position -> slot
+  const int32_t* offsets;  // [K + 1]
+  const int32_t* tiles;
+  int64_t rows;
+  int top;
+  int K;
+  int64_t slots() const { return rows * top; }
+  int64_t max_tiles() const { return slots() / kTileRows + (K + 1 < slots() ? K + 1 : slots()); }
+};
+
+int64_t tiles_len(int64_t slots, int64_t K);
+size_t group_rows_ws(int64_t slots, int64_t K);
+int launch_group_rows(const void* labels, int wide, int64_t slots, int64_t K, int32_t* order, int32_t* offsets,
+                      int32_t* tiles, char* ws, cudaStream_t st);
+
+// dtype-generic store, rounded to nearest
+__device__ __forceinline__ void store_y(void* p, int64_t i, int dt, float v) {
+  if (dt == GMMXX_FLOAT32) static_cast<float*>(p)[i] = v;
+  else if (dt == GMMXX_BFLOAT16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+inline int allow_smem(const void* kern, int bytes) {
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "kernel attributes: %s", cudaGetErrorString(e));
+  return GMMXX_OK;
+}
+
+inline int64_t elem_bytes(int dt) { return dt == GMMXX_FLOAT32 ? 4 : 2; }
+
+size_t grouped_matmul_ws(int dt, const Groups& g, int64_t n_in, int64_t n_out);
+int launch_grouped_matmul(int dt, const void* x, const Groups& g, int64_t n_in, int64_t n_out, const void* w, int wt,
+                          const void* bias, void* out, char* ws, cudaStream_t st);
+size_t grouped_backward_ws(int dt, const Groups& g, int64_t n_in, int64_t n_out);
+int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups& g, int64_t n_in, int64_t n_out,
+                            const void* w, int wt, void* gx, void* gw, void* gb, char* ws, cudaStream_t st);
+size_t orthogonalize_ws(int dt, int64_t batch, int64_t m, int64_t n);
+int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_t n, int steps, float a, float b,
+                         float c, float eps, void* q, char* ws, cudaStream_t st);
+
+}  // namespace experts
+}  // namespace gmmxx

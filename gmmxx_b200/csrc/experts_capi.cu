@@ -1,0 +1,171 @@
+// experts_capi.cu -- the extern "C" boundary of the routed products
+// (include/gmmxx_b200.h): argument validation before any CUDA call.
+#include "experts_api.cuh"
+
+#include <math.h>
+
+using namespace gmmxx;
+
+namespace {
+
+int check_dtype(int dt) {
+  if (dt < GMMXX_FLOAT32 || dt > GMMXX_FLOAT16) return set_error(GMMXX_ERR_INVALID, "unknown dtype %d", dt);
+  return GMMXX_OK;
+}
+
+int check_groups(int64_t slots, int64_t K) {
+  if (slots < 0 || K <= 0) return set_error(GMMXX_ERR_INVALID, "bad sizes slots=%lld K=%lld", (long long)slots, (long long)K);
+  if (slots >= (1ll << 31)) return set_error(GMMXX_ERR_UNSUPPORTED, "%lld slots: positions are 32-bit", (long long)slots);
+  if (K > experts::kMaxGroups)
+    return set_error(GMMXX_ERR_UNSUPPORTED, "K=%lld exceeds the routing window (<= %lld)", (long long)K,
+                     (long long)experts::kMaxGroups);
+  return GMMXX_OK;
+}
+
+int check_products(int dt, int64_t rows, int64_t top, int64_t K, int64_t n_in, int64_t n_out) {
+  if (int rc = check_dtype(dt)) return rc;
+  if (rows < 0 || top <= 0 || n_in <= 0 || n_out <= 0)
+    return set_error(GMMXX_ERR_INVALID, "bad sizes rows=%lld top_k=%lld n_in=%lld n_out=%lld", (long long)rows,
+                     (long long)top, (long long)n_in, (long long)n_out);
+  if (n_in > (1 << 20) || n_out > (1 << 20) || top > (1 << 16))
+    return set_error(GMMXX_ERR_UNSUPPORTED, "n_in=%lld n_out=%lld top_k=%lld exceed the product window",
+                     (long long)n_in, (long long)n_out, (long long)top);
+  if (rows > (1ll << 31)) return set_error(GMMXX_ERR_UNSUPPORTED, "%lld rows: positions are 32-bit", (long long)rows);
+  return check_groups(rows * top, K);
+}
+
+int check_ws(const void* ws, size_t bytes, size_t need) {
+  if (ws == nullptr) return set_error(GMMXX_ERR_INVALID, "workspace is NULL");
+  if ((reinterpret_cast<uintptr_t>(ws) & 255) != 0) return set_error(GMMXX_ERR_INVALID, "workspace must be 256-byte aligned");
+  if (bytes < need)
+    return set_error(GMMXX_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %zu bytes required", bytes, need);
+  return GMMXX_OK;
+}
+
+#define GMMXX_REQUIRE(p, name) \
+  if ((p) == nullptr) return set_error(GMMXX_ERR_INVALID, "%s is NULL", name)
+
+experts::Groups make_groups(int64_t rows, int64_t top, int64_t K, const int32_t* order, const int32_t* offsets,
+                            const int32_t* tiles) {
+  experts::Groups g{};
+  g.order = order;
+  g.offsets = offsets;
+  g.tiles = tiles;
+  g.rows = rows;
+  g.top = (int)top;
+  g.K = (int)K;
+  return g;
+}
+
+int check_matrices(int dt, int64_t batch, int64_t m, int64_t n) {
+  if (int rc = check_dtype(dt)) return rc;
+  if (batch < 0 || m <= 0 || n <= 0)
+    return set_error(GMMXX_ERR_INVALID, "bad sizes batch=%lld m=%lld n=%lld", (long long)batch, (long long)m, (long long)n);
+  if (m > (1 << 16) || n > (1 << 16) || batch > (1 << 20))
+    return set_error(GMMXX_ERR_UNSUPPORTED, "batch=%lld m=%lld n=%lld exceed the window (2^20, 2^16, 2^16)",
+                     (long long)batch, (long long)m, (long long)n);
+  return GMMXX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t gmmxx_group_tiles_len(int64_t slots, int64_t K) {
+  if (check_groups(slots, K)) return -1;
+  return experts::tiles_len(slots, K);
+}
+
+size_t gmmxx_group_rows_workspace_bytes(int64_t slots, int64_t K) {
+  if (check_groups(slots, K)) return 0;
+  return experts::group_rows_ws(slots, K);
+}
+
+int gmmxx_group_rows(const void* labels, int label_bytes, int64_t slots, int64_t K, int32_t* order_out,
+                     int32_t* offsets_out, int32_t* tiles_out, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_groups(slots, K)) return rc;
+  if (label_bytes != 4 && label_bytes != 8)
+    return set_error(GMMXX_ERR_INVALID, "labels must be int32 or int64 (label_bytes 4 or 8, got %d)", label_bytes);
+  if (slots > 0) {
+    GMMXX_REQUIRE(labels, "labels");
+    GMMXX_REQUIRE(order_out, "order_out");
+  }
+  GMMXX_REQUIRE(offsets_out, "offsets_out");
+  GMMXX_REQUIRE(tiles_out, "tiles_out");
+  if (int rc = check_ws(workspace, workspace_bytes, experts::group_rows_ws(slots, K))) return rc;
+  return experts::launch_group_rows(labels, label_bytes == 8, slots, K, order_out, offsets_out, tiles_out,
+                                    static_cast<char*>(workspace), static_cast<cudaStream_t>(stream));
+}
+
+size_t gmmxx_grouped_matmul_workspace_bytes(int dtype, int64_t rows, int64_t top_k, int64_t K, int64_t n_in,
+                                            int64_t n_out) {
+  if (check_products(dtype, rows, top_k, K, n_in, n_out)) return 0;
+  return experts::grouped_matmul_ws(dtype, make_groups(rows, top_k, K, nullptr, nullptr, nullptr), n_in, n_out);
+}
+
+int gmmxx_grouped_matmul(int dtype, const void* x, int64_t rows, int64_t top_k, int64_t K, int64_t n_in, int64_t n_out,
+                         const int32_t* order, const int32_t* offsets, const int32_t* tiles, const void* weight,
+                         int weight_transposed, const void* bias, void* out, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  if (int rc = check_products(dtype, rows, top_k, K, n_in, n_out)) return rc;
+  if (rows == 0) return GMMXX_OK;
+  GMMXX_REQUIRE(x, "x");
+  GMMXX_REQUIRE(order, "order");
+  GMMXX_REQUIRE(offsets, "offsets");
+  GMMXX_REQUIRE(tiles, "tiles");
+  GMMXX_REQUIRE(weight, "weight");
+  GMMXX_REQUIRE(out, "out");
+  const experts::Groups g = make_groups(rows, top_k, K, order, offsets, tiles);
+  if (int rc = check_ws(workspace, workspace_bytes, experts::grouped_matmul_ws(dtype, g, n_in, n_out))) return rc;
+  return experts::launch_grouped_matmul(dtype, x, g, n_in, n_out, weight, weight_transposed != 0, bias, out,
+                                        static_cast<char*>(workspace), static_cast<cudaStream_t>(stream));
+}
+
+size_t gmmxx_grouped_matmul_backward_workspace_bytes(int dtype, int64_t rows, int64_t top_k, int64_t K, int64_t n_in,
+                                                     int64_t n_out) {
+  if (check_products(dtype, rows, top_k, K, n_in, n_out)) return 0;
+  return experts::grouped_backward_ws(dtype, make_groups(rows, top_k, K, nullptr, nullptr, nullptr), n_in, n_out);
+}
+
+int gmmxx_grouped_matmul_backward(int dtype, const void* grad_out, const void* x, int64_t rows, int64_t top_k,
+                                  int64_t K, int64_t n_in, int64_t n_out, const int32_t* order, const int32_t* offsets,
+                                  const int32_t* tiles, const void* weight, int weight_transposed, void* grad_x,
+                                  void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  if (int rc = check_products(dtype, rows, top_k, K, n_in, n_out)) return rc;
+  if (grad_x == nullptr && grad_weight == nullptr && grad_bias == nullptr) return GMMXX_OK;
+  if (rows > 0) {
+    GMMXX_REQUIRE(grad_out, "grad_out");
+    GMMXX_REQUIRE(order, "order");
+    GMMXX_REQUIRE(tiles, "tiles");
+    if (grad_x != nullptr) GMMXX_REQUIRE(weight, "weight");
+    if (grad_weight != nullptr) GMMXX_REQUIRE(x, "x");
+  }
+  GMMXX_REQUIRE(offsets, "offsets");
+  const experts::Groups g = make_groups(rows, top_k, K, order, offsets, tiles);
+  if (int rc = check_ws(workspace, workspace_bytes, experts::grouped_backward_ws(dtype, g, n_in, n_out))) return rc;
+  return experts::launch_grouped_backward(dtype, grad_out, x, g, n_in, n_out, weight, weight_transposed != 0, grad_x,
+                                          grad_weight, grad_bias, static_cast<char*>(workspace),
+                                          static_cast<cudaStream_t>(stream));
+}
+
+size_t gmmxx_orthogonalize_workspace_bytes(int dtype, int64_t batch, int64_t m, int64_t n) {
+  if (check_matrices(dtype, batch, m, n)) return 0;
+  return experts::orthogonalize_ws(dtype, batch, m, n);
+}
+
+int gmmxx_orthogonalize(int dtype, const void* g, int64_t batch, int64_t m, int64_t n, int steps, float a, float b,
+                        float c, float eps, void* q, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_matrices(dtype, batch, m, n)) return rc;
+  if (steps < 0 || steps > 100) return set_error(GMMXX_ERR_INVALID, "steps must be in [0, 100], got %d", steps);
+  if (!isfinite(a) || !isfinite(b) || !isfinite(c)) return set_error(GMMXX_ERR_INVALID, "coefficients must be finite");
+  if (!(eps >= 0.f) || !isfinite(eps)) return set_error(GMMXX_ERR_INVALID, "eps must be finite and not negative");
+  if (batch == 0) return GMMXX_OK;
+  GMMXX_REQUIRE(g, "g");
+  GMMXX_REQUIRE(q, "q");
+  if (int rc = check_ws(workspace, workspace_bytes, experts::orthogonalize_ws(dtype, batch, m, n))) return rc;
+  return experts::launch_orthogonalize(dtype, g, batch, m, n, steps, a, b, c, eps, q, static_cast<char*>(workspace),
+                                       static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,255 @@
+"""Products of rows with their component's matrix: routing, forward,
+gradients, and the orthogonalisation of the learned matrices.
+
+A mixture answers with a component per row (``predict``, ``*_assign``) or a
+few (the largest of ``predict_proba``).  These operators do the work that
+follows per component -- a rotation, whitening or linear map of each
+component's own, mixtures of linear experts with the mixture as their router:
+
+* :func:`group_rows` sorts the rows by component on the device, without a host
+  synchronisation, into a :class:`RowGroups` that the products take;
+* :func:`grouped_matmul` multiplies each row with its component's matrix,
+  :func:`grouped_matmul_backward` gives the gradients of rows, matrices and
+  biases;
+* :func:`orthogonalize` runs the Newton-Schulz iteration on a stack of
+  matrices (the per-component rotation nearest to a correlation, the
+  orthogonalised update of an expert).
+
+Like the operators of ``cuda_ops`` they take CUDA tensors (``ValueError``
+otherwise; non-contiguous ones are copied), run on the current stream of the
+tensors' device, never synchronise, can be captured into a CUDA graph and
+give the same bits on every run.  Sums are held in fp32 or more whatever the
+type.  They compute values, not autograd nodes: an input that requires grad is
+refused while gradients are enabled (call them under ``torch.no_grad()`` and
+chain with :func:`grouped_matmul_backward`).
+"""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Optional, Sequence, Tuple
+
+import torch
+
+from . import _native as nat
+from . import engine
+from .cuda_ops import _check_input, require_cuda
+
+# Muon's quintic: a x + b x^3 + c x^5 lifts every singular value in (0, 1] towards 1
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+class RowGroups(NamedTuple):
+    """Slots sorted by component (:func:`group_rows`).  A slot is one (row,
+    choice) pair, ``row * top_k + choice``."""
+
+    order: torch.Tensor  # (slots,) int32: slots by component, unassigned ones last
+    offsets: torch.Tensor  # (n_groups + 1,) int32: group k is order[offsets[k]:offsets[k + 1]]
+    tiles: torch.Tensor  # the product kernels' table of row tiles
+    n_rows: int
+    top_k: int
+    n_groups: int
+    shape: Tuple[int, ...]  # of the labels: (N,) or (N, top_k)
+
+
+def _check(t, name: str, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires grad: this operator records no autograd node (use torch.no_grad() and "
+                         "grouped_matmul_backward)")
+    return _check_input(t, name, dtype=dtype)
+
+
+def _check_float(t, name: str) -> torch.Tensor:
+    t = _check(t, name)
+    if t.dtype not in engine._X_DTYPES:
+        raise TypeError(f"{name} dtype {t.dtype} not supported (float32, bfloat16, float16)")
+    return t
+
+
+def _same_device(dev: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+
+
+def _workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
+    # of its own per call, from the caching allocator: calls on several streams
+    # and captured graphs never share one
+    return torch.empty(max(256, nbytes), dtype=torch.uint8, device=dev)
+
+
+def group_rows(labels: torch.Tensor, n_groups: int) -> RowGroups:
+    """Sort rows by the component they are assigned to.
+
+    ``labels`` (N,) or (N, top_k), int32 or int64, as ``predict`` / ``*_assign``
+    give them.  A label outside ``[0, n_groups)`` (for instance -1) leaves its
+    slot unassigned.  Within a component the slots keep their order."""
+    require_cuda()
+    labels = _check(labels, "labels")
+    if labels.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"labels: dtype must be torch.int32 or torch.int64, got {labels.dtype}")
+    if labels.ndim not in (1, 2):
+        raise ValueError("labels must have shape (N,) or (N, top_k)")
+    n_groups = int(n_groups)
+    if n_groups <= 0:
+        raise ValueError("n_groups must be positive")
+    top = 1 if labels.ndim == 1 else labels.shape[1]
+    if top == 0:
+        raise ValueError("labels must have at least one choice per row")
+    slots, dev = labels.numel(), labels.device
+    tiles_len = nat.group_tiles_len(slots, n_groups)
+    order = torch.empty((slots,), dtype=torch.int32, device=dev)
+    offsets = torch.empty((n_groups + 1,), dtype=torch.int32, device=dev)
+    tiles = torch.empty((tiles_len,), dtype=torch.int32, device=dev)
+    ws = _workspace(nat.group_rows_workspace_bytes(slots, n_groups), dev)
+    with torch.cuda.device(dev):
+        nat.call("gmmxx_group_rows", labels.data_ptr(), labels.element_size(), slots, n_groups, order.data_ptr(),
+                 offsets.data_ptr(), tiles.data_ptr(), ws.data_ptr(), ws.numel(), engine._stream_ptr(dev))
+    return RowGroups(order, offsets, tiles, labels.shape[0], top, n_groups, tuple(labels.shape))
+
+
+def _weight(weight: torch.Tensor, groups: RowGroups) -> Tuple[torch.Tensor, int]:
+    """(weight, 1 when its memory holds (K, n_out, n_in)): a transposed view, as
+    of stacked ``nn.Linear`` weights, is read in place."""
+    if not torch.is_tensor(weight):
+        raise TypeError("weight must be a torch.Tensor")
+    if weight.ndim != 3 or weight.shape[0] != groups.n_groups:
+        raise ValueError(f"weight must have shape ({groups.n_groups}, n_in, n_out), got {tuple(weight.shape)}")
+    if weight.shape[1] == 0 or weight.shape[2] == 0:
+        raise ValueError("weight must not be empty")
+    if not weight.is_contiguous() and weight.transpose(1, 2).is_contiguous():
+        return _check_float(weight.transpose(1, 2), "weight"), 1
+    return _check_float(weight, "weight"), 0
+
+
+def _check_groups(groups) -> RowGroups:
+    if not isinstance(groups, RowGroups):
+        raise TypeError("groups must be a RowGroups (group_rows)")
+    slots = groups.n_rows * groups.top_k
+    sizes = {"order": slots, "offsets": groups.n_groups + 1, "tiles": nat.group_tiles_len(slots, groups.n_groups)}
+    for name, size in sizes.items():
+        t = getattr(groups, name)
+        if t.dtype != torch.int32 or t.shape != (size,) or not t.is_contiguous() or t.device != groups.order.device:
+            raise ValueError(f"groups.{name} must be the int32 tensor that group_rows returned")
+    return groups
+
+
+def _rows(t, name: str, shape: Tuple[int, ...], like: torch.Tensor) -> torch.Tensor:
+    t = _check_float(t, name)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype != like.dtype:
+        raise ValueError(f"{name}: dtype must be {like.dtype}, got {t.dtype}")
+    return t
+
+
+def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups,
+                   bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Each row times its component's matrix: ``out[n, t] = x[n] @
+    weight[label[n, t]] + bias[label[n, t]]``, zeros where the slot is unassigned.
+
+    ``x`` (N, n_in), ``weight`` (K, n_in, n_out) (a transposed view of
+    (K, n_out, n_in) is read in place), ``bias`` (K, n_out), all float32,
+    bfloat16 or float16 alike; ``groups`` from :func:`group_rows` over the N
+    rows' labels.  Returns (N, n_out) for labels (N,), (N, top_k, n_out) for
+    labels (N, top_k), in x's type."""
+    require_cuda()
+    groups = _check_groups(groups)
+    w, wt = _weight(weight, groups)
+    k, n_in, n_out = weight.shape
+    x = _rows(x, "x", (groups.n_rows, n_in), w)
+    if bias is not None:
+        bias = _rows(bias, "bias", (k, n_out), w)
+    dev = x.device
+    _same_device(dev, weight=w, bias=bias, groups=groups.order)
+    dt = engine._X_DTYPES[x.dtype]
+    out = torch.empty((*groups.shape, n_out), dtype=x.dtype, device=dev)
+    ws = _workspace(nat.grouped_matmul_workspace_bytes(dt, groups.n_rows, groups.top_k, k, n_in, n_out), dev)
+    with torch.cuda.device(dev):
+        nat.call("gmmxx_grouped_matmul", dt, x.data_ptr(), groups.n_rows, groups.top_k, k, n_in, n_out,
+                 groups.order.data_ptr(), groups.offsets.data_ptr(), groups.tiles.data_ptr(), w.data_ptr(), wt,
+                 engine._p(bias), out.data_ptr(), ws.data_ptr(), ws.numel(), engine._stream_ptr(dev))
+    return out
+
+
+def grouped_matmul_backward(grad_out: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, *,
+                            bias: bool = False, need_x: bool = True, need_weight: bool = True):
+    """Gradients of :func:`grouped_matmul`: ``(grad_x, grad_weight, grad_bias)``
+    in x's type and the shapes (and, for a transposed weight, the memory order)
+    of x, weight and bias.  ``grad_out`` has the forward's output shape; rows of
+    unassigned slots do not count.  ``grad_x`` sums over a row's top_k slots.
+    ``need_x`` / ``need_weight`` False and ``bias`` False leave ``None`` in the
+    place.  A component without rows gets zeros."""
+    require_cuda()
+    groups = _check_groups(groups)
+    w, wt = _weight(weight, groups)
+    k, n_in, n_out = weight.shape
+    x = _rows(x, "x", (groups.n_rows, n_in), w)
+    grad_out = _rows(grad_out, "grad_out", (*groups.shape, n_out), w)
+    dev = x.device
+    _same_device(dev, weight=w, grad_out=grad_out, groups=groups.order)
+    dt = engine._X_DTYPES[x.dtype]
+    grad_x = torch.empty_like(x) if need_x else None
+    grad_w = torch.empty_like(w) if need_weight else None
+    grad_b = torch.empty((k, n_out), dtype=x.dtype, device=dev) if bias else None
+    ws = _workspace(nat.grouped_matmul_backward_workspace_bytes(dt, groups.n_rows, groups.top_k, k, n_in, n_out), dev)
+    with torch.cuda.device(dev):
+        nat.call("gmmxx_grouped_matmul_backward", dt, grad_out.data_ptr(), x.data_ptr(), groups.n_rows, groups.top_k,
+                 k, n_in, n_out, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.tiles.data_ptr(),
+                 w.data_ptr(), wt, engine._p(grad_x), engine._p(grad_w), engine._p(grad_b), ws.data_ptr(),
+                 ws.numel(), engine._stream_ptr(dev))
+    if grad_w is not None and wt:
+        grad_w = grad_w.transpose(1, 2)
+    return grad_x, grad_w, grad_b
+
+
+def _check_polynomial(a: float, b: float, c: float, steps: int) -> None:
+    """Refuse coefficients that carry a singular value of [0, 1] beyond what the
+    kernels' 16-bit planes hold: with |X|_F <= 1 at the start, the iterates'
+    singular values are those of the scalar polynomial."""
+    if not all(math.isfinite(v) for v in (a, b, c)):
+        raise ValueError("coefficients must be finite")
+    top = 1.0
+    for _ in range(steps):
+        # |a s + b s^3 + c s^5| over [0, top], and the products on the way
+        grid = [top * i / 512.0 for i in range(513)]
+        inner = max(abs(b * s * s + c * s**4) for s in grid)
+        top = max(abs(a * s + b * s**3 + c * s**5) for s in grid)
+        if top > 2.0 or inner > 8.0:
+            raise ValueError("coefficients make the iteration diverge: a singular value of [0, 1] leaves [-2, 2]")
+
+
+def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients: Sequence[float] = NEWTON_SCHULZ,
+                  eps: float = 1e-7) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of each matrix of ``g`` (..., m, n),
+    float32, bfloat16 or float16: ``X = g / (|g|_F + eps)``, then ``steps``
+    times ``X <- a X + (b P + c P^2) X`` with ``P = X X^T`` (over the shorter
+    side), which drives every singular value towards 1 and leaves the singular
+    vectors.  The default coefficients are Muon's.  Returns the type of ``g``."""
+    require_cuda()
+    g = _check_float(g, "g")
+    if g.ndim < 2 or g.shape[-1] == 0 or g.shape[-2] == 0:
+        raise ValueError("g must have shape (..., m, n) with m, n > 0")
+    steps = int(steps)
+    if steps < 0 or steps > 100:
+        raise ValueError("steps must be in [0, 100]")
+    if len(coefficients) != 3:
+        raise ValueError("coefficients must be three numbers (a, b, c)")
+    a, b, c = (float(v) for v in coefficients)
+    _check_polynomial(a, b, c, steps)
+    eps = float(eps)
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError("eps must be finite and not negative")
+    m, n = g.shape[-2:]
+    batch = math.prod(g.shape[:-2])
+    q = torch.empty_like(g)
+    if batch == 0:
+        return q
+    dev, dt = g.device, engine._X_DTYPES[g.dtype]
+    ws = _workspace(nat.orthogonalize_workspace_bytes(dt, batch, m, n), dev)
+    with torch.cuda.device(dev):
+        nat.call("gmmxx_orthogonalize", dt, g.data_ptr(), batch, m, n, steps, a, b, c, eps, q.data_ptr(),
+                 ws.data_ptr(), ws.numel(), engine._stream_ptr(dev))
+    return q

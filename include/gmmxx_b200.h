@@ -271,6 +271,57 @@ GMMXX_API int gmmxx_label_stats(int x_dtype, const void* x, int64_t B, int64_t N
                                 const int64_t* labels, const float* means, int mode, float* stats_out,
                                 void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- products of rows with their component's matrix ------------------------
+ * Rows are routed to components by labels (one label per row, as gmmxx_assign
+ * writes them, or top_k labels per row); a *slot* is one (row, choice) pair,
+ * slot = row * top_k + choice.  gmmxx_group_rows sorts the slots by component;
+ * the products take its order / offsets / tiles.  dtype is the type of x,
+ * weight, bias, gradients and outputs (gmmxx_dtype); sums are fp32.
+ *
+ * gmmxx_group_rows: labels (slots) int32 or int64 (label_bytes 4 / 8); a label
+ *   outside [0, K) leaves its slot unassigned.  order_out (slots): the slots
+ *   sorted by label, equal labels in slot order, unassigned slots last.
+ *   offsets_out (K + 1): group k is order[offsets[k] .. offsets[k + 1]).
+ *   tiles_out: gmmxx_group_tiles_len(slots, K) int32, the table of row tiles
+ *   that the product kernels walk (opaque).  slots < 2^31, 1 <= K <= 32768. */
+GMMXX_API int64_t gmmxx_group_tiles_len(int64_t slots, int64_t K);
+GMMXX_API size_t gmmxx_group_rows_workspace_bytes(int64_t slots, int64_t K);
+GMMXX_API int gmmxx_group_rows(const void* labels, int label_bytes, int64_t slots, int64_t K, int32_t* order_out,
+                               int32_t* offsets_out, int32_t* tiles_out, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/* out[slot] = x[row] W[k] + bias[k] for the component k of the slot, 0 for an
+ * unassigned slot.  x (rows, n_in); weight (K, n_in, n_out), or (K, n_out, n_in)
+ * with weight_transposed; bias (K, n_out) or NULL; out (rows * top_k, n_out). */
+GMMXX_API size_t gmmxx_grouped_matmul_workspace_bytes(int dtype, int64_t rows, int64_t top_k, int64_t K, int64_t n_in,
+                                                      int64_t n_out);
+GMMXX_API int gmmxx_grouped_matmul(int dtype, const void* x, int64_t rows, int64_t top_k, int64_t K, int64_t n_in,
+                                   int64_t n_out, const int32_t* order, const int32_t* offsets, const int32_t* tiles,
+                                   const void* weight, int weight_transposed, const void* bias, void* out,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of gmmxx_grouped_matmul for grad_out (rows * top_k, n_out):
+ * grad_x (rows, n_in) = sum over the row's slots of grad_out W^T; grad_weight
+ * (in the weight's layout) = sum over the group's slots of x^T grad_out;
+ * grad_bias (K, n_out) = sum over the group's slots of grad_out.  Each of the
+ * three may be NULL (not computed).  A component without rows gets zeros. */
+GMMXX_API size_t gmmxx_grouped_matmul_backward_workspace_bytes(int dtype, int64_t rows, int64_t top_k, int64_t K,
+                                                               int64_t n_in, int64_t n_out);
+GMMXX_API int gmmxx_grouped_matmul_backward(int dtype, const void* grad_out, const void* x, int64_t rows,
+                                            int64_t top_k, int64_t K, int64_t n_in, int64_t n_out,
+                                            const int32_t* order, const int32_t* offsets, const int32_t* tiles,
+                                            const void* weight, int weight_transposed, void* grad_x,
+                                            void* grad_weight, void* grad_bias, void* workspace,
+                                            size_t workspace_bytes, void* stream);
+
+/* Newton-Schulz orthogonalisation of a stack of matrices g (batch, m, n):
+ * X = g / (|g|_F + eps), then `steps` times X <- a X + (b P + c P^2) X with
+ * P = X X^T (m <= n; X^T X on the right for m > n); q (batch, m, n) = X. */
+GMMXX_API size_t gmmxx_orthogonalize_workspace_bytes(int dtype, int64_t batch, int64_t m, int64_t n);
+GMMXX_API int gmmxx_orthogonalize(int dtype, const void* g, int64_t batch, int64_t m, int64_t n, int steps, float a,
+                                  float b, float c, float eps, void* q, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
