@@ -1,240 +1,574 @@
-// experts.cu -- products of rows with their component's matrix, their
-// gradients, and the Newton-Schulz iteration, on the CUDA cores: 64 x 64 tiles,
-// fp32 sums, one row tile per block, every type and size.
-#include "experts_api.cuh"
+// experts.cu -- the routed products and the Newton-Schulz iteration: operand
+// preparation, launch sequences and the small kernels around the tensor-core
+// product kernel (experts_tc.cu).
+#include "experts_tc.cuh"
+
+#include <algorithm>
 
 namespace gmmxx {
 namespace experts {
 namespace {
 
-constexpr int kT = 64, kKc = 16;
+inline int64_t al256(int64_t v) { return round_up(v, 256); }
+inline int64_t pad8(int64_t v) { return round_up(v, 8); }
 
-struct Tile {
-  float a[kKc][kT + 4];
-  float b[kKc][kT + 4];
+// ---------------------------------------------------------------------------
+// operands
+// ---------------------------------------------------------------------------
+
+// A 16-bit matrix whose rows are multiples of 16 bytes is read by TMA where it
+// lies; any other type or row length is first laid out as planes of padded rows.
+bool direct(int dt, int64_t cols) { return dt != GMMXX_FLOAT32 && cols % 8 == 0; }
+int planes_of(int dt) { return dt == GMMXX_FLOAT32 ? 3 : 1; }
+int64_t pack_bytes(int dt, int64_t rows, int64_t cols) {
+  return direct(dt, cols) ? 0 : al256(rows * pad8(cols) * 2) * planes_of(dt);
+}
+
+// x = x0 + x1 + x2 exactly, each the leading 8 bits of what is left (cut, not
+// rounded, so that no plane overflows).  Infinity and NaN stay in x0.
+__device__ __forceinline__ void split3(float x, uint32_t* h) {
+  const uint32_t b = __float_as_uint(x);
+  if ((b & 0x7f800000u) == 0x7f800000u) {
+    h[0] = (b >> 16) | ((b & 0xffffu) ? 0x40u : 0u);  // a NaN keeps a mantissa bit
+    h[1] = h[2] = 0;
+    return;
+  }
+  h[0] = b >> 16;
+  const float r = x - __uint_as_float(b & 0xffff0000u);
+  const uint32_t rb = __float_as_uint(r);
+  h[1] = rb >> 16;
+  h[2] = __float_as_uint(r - __uint_as_float(rb & 0xffff0000u)) >> 16;
+}
+
+// [rows][cols] of any type -> 1 plane (16-bit types, copied) or 3 (fp32) of rows of ld elements
+__global__ void __launch_bounds__(256) pack_kernel(const void* src, int f32, int64_t rows, int cols, int ld,
+                                                   uint16_t* dst, int64_t plane) {
+  const int per = ld / 8;
+  const int64_t n = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per;
+    const int c = (int)(i % per) * 8;
+    const int64_t at = r * cols + c;
+    uint32_t q[3][4] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t h[3] = {0, 0, 0};
+      if (c + j < cols) {
+        if (f32) split3(static_cast<const float*>(src)[at + j], h);
+        else h[0] = static_cast<const uint16_t*>(src)[at + j];
+      }
+#pragma unroll
+      for (int p = 0; p < 3; ++p) q[p][j >> 1] |= h[p] << ((j & 1) * 16);
+    }
+    const int np = f32 ? 3 : 1;
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+      if (p < np)
+        *reinterpret_cast<uint4*>(dst + p * plane + r * ld + c) = make_uint4(q[p][0], q[p][1], q[p][2], q[p][3]);
+  }
+}
+
+struct Planes {
+  const void* base[3];
+  int64_t ld;
+  int n;
+  int fp16;
 };
 
-__device__ __forceinline__ void tile_fma(const Tile& t, float acc[4][4]) {
-  const int tr = threadIdx.x >> 4, tc = threadIdx.x & 15;
-#pragma unroll
-  for (int kk = 0; kk < kKc; ++kk)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(t.a[kk][tr * 4 + i], t.b[kk][tc * 4 + j], acc[i][j]);
-}
-
-// out[slot] = x[slot / div] . W[k] (+ bias[k]); w_in / w_out: element strides
-__global__ void __launch_bounds__(256) rows_kernel(int dt, const void* x, int div, Groups g, int n_in, int n_out,
-                                                   const void* w, int64_t w_in, int64_t w_out, const void* bias,
-                                                   void* out, int out_dt) {
-  __shared__ Tile t;
-  const int tile = blockIdx.x >> 1;
-  if (tile >= g.tiles[0]) return;
-  const int32_t* e = g.tiles + kTileHeader + (int64_t)tile * kTileInts;
-  const int k = e[0], pos = e[1] + (blockIdx.x & 1) * kT, n = e[2] - (blockIdx.x & 1) * kT;
-  if (n <= 0) return;
-  const int c0 = blockIdx.y * kT;
-  const int64_t wk = (int64_t)k * n_in * n_out;
-  float acc[4][4] = {};
-  if (k < g.K)
-    for (int i0 = 0; i0 < n_in; i0 += kKc) {
-      for (int i = threadIdx.x; i < kT * kKc; i += 256) {
-        const int r = i / kKc, kk = i % kKc;
-        t.a[kk][r] = r < n && i0 + kk < n_in ? load_x(x, (int64_t)(g.order[pos + r] / div) * n_in + i0 + kk, dt) : 0.f;
-        const int c = i % kT, kb = i / kT;
-        t.b[kb][c] = c0 + c < n_out && i0 + kb < n_in ? load_x(w, wk + (i0 + kb) * w_in + (c0 + c) * w_out, dt) : 0.f;
-      }
-      __syncthreads();
-      tile_fma(t, acc);
-      __syncthreads();
-    }
-  const int tr = threadIdx.x >> 4, tc = threadIdx.x & 15;
-  for (int i = 0; i < 4; ++i) {
-    if (tr * 4 + i >= n) continue;
-    const int64_t slot = g.order[pos + tr * 4 + i];
-    for (int j = 0; j < 4; ++j) {
-      const int c = c0 + tc * 4 + j;
-      if (c >= n_out) continue;
-      float v = acc[i][j];
-      if (bias != nullptr && k < g.K) v += load_x(bias, (int64_t)k * n_out + c, dt);
-      store_y(out, slot * n_out + c, out_dt, v);
-    }
+int operand(int dt, const void* src, int64_t rows, int64_t cols, char*& ws, Planes* out, cudaStream_t st) {
+  out->fp16 = dt == GMMXX_FLOAT16;
+  out->n = planes_of(dt);
+  if (direct(dt, cols)) {
+    out->base[0] = src;
+    out->ld = cols;
+    return GMMXX_OK;
   }
+  out->ld = pad8(cols);
+  const int64_t plane = al256(rows * out->ld * 2);
+  for (int p = 0; p < out->n; ++p) out->base[p] = ws + p * plane;
+  const int64_t blocks = std::min<int64_t>(148 * 16, ceil_div(rows * out->ld / 8, 256));
+  if (blocks > 0)
+    pack_kernel<<<(unsigned)blocks, 256, 0, st>>>(src, dt == GMMXX_FLOAT32, rows, (int)cols, (int)out->ld,
+                                                  reinterpret_cast<uint16_t*>(ws), plane / 2);
+  ws += plane * out->n;
+  return check_launch("pack_kernel");
 }
 
-// gw[k] = sum over the group's slots of x^T gy
-__global__ void __launch_bounds__(256) weight_kernel(int dt, const void* x, const void* gy, Groups g, int n_in,
-                                                     int n_out, void* gw, int64_t w_in, int64_t w_out) {
-  __shared__ Tile t;
-  const int k = blockIdx.z, r0 = blockIdx.x * kT, c0 = blockIdx.y * kT;
-  const int p0 = g.offsets[k], p1 = g.offsets[k + 1];
-  float acc[4][4] = {};
-  for (int p = p0; p < p1; p += kKc) {
-    for (int i = threadIdx.x; i < kT * kKc; i += 256) {
-      const int c = i % kT, kk = i / kT;
-      const bool in = p + kk < p1;
-      const int64_t slot = in ? g.order[p + kk] : 0;
-      t.a[kk][c] = in && r0 + c < n_in ? load_x(x, slot / g.top * n_in + r0 + c, dt) : 0.f;
-      t.b[kk][c] = in && c0 + c < n_out ? load_x(gy, slot * n_out + c0 + c, dt) : 0.f;
-    }
-    __syncthreads();
-    tile_fma(t, acc);
-    __syncthreads();
-  }
-  const int tr = threadIdx.x >> 4, tc = threadIdx.x & 15;
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int r = r0 + tr * 4 + i, c = c0 + tc * 4 + j;
-      if (r < n_in && c < n_out) store_y(gw, (int64_t)k * n_in * n_out + r * w_in + c * w_out, dt, acc[i][j]);
-    }
+int rows_maps(const Planes& p, int64_t cols, int64_t rows, CUtensorMap* maps) {
+  for (int i = 0; i < p.n; ++i)
+    if (int rc = encode_rows(&maps[i], p.base[i], p.fp16, cols, rows, p.ld)) return rc;
+  return GMMXX_OK;
 }
 
-__global__ void bias_kernel(int dt, const void* gy, Groups g, int n_out, void* gb) {
-  const int k = blockIdx.y, c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= n_out) return;
-  float s = 0.f;
-  for (int p = g.offsets[k]; p < g.offsets[k + 1]; ++p) s += load_x(gy, (int64_t)g.order[p] * n_out + c, dt);
-  store_y(gb, (int64_t)k * n_out + c, dt, s);
+int stack_maps(const Planes& p, int64_t cols, int64_t rows, int64_t stack, int box_rows, CUtensorMap* maps) {
+  for (int i = 0; i < p.n; ++i)
+    if (int rc = encode_stack(&maps[i], p.base[i], p.fp16, cols, rows, p.ld, stack, rows * p.ld, box_rows)) return rc;
+  return GMMXX_OK;
+}
+
+// Tile columns: the widest tile that still gives every SM one (wider tiles
+// read fewer operand bytes per product; narrower ones spread short work).
+// Three planes of 256 columns would leave a single stage.
+int tile_columns(int64_t row_tiles, int64_t n, int planes, int max_bn) {
+  int bn = planes == 1 ? 256 : 128;
+  bn = std::min(bn, max_bn);
+  while (bn > 64 && (n <= bn / 2 || row_tiles * ceil_div(n, bn) < 148)) bn /= 2;
+  return bn;
+}
+
+int elem_size(int dt) { return dt == GMMXX_FLOAT32 ? 4 : 2; }
+bool vec_ok(const void* p, int dt, int64_t ld) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * elem_size(dt)) % 16 == 0;
+}
+
+// ---------------------------------------------------------------------------
+// rows x their group's matrix
+// ---------------------------------------------------------------------------
+
+// out[slot] = src[slot / div] . W, W (K, k_dim, n) when !b_kmajor, (K, n, k_dim) when b_kmajor
+int rows_product(int dt, const Planes& src, int64_t src_rows, int div, const Groups& g, int64_t k_dim, int64_t n,
+                 const Planes& w, bool b_kmajor, const void* bias, void* out, int out_dt, cudaStream_t st) {
+  const int bn = tile_columns(ceil_div(g.slots(), kTileRows), n, src.n, 256);
+  ProductMaps maps;
+  if (int rc = rows_maps(src, k_dim, src_rows, maps.a)) return rc;
+  if (int rc = b_kmajor ? stack_maps(w, k_dim, n, g.K, bn, maps.b) : stack_maps(w, n, k_dim, g.K, kBlockK, maps.b))
+    return rc;
+  ProductArgs a{};
+  a.n = (int)n;
+  a.k = (int)k_dim;
+  a.bn = bn;
+  a.stages = product_stages(src.n, bn);
+  a.mt = 1;
+  a.nt = (int)ceil_div(n, bn);
+  a.b_mn = b_kmajor ? 0 : 1;
+  a.idesc = product_idesc(src.fp16, bn, 0, a.b_mn);
+  a.order = g.order;
+  a.table = g.tiles;
+  a.div_a = div;
+  a.div_b = 1;
+  a.groups = g.K;
+  a.out = out;
+  a.out_dt = out_dt;
+  a.ldo = n;
+  a.vec = vec_ok(out, out_dt, n);
+  a.bias = bias;
+  a.bias_dt = dt;
+  return launch_product(kRows, src.n, maps, a, g.max_tiles(), st);
 }
 
 // gx[row] = sum over the row's slots, rounded once
 __global__ void sum_slots_kernel(const float* part, int64_t rows, int top, int n, void* out, int dt) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= rows * n) return;
-  const int64_t row = i / n, c = i % n;
-  float s = 0.f;
-  for (int t = 0; t < top; ++t) s += part[(row * top + t) * n + c];
-  store_y(out, i, dt, s);
-}
-
-// d = alpha * (A or A^T) . (B or B^T) + beta * c for a batch; m x n x k, row-major fp32
-__global__ void __launch_bounds__(256) batch_kernel(const float* a, int at, const float* b, int bt, const float* c,
-                                                    float* d, int m, int n, int k, float alpha, float beta) {
-  __shared__ Tile t;
-  const int64_t z = blockIdx.z;
-  a += z * m * k;
-  b += z * n * k;
-  const int r0 = blockIdx.x * kT, c0 = blockIdx.y * kT;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < k; k0 += kKc) {
-    for (int i = threadIdx.x; i < kT * kKc; i += 256) {
-      const int r = i % kT, kk = i / kT;
-      const bool in = k0 + kk < k;
-      t.a[kk][r] = in && r0 + r < m ? a[at ? (int64_t)(k0 + kk) * m + r0 + r : (int64_t)(r0 + r) * k + k0 + kk] : 0.f;
-      t.b[kk][r] = in && c0 + r < n ? b[bt ? (int64_t)(c0 + r) * k + k0 + kk : (int64_t)(k0 + kk) * n + c0 + r] : 0.f;
-    }
-    __syncthreads();
-    tile_fma(t, acc);
-    __syncthreads();
+  const int64_t total = rows * n;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i / n, c = i % n;
+    float s = 0.f;
+    for (int t = 0; t < top; ++t) s += part[(row * top + t) * n + c];
+    store_y(out, i, dt, s);
   }
-  const int tr = threadIdx.x >> 4, tc = threadIdx.x & 15;
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int r = r0 + tr * 4 + i, cc = c0 + tc * 4 + j;
-      if (r >= m || cc >= n) continue;
-      const int64_t o = z * m * n + (int64_t)r * n + cc;
-      d[o] = alpha * acc[i][j] + (c != nullptr ? beta * c[o] : 0.f);
-    }
 }
 
-__global__ void __launch_bounds__(1024) normalise_kernel(int dt, const void* g, int64_t n, float eps, float* x) {
-  __shared__ double red[32];
-  const int64_t base = (int64_t)blockIdx.x * n;
+// ---------------------------------------------------------------------------
+// the matrices' gradient
+// ---------------------------------------------------------------------------
+
+// Each group's rows are cut into segments of at most `seg` rows; a group of one
+// segment is written as it is, the others go through fp32 partials that are
+// added in segment order.
+struct SegPlan {
+  int64_t seg, max_segs, max_slots, max_split;
+};
+
+SegPlan seg_plan(const Groups& g, int64_t m, int64_t n) {
+  const int64_t tiles = ceil_div(m, 128) * ceil_div(n, 256), slots = std::max<int64_t>(1, g.slots());
+  SegPlan p{};
+  // about two waves of segments over the SMs, never short ones (a partial costs
+  // 8 m n bytes) ...
+  p.seg = std::max<int64_t>(512, slots * tiles / (2 * 148));
+  // ... and where the groups alone fill the GPU only those far above the average are cut
+  if (g.K * tiles >= 2 * 148) p.seg = std::max<int64_t>(p.seg, 2 * ceil_div(slots, g.K));
+  // ... and no accumulator takes more than 2048 additions (each costs up to 3.4e-8 of the sum)
+  p.seg = std::min<int64_t>(round_up(p.seg, kBlockK), 32768);
+  p.max_slots = slots > p.seg ? 2 * slots / p.seg + 1 : 0;
+  p.max_split = slots > p.seg ? slots / p.seg + 1 : 0;
+  p.max_segs = g.K + p.max_slots;
+  return p;
+}
+
+__device__ __forceinline__ int block_exclusive(int v, int* red, int* total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += t;
+  }
+  __syncthreads();
+  if (lane == 31) red[w] = s;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int i = 0; i < 32; ++i) {
+    if (i < w) before += red[i];
+    all += red[i];
+  }
+  *total = all;
+  return before + s - v;
+}
+
+// table: [0] segments, [1] split groups; per segment {group, first position,
+// rows, partial slot or -1}; split[i] = {group, first slot, segments, 0}
+__global__ void __launch_bounds__(1024) segments_kernel(const int32_t* offsets, int K, int seg, int32_t* table,
+                                                        int4* split) {
+  __shared__ int red[32];
+  int seg0 = 0, slot0 = 0, split0 = 0;
+  for (int k0 = 0; k0 < K; k0 += 1024) {
+    const int k = k0 + threadIdx.x;
+    const int pos = k < K ? offsets[k] : 0, c = k < K ? offsets[k + 1] - pos : 0;
+    const int ns = k < K ? max(1, (int)(((int64_t)c + seg - 1) / seg)) : 0;
+    int n_segs, n_slots, n_split;
+    const int s = seg0 + block_exclusive(ns, red, &n_segs);
+    const int sl = slot0 + block_exclusive(ns > 1 ? ns : 0, red, &n_slots);
+    const int sp = split0 + block_exclusive(ns > 1 ? 1 : 0, red, &n_split);
+    for (int i = 0; i < ns; ++i)
+      reinterpret_cast<int4*>(table + kSegHeader)[s + i] =
+          make_int4(k, pos + i * seg, min(seg, c - i * seg), ns > 1 ? sl + i : -1);
+    if (ns > 1) split[sp] = make_int4(k, sl, ns, 0);
+    seg0 += n_segs;
+    slot0 += n_slots;
+    split0 += n_split;
+  }
+  if (threadIdx.x == 0) {
+    table[0] = seg0;
+    table[1] = split0;
+  }
+}
+
+// sums of the partials of the split groups, in segment order
+__global__ void __launch_bounds__(256) join_kernel(const int32_t* table, const int4* split, const float* part,
+                                                   int64_t size, void* out, int dt) {
+  const int64_t chunks = (size + 255) / 256, total = table[1] * chunks;
+  for (int64_t it = blockIdx.x; it < total; it += gridDim.x) {
+    const int4 s = split[it / chunks];
+    const int64_t i = it % chunks * 256 + threadIdx.x;
+    if (i >= size) continue;
+    const float* p = part + s.y * size + i;
+    float v = 0.f;
+#pragma unroll 4
+    for (int j = 0; j < s.z; ++j) v += p[j * size];
+    store_y(out, s.x * size + i, dt, v);
+  }
+}
+
+// gb: column sums of each segment's gathered gradients.  16 row lanes x 16
+// column lanes of 8 columns; the row lanes' sums are added in lane order.
+__global__ void __launch_bounds__(256) bias_kernel(const int32_t* table, const int32_t* order, const void* gy, int dt,
+                                                   int n, int vec, float* part, void* out) {
+  __shared__ float red[16][129];
+  const int64_t segs = table[0];
+  const int rl = threadIdx.x >> 4, c = blockIdx.x * 128 + (threadIdx.x & 15) * 8;
+  for (int64_t it = blockIdx.y; it < segs; it += gridDim.y) {
+    const int4 s = reinterpret_cast<const int4*>(table + kSegHeader)[it];
+    float acc[8] = {};
+    if (c < n) {
+#pragma unroll 2
+      for (int r = rl; r < s.z; r += 16) {
+        const int64_t at = (int64_t)order[s.y + r] * n + c;
+        if (vec && dt != GMMXX_FLOAT32) {
+          const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(gy) + at);
+          const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float2 f;
+            if (dt == GMMXX_BFLOAT16) f = make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u));
+            else f = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
+            acc[2 * j] += f.x;
+            acc[2 * j + 1] += f.y;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (c + j < n) acc[j] += load_x(gy, at + j, dt);
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) red[rl][(threadIdx.x & 15) * 8 + j] = acc[j];
+    __syncthreads();
+    const int cc = blockIdx.x * 128 + threadIdx.x;
+    if (threadIdx.x < 128 && cc < n) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v += red[i][threadIdx.x];
+      if (s.w >= 0) part[(int64_t)s.w * n + cc] = v;
+      else store_y(out, (int64_t)s.x * n + cc, dt, v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Newton-Schulz
+// ---------------------------------------------------------------------------
+
+constexpr int kNormBlocks = 64;  // per matrix, at most
+
+__global__ void __launch_bounds__(256) square_sum_kernel(int dt, const void* g, int64_t n, double* part) {
+  __shared__ double red[8];
+  const int64_t base = (int64_t)blockIdx.y * n;
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const double v = load_x(g, base + i, dt);
     s += v * v;
   }
   s = block_sum(s, red);
+  if (threadIdx.x == 0) part[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = s;
+}
+
+// x = g / (|g| + eps) as fp16 planes of x * kPlaneScale, or (q) rounded to the result
+__global__ void __launch_bounds__(256) scale_kernel(int dt, const void* g, int64_t m, int n, int ld, float eps,
+                                                    const double* part, int nparts, __half* hi, __half* lo, void* q) {
+  const int64_t z = blockIdx.y, total = m * n;
+  double s = 0.0;
+  for (int i = 0; i < nparts; ++i) s += part[z * nparts + i];
   const double inv = 1.0 / (sqrt(s) + (double)eps);
-  for (int64_t i = threadIdx.x; i < n; i += 1024) x[base + i] = (float)(load_x(g, base + i, dt) * inv);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const double v = load_x(g, z * total + i, dt) * inv;
+    if (q != nullptr) {
+      store_y(q, z * total + i, dt, (float)v);
+      continue;
+    }
+    const int64_t at = (z * m + i / n) * ld + i % n;
+    const float f = (float)(v * kPlaneScale);
+    const __half h = __float2half_rn(f);
+    hi[at] = h;
+    if (lo != nullptr) lo[at] = __float2half_rn(f - __half2float(h));
+  }
 }
 
-__global__ void round_kernel(const float* x, int64_t n, void* q, int dt) {
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
-    store_y(q, i, dt, x[i]);
+struct NsPlan {
+  int planes;
+  int64_t lo, hi, ldx, ldp, x_plane, p_plane;  // bytes per plane
+  int64_t x, y, p, q, part, bytes;
+  int nparts;
+};
+
+// One fp16 plane per iterate where the result is rounded to bf16 and the short
+// side is long (its error, 1.0e-3 .. 1.3e-3 of the norm, stays below bf16's own
+// 1.7e-3), else two.
+NsPlan ns_plan(int dt, int64_t batch, int64_t m, int64_t n) {
+  NsPlan s{};
+  s.lo = std::min(m, n);
+  s.hi = std::max(m, n);
+  s.planes = dt == GMMXX_BFLOAT16 && s.lo >= 256 ? 1 : 2;
+  s.ldx = pad8(n);
+  s.ldp = pad8(s.lo);
+  s.x_plane = al256(batch * m * s.ldx * 2);
+  s.p_plane = al256(batch * s.lo * s.ldp * 2);
+  s.nparts = (int)std::min<int64_t>(kNormBlocks, ceil_div(m * n, 4096));
+  int64_t off = 0;
+  s.x = off; off += s.x_plane * s.planes;
+  s.y = off; off += s.x_plane * s.planes;
+  s.p = off; off += s.p_plane * s.planes;
+  s.q = off; off += s.p_plane * s.planes;
+  s.part = off; off += al256(batch * s.nparts * 8);
+  s.bytes = off;
+  return s;
 }
 
-int launch_rows(int dt, const void* x, int div, const Groups& g, int64_t n_in, int64_t n_out, const void* w,
-                int64_t w_in, int64_t w_out, const void* bias, void* out, int out_dt, cudaStream_t st) {
-  dim3 grid((unsigned)(2 * g.max_tiles()), (unsigned)ceil_div(n_out, kT));
-  rows_kernel<<<grid, 256, 0, st>>>(dt, x, div, g, (int)n_in, (int)n_out, w, w_in, w_out, bias, out, out_dt);
-  return check_launch("rows_kernel");
+struct Stack {  // planes of a stack of matrices
+  char* base;
+  int64_t plane, rows, cols, ld;
+};
+
+int stack_operand(const Stack& s, int planes, int64_t batch, int box_rows, CUtensorMap* maps) {
+  for (int i = 0; i < planes; ++i)
+    if (int rc = encode_stack(&maps[i], s.base + i * s.plane, 1, s.cols, s.rows, s.ld, batch, s.rows * s.ld, box_rows))
+      return rc;
+  return GMMXX_OK;
 }
 
 }  // namespace
 
-size_t grouped_matmul_ws(int, const Groups&, int64_t, int64_t) { return 256; }
-
-int launch_grouped_matmul(int dt, const void* x, const Groups& g, int64_t n_in, int64_t n_out, const void* w, int wt,
-                          const void* bias, void* out, char*, cudaStream_t st) {
-  return launch_rows(dt, x, g.top, g, n_in, n_out, w, wt ? 1 : n_out, wt ? n_in : 1, bias, out, dt, st);
+size_t grouped_matmul_ws(int dt, const Groups& g, int64_t n_in, int64_t n_out) {
+  // the weight's inner length is n_out or (transposed) n_in: room for either
+  const int64_t w = std::max(pack_bytes(dt, g.K * n_in, n_out), pack_bytes(dt, g.K * n_out, n_in));
+  return (size_t)(256 + pack_bytes(dt, g.rows, n_in) + w);
 }
 
-size_t grouped_backward_ws(int, const Groups& g, int64_t n_in, int64_t) {
-  return 256 + (g.top > 1 ? (size_t)(g.slots() * n_in * 4) : 0);
+int launch_grouped_matmul(int dt, const void* x, const Groups& g, int64_t n_in, int64_t n_out, const void* w, int wt,
+                          const void* bias, void* out, char* ws, cudaStream_t st) {
+  Planes px, pw;
+  if (int rc = operand(dt, x, g.rows, n_in, ws, &px, st)) return rc;
+  if (int rc = operand(dt, w, g.K * (wt ? n_out : n_in), wt ? n_in : n_out, ws, &pw, st)) return rc;
+  return rows_product(dt, px, g.rows, g.top, g, n_in, n_out, pw, wt != 0, bias, out, dt, st);
+}
+
+size_t grouped_backward_ws(int dt, const Groups& g, int64_t n_in, int64_t n_out) {
+  const SegPlan p = seg_plan(g, n_in, n_out);
+  const int64_t w = std::max(pack_bytes(dt, g.K * n_in, n_out), pack_bytes(dt, g.K * n_out, n_in));
+  return (size_t)(256 + pack_bytes(dt, g.slots(), n_out) + w + pack_bytes(dt, g.rows, n_in) +
+                  (g.top > 1 ? al256(g.slots() * n_in * 4) : 0) + al256((kSegHeader + kSegInts * p.max_segs) * 4) +
+                  al256(p.max_split * 16) + al256(p.max_slots * n_in * n_out * 4) + al256(p.max_slots * n_out * 4));
 }
 
 int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups& g, int64_t n_in, int64_t n_out,
                             const void* w, int wt, void* gx, void* gw, void* gb, char* ws, cudaStream_t st) {
-  if (gx != nullptr && g.rows > 0) {
-    float* part = reinterpret_cast<float*>(ws);
-    const bool sum = g.top > 1;
-    if (int rc = launch_rows(dt, gy, 1, g, n_out, n_in, w, wt ? n_in : 1, wt ? 1 : n_out, nullptr,
-                             sum ? static_cast<void*>(part) : gx, sum ? GMMXX_FLOAT32 : dt, st))
+  Planes pg, pw, px;
+  const int64_t slots = g.slots();
+  if (slots > 0 && (gx != nullptr || gw != nullptr))
+    if (int rc = operand(dt, gy, slots, n_out, ws, &pg, st)) return rc;
+  if (slots > 0 && gx != nullptr) {
+    if (int rc = operand(dt, w, g.K * (wt ? n_out : n_in), wt ? n_in : n_out, ws, &pw, st)) return rc;
+    void* to = gx;
+    if (g.top > 1) {
+      to = ws;
+      ws += al256(slots * n_in * 4);
+    }
+    if (int rc = rows_product(dt, pg, slots, 1, g, n_out, n_in, pw, wt == 0, nullptr, to,
+                              g.top > 1 ? GMMXX_FLOAT32 : dt, st))
       return rc;
-    if (sum) {
-      sum_slots_kernel<<<(unsigned)ceil_div(g.rows * n_in, 256), 256, 0, st>>>(part, g.rows, g.top, (int)n_in, gx, dt);
+    if (g.top > 1) {
+      const int64_t blocks = std::min<int64_t>(148 * 16, ceil_div(g.rows * n_in, 256));
+      sum_slots_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const float*>(to), g.rows, g.top, (int)n_in, gx, dt);
       if (int rc = check_launch("sum_slots_kernel")) return rc;
     }
   }
+  if (gw == nullptr && gb == nullptr) return GMMXX_OK;
+  if (slots == 0) {
+    cudaError_t e = cudaSuccess;
+    if (gw != nullptr) e = cudaMemsetAsync(gw, 0, (size_t)(g.K * n_in * n_out * elem_bytes(dt)), st);
+    if (e == cudaSuccess && gb != nullptr) e = cudaMemsetAsync(gb, 0, (size_t)(g.K * n_out * elem_bytes(dt)), st);
+    return e == cudaSuccess ? GMMXX_OK : set_error(GMMXX_ERR_CUDA, "memset: %s", cudaGetErrorString(e));
+  }
+  const SegPlan p = seg_plan(g, n_in, n_out);
+  int32_t* table = reinterpret_cast<int32_t*>(ws);
+  ws += al256((kSegHeader + kSegInts * p.max_segs) * 4);
+  int4* split = reinterpret_cast<int4*>(ws);
+  ws += al256(p.max_split * 16);
+  float* part = reinterpret_cast<float*>(ws);
+  ws += al256(p.max_slots * n_in * n_out * 4);
+  float* part_b = reinterpret_cast<float*>(ws);
+  ws += al256(p.max_slots * n_out * 4);
+  segments_kernel<<<1, 1024, 0, st>>>(g.offsets, g.K, (int)p.seg, table, split);
+  if (int rc = check_launch("segments_kernel")) return rc;
   if (gw != nullptr) {
-    dim3 grid((unsigned)ceil_div(n_in, kT), (unsigned)ceil_div(n_out, kT), (unsigned)g.K);
-    weight_kernel<<<grid, 256, 0, st>>>(dt, x, gy, g, (int)n_in, (int)n_out, gw, wt ? 1 : n_out, wt ? n_in : 1);
-    if (int rc = check_launch("weight_kernel")) return rc;
+    if (int rc = operand(dt, x, g.rows, n_in, ws, &px, st)) return rc;
+    // (n_in x n_out) = x^T gy; for a transposed weight (n_out x n_in) = gy^T x
+    const int64_t m = wt ? n_out : n_in, n = wt ? n_in : n_out;
+    const int planes = planes_of(dt);
+    const int bn = tile_columns(p.max_segs * ceil_div(m, 128), n, planes, 256);
+    ProductMaps maps;
+    if (int rc = rows_maps(px, n_in, g.rows, wt ? maps.b : maps.a)) return rc;
+    if (int rc = rows_maps(pg, n_out, slots, wt ? maps.a : maps.b)) return rc;
+    ProductArgs a{};
+    a.m = (int)m;
+    a.n = (int)n;
+    a.bn = bn;
+    a.stages = product_stages(planes, bn);
+    a.mt = (int)ceil_div(m, 128);
+    a.nt = (int)ceil_div(n, bn);
+    a.a_mn = a.b_mn = 1;
+    a.idesc = product_idesc(px.fp16, bn, 1, 1);
+    a.order = g.order;
+    a.table = table;
+    a.div_a = wt ? 1 : g.top;
+    a.div_b = wt ? g.top : 1;
+    a.groups = g.K;
+    a.out = gw;
+    a.out_dt = dt;
+    a.ldo = n;
+    a.out_stride = m * n;
+    a.vec = vec_ok(gw, dt, n);
+    a.part = part;
+    if (int rc = launch_product(kWeights, planes, maps, a, p.max_segs, st)) return rc;
+    if (p.max_split > 0) {
+      join_kernel<<<148 * 8, 256, 0, st>>>(table, split, part, m * n, gw, dt);
+      if (int rc = check_launch("join_kernel")) return rc;
+    }
   }
   if (gb != nullptr) {
-    bias_kernel<<<dim3((unsigned)ceil_div(n_out, 256), (unsigned)g.K), 256, 0, st>>>(dt, gy, g, (int)n_out, gb);
+    const dim3 grid((unsigned)ceil_div(n_out, 128), (unsigned)std::min<int64_t>(65535, p.max_segs));
+    bias_kernel<<<grid, 256, 0, st>>>(table, g.order, gy, dt, (int)n_out, vec_ok(gy, dt, n_out), part_b, gb);
     if (int rc = check_launch("bias_kernel")) return rc;
+    if (p.max_split > 0) {
+      join_kernel<<<148, 256, 0, st>>>(table, split, part_b, n_out, gb, dt);
+      if (int rc = check_launch("join_kernel")) return rc;
+    }
   }
   return GMMXX_OK;
 }
 
-size_t orthogonalize_ws(int, int64_t batch, int64_t m, int64_t n) {
-  const int64_t lo = m < n ? m : n;
-  return (size_t)(4 * batch * (2 * m * n + 2 * lo * lo) + 256);
+size_t orthogonalize_ws(int dt, int64_t batch, int64_t m, int64_t n) {
+  return (size_t)(ns_plan(dt, batch, m, n).bytes + 256);
 }
 
 int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_t n, int steps, float a, float b,
                          float c, float eps, void* q, char* ws, cudaStream_t st) {
-  const int64_t lo = m < n ? m : n, hi = m < n ? n : m;
-  float* x = reinterpret_cast<float*>(ws);
-  float* y = x + batch * m * n;
-  float* p = y + batch * m * n;
-  float* r = p + batch * lo * lo;
-  normalise_kernel<<<(unsigned)batch, 1024, 0, st>>>(dt, g, m * n, eps, x);
-  if (int rc = check_launch("normalise_kernel")) return rc;
-  for (int64_t z0 = 0; z0 < batch; z0 += 65535) {  // grid z
-    const unsigned nz = (unsigned)(batch - z0 < 65535 ? batch - z0 : 65535);
-    const unsigned tl = (unsigned)ceil_div(lo, kT);
-    float *xs = x + z0 * m * n, *ys = y + z0 * m * n, *ps = p + z0 * lo * lo, *rs = r + z0 * lo * lo;
-    for (int s = 0; s < steps; ++s) {
-      const bool wide = m <= n;
-      batch_kernel<<<dim3(tl, tl, nz), 256, 0, st>>>(xs, wide ? 0 : 1, xs, wide ? 1 : 0, nullptr, ps, (int)lo, (int)lo,
-                                                     (int)hi, 1.f, 0.f);
-      batch_kernel<<<dim3(tl, tl, nz), 256, 0, st>>>(ps, 0, ps, 0, ps, rs, (int)lo, (int)lo, (int)lo, c, b);
-      dim3 grid((unsigned)ceil_div(m, kT), (unsigned)ceil_div(n, kT), nz);
-      if (wide) batch_kernel<<<grid, 256, 0, st>>>(rs, 0, xs, 0, xs, ys, (int)m, (int)n, (int)lo, 1.f, a);
-      else batch_kernel<<<grid, 256, 0, st>>>(xs, 0, rs, 0, xs, ys, (int)m, (int)n, (int)lo, 1.f, a);
-      float* t = xs;
-      xs = ys;
-      ys = t;
-    }
-    if (int rc = check_launch("batch_kernel")) return rc;
+  const NsPlan s = ns_plan(dt, batch, m, n);
+  const int64_t size = m * n;
+  double* part = reinterpret_cast<double*>(ws + s.part);
+  for (int64_t z0 = 0; z0 < batch; z0 += 65535) {  // grid y
+    const unsigned nz = (unsigned)std::min<int64_t>(65535, batch - z0);
+    const char* gz = static_cast<const char*>(g) + z0 * size * elem_bytes(dt);
+    double* pz = part + z0 * s.nparts;
+    square_sum_kernel<<<dim3((unsigned)s.nparts, nz), 256, 0, st>>>(dt, gz, size, pz);
+    if (int rc = check_launch("square_sum_kernel")) return rc;
+    __half* hi = reinterpret_cast<__half*>(ws + s.x) + z0 * m * s.ldx;
+    __half* lo = s.planes > 1 ? reinterpret_cast<__half*>(ws + s.x + s.x_plane) + z0 * m * s.ldx : nullptr;
+    scale_kernel<<<dim3((unsigned)std::min<int64_t>(256, ceil_div(size, 1024)), nz), 256, 0, st>>>(
+        dt, gz, m, (int)n, (int)s.ldx, eps, pz, s.nparts, hi, lo,
+        steps == 0 ? static_cast<char*>(q) + z0 * size * elem_bytes(dt) : nullptr);
+    if (int rc = check_launch("scale_kernel")) return rc;
   }
-  round_kernel<<<148 * 4, 256, 0, st>>>((steps & 1) ? y : x, batch * m * n, q, dt);
-  return check_launch("round_kernel");
+  Stack X{ws + s.x, s.x_plane, m, n, s.ldx}, Y{ws + s.y, s.x_plane, m, n, s.ldx};
+  const Stack P{ws + s.p, s.p_plane, s.lo, s.lo, s.ldp}, Q{ws + s.q, s.p_plane, s.lo, s.lo, s.ldp};
+  const bool wide = m <= n;
+  const int max_bn = s.planes == 1 ? 256 : 128;
+  auto product = [&](const Stack& A, bool a_mn, const Stack& B, bool b_mn, int64_t rows, int64_t cols, int64_t k,
+                     float alpha, float beta, const Stack* E, const Stack& O, void* out) {
+    const int bn = tile_columns(batch * ceil_div(rows, 128), cols, s.planes, max_bn);
+    ProductMaps maps;
+    if (int rc = stack_operand(A, s.planes, batch, a_mn ? kBlockK : 128, maps.a)) return rc;
+    if (int rc = stack_operand(B, s.planes, batch, b_mn ? kBlockK : bn, maps.b)) return rc;
+    ProductArgs t{};
+    t.m = (int)rows;
+    t.n = (int)cols;
+    t.k = (int)k;
+    t.bn = bn;
+    t.stages = product_stages(s.planes, bn);
+    t.mt = (int)ceil_div(rows, 128);
+    t.nt = (int)ceil_div(cols, bn);
+    t.a_mn = a_mn;
+    t.b_mn = b_mn;
+    t.idesc = product_idesc(1, bn, a_mn, b_mn);
+    t.items = batch;
+    t.alpha = alpha / kPlaneScale;
+    t.beta = beta;
+    for (int i = 0; i < s.planes; ++i) {
+      if (E != nullptr) t.e[i] = reinterpret_cast<const __half*>(E->base + i * E->plane);
+      t.o[i] = reinterpret_cast<__half*>(O.base + i * O.plane);
+    }
+    t.ldp = O.ld;
+    t.p_stride = O.rows * O.ld;
+    t.out = out;
+    t.out_dt = dt;
+    t.ldo = cols;
+    t.out_stride = rows * cols;
+    t.vec = vec_ok(out, dt, cols) && vec_ok(out, dt, rows * cols);
+    return launch_product(kBatch, s.planes, maps, t, batch, st);
+  };
+  for (int i = 0; i < steps; ++i) {
+    void* out = i == steps - 1 ? q : nullptr;
+    if (int rc = wide ? product(X, false, X, false, s.lo, s.lo, s.hi, 1.f, 0.f, nullptr, P, nullptr)
+                      : product(X, true, X, true, s.lo, s.lo, s.hi, 1.f, 0.f, nullptr, P, nullptr))
+      return rc;
+    // P is symmetric: its rows serve as the columns of the second factor
+    if (int rc = product(P, false, P, false, s.lo, s.lo, s.lo, c, b, &P, Q, nullptr)) return rc;
+    if (int rc = wide ? product(Q, false, X, true, m, n, s.lo, 1.f, a, &X, Y, out)
+                      : product(X, false, Q, false, m, n, s.lo, 1.f, a, &X, Y, out))
+      return rc;
+    std::swap(X, Y);
+  }
+  return GMMXX_OK;
 }
 
 }  // namespace experts

@@ -42,6 +42,11 @@ int check_ws(const void* ws, size_t bytes, size_t need) {
   return GMMXX_OK;
 }
 
+// the tensor-core loads start on 16-byte boundaries
+#define GMMXX_ALIGNED(p, name)                              \
+  if ((reinterpret_cast<uintptr_t>(p) & 15) != 0)           \
+  return set_error(GMMXX_ERR_INVALID, "%s must be 16-byte aligned", name)
+
 #define GMMXX_REQUIRE(p, name) \
   if ((p) == nullptr) return set_error(GMMXX_ERR_INVALID, "%s is NULL", name)
 
@@ -115,6 +120,8 @@ int gmmxx_grouped_matmul(int dtype, const void* x, int64_t rows, int64_t top_k, 
   GMMXX_REQUIRE(tiles, "tiles");
   GMMXX_REQUIRE(weight, "weight");
   GMMXX_REQUIRE(out, "out");
+  GMMXX_ALIGNED(x, "x");
+  GMMXX_ALIGNED(weight, "weight");
   const experts::Groups g = make_groups(rows, top_k, K, order, offsets, tiles);
   if (int rc = check_ws(workspace, workspace_bytes, experts::grouped_matmul_ws(dtype, g, n_in, n_out))) return rc;
   return experts::launch_grouped_matmul(dtype, x, g, n_in, n_out, weight, weight_transposed != 0, bias, out,
@@ -141,12 +148,20 @@ int gmmxx_grouped_matmul_backward(int dtype, const void* grad_out, const void* x
     if (grad_x != nullptr) GMMXX_REQUIRE(weight, "weight");
     if (grad_weight != nullptr) GMMXX_REQUIRE(x, "x");
   }
+  GMMXX_ALIGNED(grad_out, "grad_out");
+  GMMXX_ALIGNED(x, "x");
+  GMMXX_ALIGNED(weight, "weight");
   GMMXX_REQUIRE(offsets, "offsets");
   const experts::Groups g = make_groups(rows, top_k, K, order, offsets, tiles);
   if (int rc = check_ws(workspace, workspace_bytes, experts::grouped_backward_ws(dtype, g, n_in, n_out))) return rc;
   return experts::launch_grouped_backward(dtype, grad_out, x, g, n_in, n_out, weight, weight_transposed != 0, grad_x,
                                           grad_weight, grad_bias, static_cast<char*>(workspace),
                                           static_cast<cudaStream_t>(stream));
+}
+
+int gmmxx_products_status(int* status_out, void* stream) {
+  GMMXX_REQUIRE(status_out, "status_out");
+  return experts::read_status(status_out, static_cast<cudaStream_t>(stream));
 }
 
 size_t gmmxx_orthogonalize_workspace_bytes(int dtype, int64_t batch, int64_t m, int64_t n) {

@@ -1,0 +1,593 @@
+// experts_tc.cu -- the product kernel of the routed products and of the
+// Newton-Schulz iteration, on the 5th-generation tensor cores.
+//
+//   D[128 x bn] = sum over k of A[128 x k] B[k x bn]      (fp32 in tensor memory)
+//
+// One persistent CTA per SM walks output tiles.  A TMA warp fills a ring of
+// stages (64 contraction elements of A and B each, 128-byte swizzle), one
+// thread issues tcgen05.mma, and eight epilogue warps drain one accumulator
+// from tensor memory while the next tile's products go to the other.
+//
+// Routed rows are never copied: the TMA's gather (tile::gather4, four rows of
+// 128 bytes per instruction) fetches each row where it lies, for kRows as the
+// K-major A operand, for kWeights -- where the rows are the contraction -- as
+// MN-major A and B operands.  Both are the same bytes in shared memory (rows
+// of 64 elements, swizzled), read through different descriptors.
+//
+// Ragged ends.  kRows: rows behind the tile's last are fetched as copies of
+// its first and not stored.  kWeights: the last stage of a segment issues only
+// the 16-row steps that hold rows, and the rest of its last step is zeroed in
+// both operands first (zeroing one would leave NaN * 0).
+//
+// Sums.  The tensor core adds to an accumulator by cutting, not rounding: an
+// addition costs about 3.4e-8 of the sum, always towards zero (measured: 8e-7
+// after 24 additions of 16 products).  That is nothing beside the rounding to 16
+// bits, but not for fp32 results: there the leading planes' products and the
+// others (2^-8 of them and less) go to accumulators of their own, and every
+// kChunk stages (8 additions) both are added into fp32 registers of the
+// epilogue warps.
+//
+// Planes.  16-bit factors are multiplied as they are (1 plane).  fp32 factors
+// arrive as three bf16 planes x = x0 + x1 + x2 of 8 significant bits each
+// (exact) and six products x0w0 + x0w1 + x1w0 + x1w1 + x0w2 + x2w0, which
+// drops 2^-24 of each product; 16-bit products are exact in the tensor core
+// and summed in fp32.  The Newton-Schulz iterates are two fp16 planes of
+// value * 4096 (|value| < 16 by the check on the coefficients; the second
+// plane then keeps its 11 bits down to values of 2^-26) and three products,
+// 22 bits; where the result is rounded to bf16 one plane is enough.
+#include "experts_tc.cuh"
+#include "tc_ptx.cuh"
+
+#include <algorithm>
+
+namespace gmmxx {
+namespace experts {
+
+using namespace ptx;
+
+__device__ int g_status = 0;  // sticky: 1 when a bounded wait ran out (gmmxx_products_status)
+
+namespace {
+
+constexpr int kBM = 128;
+constexpr int kThreadsTc = 384;
+constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
+constexpr int kABytes = kBM * 128;  // one plane of A per stage
+constexpr int kMaxStages = 8;
+constexpr int kChunk = 2;  // stages per accumulation where there are several planes
+constexpr int kSmemLimit = 232448 - 1024;
+
+struct Bars {
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  uint64_t accfull[2], accempty[2];
+  uint32_t tmem_base;
+  int abort;
+};
+
+__device__ __forceinline__ void gather4(void* dst, const CUtensorMap* map, int x, const int* r, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+      "%4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void mma_16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  mma_bf16(d, a, b, idesc, acc);  // kind::f16: the types are the descriptor's
+}
+
+// a bounded wait ran out: every warp of the block stops at its next wait
+__device__ __forceinline__ void give_up(Bars* bars, int lane) {
+  if (lane == 0) {
+    *(volatile int*)&bars->abort = 1;
+    atomicOr(&g_status, 1);
+  }
+}
+
+// one output tile
+struct Tile {
+  int g;       // group / matrix
+  int pos;     // first position (routed)
+  int rows;    // kRows: rows of the tile; kWeights: rows of the segment; kBatch: rows of the tile
+  int m0, n0;
+  int slot;    // kWeights: partial slot or -1
+  int kb;      // contraction stages; 0: the result is zero
+};
+
+template <int KIND>
+__device__ __forceinline__ int64_t tile_count(const ProductArgs& a) {
+  const int64_t items = KIND == kBatch ? a.items : (int64_t)__ldg(a.table);
+  return items * a.mt * a.nt;
+}
+
+template <int KIND>
+__device__ __forceinline__ Tile decode(const ProductArgs& a, int64_t it) {
+  Tile t;
+  t.n0 = (int)(it % a.nt) * a.bn;
+  it /= a.nt;
+  if (KIND == kRows) {
+    const int32_t* e = a.table + kTileHeader + it * kTileInts;
+    t.g = __ldg(e);
+    t.pos = __ldg(e + 1);
+    t.rows = __ldg(e + 2);
+    t.m0 = 0;
+    t.slot = -1;
+    t.kb = t.g < a.groups ? (a.k + kBlockK - 1) / kBlockK : 0;
+    return t;
+  }
+  t.m0 = (int)(it % a.mt) * kBM;
+  it /= a.mt;
+  if (KIND == kWeights) {
+    const int32_t* e = a.table + kSegHeader + it * kSegInts;
+    t.g = __ldg(e);
+    t.pos = __ldg(e + 1);
+    t.rows = __ldg(e + 2);
+    t.slot = __ldg(e + 3);
+    t.kb = (t.rows + kBlockK - 1) / kBlockK;
+  } else {
+    t.g = (int)it;
+    t.pos = 0;
+    t.rows = min(kBM, a.m - t.m0);
+    t.slot = -1;
+    t.kb = (a.k + kBlockK - 1) / kBlockK;
+  }
+  return t;
+}
+
+__device__ __forceinline__ uint4 pack8(const float* v, int dt) {
+  uint4 q;
+  uint32_t* p = reinterpret_cast<uint32_t*>(&q);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (dt == GMMXX_BFLOAT16) {
+      p[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+    } else {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      p[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  return q;
+}
+
+// 32 values of one row to out[row0 + c], nv of them valid
+__device__ __forceinline__ void store32(void* out, int dt, int64_t at, const float* v, int nv, int vec) {
+  if (vec && nv >= 32) {
+    if (dt == GMMXX_FLOAT32) {
+      float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+      uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = pack8(v + 8 * i, dt);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (i < nv) store_y(out, at + i, dt, v[i]);
+}
+
+// kBatch: 32 values of one row: combine with the planes e and write planes or the result
+template <int PLANES>
+__device__ __forceinline__ void batch32(const ProductArgs& a, const Tile& t, int row, int c, float* v, int nv) {
+  const int64_t at = t.g * a.p_stride + (int64_t)row * a.ldp + c;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] *= a.alpha;
+  if (a.e[0] != nullptr) {
+#pragma unroll
+    for (int i0 = 0; i0 < 32; i0 += 8) {  // ldp is a multiple of 8: whole 16-byte pieces (their tail is never used)
+      if (i0 >= nv) break;
+#pragma unroll
+      for (int p = PLANES - 1; p >= 0; --p) {
+        const uint4 q = *reinterpret_cast<const uint4*>(a.e[p] + at + i0);
+        const __half2* h = reinterpret_cast<const __half2*>(&q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = __half22float2(h[i]);
+          v[i0 + 2 * i] = fmaf(a.beta, f.x, v[i0 + 2 * i]);
+          v[i0 + 2 * i + 1] = fmaf(a.beta, f.y, v[i0 + 2 * i + 1]);
+        }
+      }
+    }
+  }
+  if (a.out != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] *= 1.f / kPlaneScale;
+    store32(a.out, a.out_dt, t.g * a.out_stride + (int64_t)row * a.ldo + c, v, nv, a.vec);
+    return;
+  }
+#pragma unroll
+  for (int i0 = 0; i0 < 32; i0 += 8) {
+    if (i0 >= nv) break;
+    uint4 q[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = v[i0 + 2 * i], y = v[i0 + 2 * i + 1];
+      const __half2 hi = __floats2half2_rn(x, y);
+      reinterpret_cast<__half2*>(&q[0])[i] = hi;
+      if (PLANES > 1) {
+        const float2 f = __half22float2(hi);
+        reinterpret_cast<__half2*>(&q[1])[i] = __floats2half2_rn(x - f.x, y - f.y);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p) *reinterpret_cast<uint4*>(a.o[p] + at + i0) = q[p];
+  }
+}
+
+template <int KIND, int PLANES>
+__global__ void __launch_bounds__(kThreadsTc, 1)
+    product_kernel(const __grid_constant__ ProductMaps maps, const ProductArgs a) {
+  extern __shared__ __align__(1024) char smem_raw[];
+  __shared__ Bars bars;
+  char* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int bbytes = a.bn * 128;  // one plane of B per stage
+  const int stage_bytes = PLANES * (kABytes + bbytes);
+  volatile int* abort = &bars.abort;
+  // two buffers of one accumulator, or of two (leading products, others)
+  constexpr int kAccs = PLANES > 1 ? 2 : 1;
+  const uint32_t tmem_cols = 2 * kAccs * a.bn;  // a power of two of at least 32
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < a.stages; ++i) {
+      mbar_init(&bars.full[i], 1);
+      mbar_init(&bars.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.accfull[i], 1);
+      mbar_init(&bars.accempty[i], kEpiWarps);
+    }
+    bars.abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 2) tmem_alloc(&bars.tmem_base, tmem_cols);
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = bars.tmem_base;
+  const int64_t total = tile_count<KIND>(a);
+
+  if (warp == 0) {
+    // ---- loads ----
+    if (lane < PLANES) {
+      prefetch_tmap(&maps.a[lane]);
+      prefetch_tmap(&maps.b[lane]);
+    }
+    int64_t fill = 0;  // stages filled so far
+    bool ok = true;
+    const int quad = lane & 15, half = lane >> 4;
+    for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
+      const Tile t = decode<KIND>(a, it);
+      if (t.kb == 0) continue;
+      int ra[4], rb[4], next[4];
+      if (KIND == kRows) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * lane + i;
+          ra[i] = __ldg(a.order + t.pos + (r < t.rows ? r : 0)) / a.div_a;
+        }
+      } else if (KIND == kWeights) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) next[i] = __ldg(a.order + t.pos + min(4 * quad + i, t.rows - 1));
+      }
+      for (int kb = 0; kb < t.kb; ++kb, ++fill) {
+        const int s = (int)(fill % a.stages);
+        const uint32_t ph = (uint32_t)((fill / a.stages) & 1);
+        if (KIND == kWeights) {  // this stage's rows; the next stage's are fetched meanwhile
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            ra[i] = next[i] / a.div_a;
+            rb[i] = next[i] / a.div_b;
+            next[i] = __ldg(a.order + t.pos + min((kb + 1) * kBlockK + 4 * quad + i, t.rows - 1));
+          }
+        }
+        ok = mbar_wait_warp(&bars.empty[s], ph ^ 1, abort);
+        if (!ok) break;
+        char* sa = sm + s * stage_bytes;
+        char* sb = sa + PLANES * kABytes;
+        uint64_t* bar = &bars.full[s];
+        if (lane == 0) mbar_expect_tx(bar, (uint32_t)stage_bytes);
+        __syncwarp();
+        const int k0 = kb * kBlockK;
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) {
+          char* pa = sa + p * kABytes;
+          char* pb = sb + p * bbytes;
+          if (KIND == kRows) {
+            gather4(pa + lane * 512, &maps.a[p], k0, ra, bar);
+          } else if (KIND == kWeights) {
+            gather4(pa + half * 8192 + quad * 512, &maps.a[p], t.m0 + half * 64, ra, bar);
+            for (int j = half; j < a.bn / 64; j += 2)
+              gather4(pb + j * 8192 + quad * 512, &maps.b[p], t.n0 + j * 64, rb, bar);
+          } else if (a.a_mn) {
+            if (lane < 2) tma_load_3d(pa + lane * 8192, &maps.a[p], t.m0 + lane * 64, k0, t.g, bar);
+          } else {
+            if (lane == 0) tma_load_3d(pa, &maps.a[p], k0, t.m0, t.g, bar);
+          }
+          if (KIND != kWeights) {
+            if (a.b_mn) {
+              if (lane < a.bn / 64) tma_load_3d(pb + lane * 8192, &maps.b[p], t.n0 + lane * 64, k0, t.g, bar);
+            } else {
+              if (lane == 0) tma_load_3d(pb, &maps.b[p], k0, t.n0, t.g, bar);
+            }
+          }
+        }
+      }
+    }
+    if (!ok) {  // the copies in flight still write shared memory: wait for them before the block ends
+      give_up(&bars, lane);
+      const int64_t first = fill > a.stages ? fill - a.stages : 0;
+      for (int64_t f = first; f < fill; ++f) mbar_wait_warp(&bars.full[f % a.stages], (uint32_t)((f / a.stages) & 1), nullptr);
+    }
+  } else if (warp == 1) {
+    // ---- products ----
+    int64_t use = 0, sums = 0;
+    bool ok = true;
+    const uint32_t step_a = a.a_mn ? 2048 : 32, step_b = a.b_mn ? 2048 : 32;  // bytes per 16 contraction elements
+    for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
+      const Tile t = decode<KIND>(a, it);
+      if (t.kb == 0) continue;
+      int buf = 0;
+      uint32_t d = 0;
+      for (int kb = 0; kb < t.kb; ++kb, ++use) {
+        const int in_sum = PLANES > 1 ? kb % kChunk : kb;  // stages already in this accumulator
+        if (in_sum == 0) {
+          buf = (int)(sums & 1);
+          ok = mbar_wait_warp(&bars.accempty[buf], (uint32_t)(((sums >> 1) & 1) ^ 1), abort);
+          if (!ok) break;
+          tmem_fence_after();
+          d = tmem + buf * kAccs * a.bn;
+          ++sums;
+        }
+        const int s = (int)(use % a.stages);
+        ok = mbar_wait_warp(&bars.full[s], (uint32_t)((use / a.stages) & 1), abort);
+        if (!ok) break;
+        char* sa = sm + s * stage_bytes;
+        char* sb = sa + PLANES * kABytes;
+        int steps = 4;
+        if (KIND == kWeights) {
+          const int left = t.rows - kb * kBlockK;
+          if (left < kBlockK) {
+            steps = (left + 15) >> 4;
+            const int zero = steps * 16 - left;  // rows to clear, of 128 bytes in each 64-column group
+            if (zero > 0) {
+              const int groups = PLANES * (2 + a.bn / 64);
+              for (int i = lane; i < groups * zero * 8; i += 32) {
+                const int grp = i / (zero * 8), r = left + (i % (zero * 8)) / 8, q = i % 8;
+                char* g = grp < 2 * PLANES ? sa + grp * 8192 : sb + (grp - 2 * PLANES) * 8192;
+                *reinterpret_cast<uint4*>(g + r * 128 + q * 16) = make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async();
+              __syncwarp();
+            }
+          }
+        }
+        if (lane == 0) {
+          tmem_fence_after();
+          constexpr int kPairs = PLANES == 1 ? 1 : PLANES == 2 ? 3 : 6;
+#pragma unroll
+          for (int c = 0; c < kPairs; ++c) {
+            constexpr int pa[6] = {0, 0, 1, 1, 0, 2}, pb[6] = {0, 1, 0, 1, 2, 0};
+            const uint32_t ua = smem_u32(sa) + pa[c] * kABytes, ub = smem_u32(sb) + pb[c] * bbytes;
+            const uint64_t da = a.a_mn ? desc_mnmajor(ua, 8192) : desc_kmajor(ua);
+            const uint64_t db = a.b_mn ? desc_mnmajor(ub, 8192) : desc_kmajor(ub);
+            for (int k = 0; k < steps; ++k)
+              mma_16(c == 0 ? d : d + a.bn, da + ((k * step_a) >> 4), db + ((k * step_b) >> 4), a.idesc,
+                     (in_sum | k) != 0 || c > 1);
+          }
+          mma_commit(&bars.empty[s]);
+          if (kb == t.kb - 1 || (PLANES > 1 && in_sum == kChunk - 1)) mma_commit(&bars.accfull[buf]);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) {  // products in flight still read shared and write tensor memory
+      give_up(&bars, lane);
+      const int64_t first = use > a.stages ? use - a.stages : 0;
+      for (int64_t u = first; u < use; ++u) mbar_wait_warp(&bars.empty[u % a.stages], (uint32_t)((u / a.stages) & 1), nullptr);
+    }
+  } else if (warp >= kEpiWarp0) {
+    // ---- results ----
+    const int w = warp - kEpiWarp0;
+    const int row = (w & 3) * 32 + lane;            // row of the tile: the accumulator's lane
+    const int c_lo = (w >> 2) * (a.bn / 2), c_hi = c_lo + a.bn / 2;
+    int64_t sums = 0;
+    bool ok = true;
+    for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
+      const Tile t = decode<KIND>(a, it);
+      float held[PLANES > 1 ? 64 : 1];  // sums of the finished accumulations (bn <= 128: 64 columns at most)
+      if (PLANES > 1) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) held[i] = 0.f;
+        for (int kb = 0; kb < t.kb; kb += kChunk, ++sums) {
+          const int buf = (int)(sums & 1);
+          ok = mbar_wait_warp(&bars.accfull[buf], (uint32_t)((sums >> 1) & 1), abort);
+          if (!ok) break;
+          tmem_fence_after();
+          const uint32_t acc = tmem + buf * 2 * a.bn + c_lo + ((uint32_t)((w & 3) * 32) << 16);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (c_lo + 32 * j < c_hi) {
+              float lead[32], rest[32];
+              tmem_ld32(acc + 32 * j, lead);
+              tmem_ld32(acc + a.bn + 32 * j, rest);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) held[32 * j + i] += lead[i] + rest[i];
+            }
+          tmem_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.accempty[buf]);
+        }
+      } else if (t.kb > 0) {
+        ok = mbar_wait_warp(&bars.accfull[sums & 1], (uint32_t)((sums >> 1) & 1), abort);
+        tmem_fence_after();
+      }
+      if (!ok) {
+        give_up(&bars, lane);
+        break;
+      }
+      const int buf = (int)(sums & 1);
+      if (PLANES == 1 && t.kb > 0) ++sums;
+      // where this thread's row goes
+      const int valid_rows = KIND == kWeights ? min(kBM, a.m - t.m0) : t.rows;
+      const bool live = row < valid_rows;
+      void* out = a.out;
+      int dt = a.out_dt, vec = a.vec;
+      int64_t at = 0;
+      if (KIND == kRows && live) {
+        at = (int64_t)__ldg(a.order + t.pos + row) * a.ldo;
+      } else if (KIND == kWeights) {
+        if (t.slot >= 0) {
+          out = a.part;
+          dt = GMMXX_FLOAT32;
+          vec = (a.n & 3) == 0;
+          at = ((int64_t)t.slot * a.m + t.m0 + row) * a.n;
+        } else {
+          at = t.g * a.out_stride + (int64_t)(t.m0 + row) * a.ldo;
+        }
+      }
+      const int n_left = a.n - t.n0;
+#pragma unroll
+      for (int j = 0; j < (PLANES > 1 ? 2 : 4); ++j) {
+        const int c = c_lo + 32 * j;
+        if (c >= c_hi) break;
+        float v[32];
+        __syncwarp();
+        if (PLANES > 1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = held[(32 * j + i) % (PLANES > 1 ? 64 : 1)];
+        } else if (t.kb > 0) {
+          tmem_ld32(tmem + buf * a.bn + c + ((uint32_t)((w & 3) * 32) << 16), v);
+          tmem_wait_ld();
+          if (c + 32 == c_hi) {  // the accumulator is in registers: free it for the tile after next
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.accempty[buf]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        }
+        const int nv = n_left - c;
+        if (!live || nv <= 0) continue;
+        if (KIND == kBatch) {
+          batch32<PLANES>(a, t, t.m0 + row, t.n0 + c, v, nv);
+        } else {
+          if (KIND == kRows && a.bias != nullptr && t.kb > 0) {
+            const int64_t b0 = (int64_t)t.g * a.n + t.n0 + c;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < nv) v[i] += load_x(a.bias, b0 + i, a.bias_dt);
+          }
+          store32(out, dt, at + t.n0 + c, v, nv, vec);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tmem_fence_before();
+  __syncthreads();
+  if (warp == 2) tmem_dealloc(tmem, tmem_cols);
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                             const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int encode(CUtensorMap* map, const void* base, int fp16, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+           const cuuint32_t* box) {
+  static const EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<EncodeFn>(p) : nullptr;
+  }();
+  if (fn == nullptr) return set_error(GMMXX_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint32_t es[3] = {1, 1, 1};
+  const CUresult rc = fn(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
+                         const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return set_error(GMMXX_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)rc);
+  return GMMXX_OK;
+}
+
+template <int KIND, int PLANES>
+int launch_one(const ProductMaps& maps, const ProductArgs& a, unsigned grid, cudaStream_t st) {
+  const int smem = a.stages * PLANES * (kABytes + a.bn * 128) + 1024;
+  if (int rc = allow_smem((const void*)product_kernel<KIND, PLANES>, smem)) return rc;
+  product_kernel<KIND, PLANES><<<grid, kThreadsTc, smem, st>>>(maps, a);
+  return check_launch("product_kernel");
+}
+
+}  // namespace
+
+// rows to gather: boxes of one row of 64 elements
+int encode_rows(CUtensorMap* map, const void* base, int fp16, int64_t cols, int64_t rows, int64_t ld) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {kBlockK, 1};
+  return encode(map, base, fp16, 2, dims, strides, box);
+}
+
+// a stack of matrices: boxes of 64 elements x box_rows rows of one matrix; what lies beyond a matrix reads as zero
+int encode_stack(CUtensorMap* map, const void* base, int fp16, int64_t cols, int64_t rows, int64_t ld, int64_t stack,
+                 int64_t stride, int box_rows) {
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)stack};
+  const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)stride * 2};
+  const cuuint32_t box[3] = {kBlockK, (cuuint32_t)box_rows, 1};
+  return encode(map, base, fp16, 3, dims, strides, box);
+}
+
+uint32_t product_idesc(int fp16, int bn, int a_mn, int b_mn) {
+  uint32_t d = idesc_bf16(kBM, bn, a_mn, b_mn);
+  if (fp16) d &= ~((1u << 7) | (1u << 10));  // A and B types: 0 = fp16, 1 = bf16
+  return d;
+}
+
+int product_stages(int planes, int bn) {
+  return std::min(kMaxStages, (kSmemLimit - 2048) / (planes * (kABytes + bn * 128)));
+}
+
+int device_sms(int* sms) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "device query: %s", cudaGetErrorString(e));
+  return GMMXX_OK;
+}
+
+int launch_product(Kind kind, int planes, const ProductMaps& maps, const ProductArgs& a, int64_t max_items,
+                   cudaStream_t st) {
+  int sms = 0;
+  if (int rc = device_sms(&sms)) return rc;
+  const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(sms, max_items * a.mt * a.nt));
+  if (kind == kRows) return planes == 1 ? launch_one<kRows, 1>(maps, a, grid, st) : launch_one<kRows, 3>(maps, a, grid, st);
+  if (kind == kWeights)
+    return planes == 1 ? launch_one<kWeights, 1>(maps, a, grid, st) : launch_one<kWeights, 3>(maps, a, grid, st);
+  return planes == 1 ? launch_one<kBatch, 1>(maps, a, grid, st) : launch_one<kBatch, 2>(maps, a, grid, st);
+}
+
+int read_status(int* out, cudaStream_t st) {
+  int v = 0;
+  const int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, g_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && v != 0) e = cudaMemcpyToSymbolAsync(g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+  if (e == cudaSuccess && v != 0) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "status read: %s", cudaGetErrorString(e));
+  *out = v != 0 ? GMMXX_ERR_TIMEOUT : GMMXX_OK;
+  return GMMXX_OK;
+}
+
+}  // namespace experts
+}  // namespace gmmxx

@@ -1,0 +1,71 @@
+// experts_tc.cuh -- the tensor-core product kernel behind the routed products
+// and the Newton-Schulz iteration: argument block and launcher.
+#pragma once
+
+#include "experts_api.cuh"
+
+#include <cuda.h>
+
+namespace gmmxx {
+namespace experts {
+
+// What a launch multiplies.  kRows: gathered rows x their group's matrix
+// (forward, and the rows' gradient).  kWeights: a group's gathered rows,
+// transposed, x its gathered gradients (the matrices' gradient).  kBatch: a
+// stack of matrices (Newton-Schulz).
+enum Kind { kRows = 0, kWeights = 1, kBatch = 2 };
+
+constexpr int kBlockK = 64;      // contraction elements of one stage: 128 bytes of a 16-bit plane
+constexpr float kPlaneScale = 4096.f;  // Newton-Schulz planes hold value * 4096 (see experts_tc.cu)
+
+struct ProductArgs {
+  // tiles of the output and of the contraction
+  int m, n;        // output extents (kRows: n only)
+  int k;           // contraction length (kWeights: per segment)
+  int bn;          // tile columns: 64, 128 or 256
+  int stages;
+  int mt, nt;      // tiles along m and n
+  int a_mn, b_mn;  // operand contiguous along M / N instead of K
+  uint32_t idesc;  // tcgen05 instruction descriptor (types, majors, M = 128, N = bn)
+  int64_t items;   // kBatch: matrices; otherwise read from the tables
+  // routing
+  const int32_t* order;
+  const int32_t* table;  // kRows: tiles; kWeights: segments
+  int div_a, div_b;      // gathered row = order[position] / div
+  int groups;
+  // result
+  void* out;
+  int out_dt;
+  int64_t ldo;           // elements between rows of out
+  int64_t out_stride;    // elements between matrices of out (kWeights, kBatch)
+  int vec;               // 16-byte stores allowed
+  const void* bias;
+  int bias_dt;
+  float* part;           // kWeights: fp32 partials of split groups
+  // kBatch epilogue: v = beta * e + alpha * acc / kPlaneScale, to planes o or (out != NULL) to out / kPlaneScale
+  const __half* e[2];
+  __half* o[2];
+  int64_t ldp, p_stride;
+  float alpha, beta;
+};
+
+struct ProductMaps {
+  CUtensorMap a[3], b[3];
+};
+
+// segments of the matrices' gradient (device table): [0] their number, then
+// per segment {group, first position, rows, partial slot or -1}
+constexpr int kSegHeader = 4;
+constexpr int kSegInts = 4;
+
+int encode_rows(CUtensorMap* map, const void* base, int fp16, int64_t cols, int64_t rows, int64_t ld);
+int encode_stack(CUtensorMap* map, const void* base, int fp16, int64_t cols, int64_t rows, int64_t ld, int64_t stack,
+                 int64_t stride, int box_rows);
+uint32_t product_idesc(int fp16, int bn, int a_mn, int b_mn);
+int product_stages(int planes, int bn);
+int launch_product(Kind kind, int planes, const ProductMaps& maps, const ProductArgs& a, int64_t max_items,
+                   cudaStream_t st);
+int device_sms(int* sms);
+
+}  // namespace experts
+}  // namespace gmmxx

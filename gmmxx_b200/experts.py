@@ -65,7 +65,7 @@ def _check_float(t, name: str) -> torch.Tensor:
     t = _check(t, name)
     if t.dtype not in engine._X_DTYPES:
         raise TypeError(f"{name} dtype {t.dtype} not supported (float32, bfloat16, float16)")
-    return t
+    return t.clone() if t.data_ptr() % 16 else t  # the kernels load from 16-byte boundaries
 
 
 def _same_device(dev: torch.device, **tensors) -> None:
@@ -78,6 +78,20 @@ def _workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
     # of its own per call, from the caching allocator: calls on several streams
     # and captured graphs never share one
     return torch.empty(max(256, nbytes), dtype=torch.uint8, device=dev)
+
+
+def check_products_status(device=None) -> None:
+    """Raise GmmxxError when a bounded device-side wait ran out in a product or
+    orthogonalisation kernel of ``device`` (default: the current one) since the
+    last check; their results are undefined then.  Synchronises the current
+    stream."""
+    require_cuda()
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    status = engine.ctypes_int()
+    with torch.cuda.device(dev):
+        nat.call("gmmxx_products_status", status.ref(), engine._stream_ptr(dev))
+    if status.value != nat.OK:
+        raise nat.GmmxxError(status.value, "a bounded device-side wait expired in a product kernel")
 
 
 def group_rows(labels: torch.Tensor, n_groups: int) -> RowGroups:

@@ -276,7 +276,10 @@ GMMXX_API int gmmxx_label_stats(int x_dtype, const void* x, int64_t B, int64_t N
  * writes them, or top_k labels per row); a *slot* is one (row, choice) pair,
  * slot = row * top_k + choice.  gmmxx_group_rows sorts the slots by component;
  * the products take its order / offsets / tiles.  dtype is the type of x,
- * weight, bias, gradients and outputs (gmmxx_dtype); sums are fp32.
+ * weight, bias, gradients and outputs (gmmxx_dtype); sums are fp32.  x, weight
+ * and grad_out start on 16-byte boundaries.  fp32 factors are multiplied as
+ * three bf16 planes: products as exact as fp32's, but an infinite factor gives
+ * NaN where fp32 would give infinity.
  *
  * gmmxx_group_rows: labels (slots) int32 or int64 (label_bytes 4 / 8); a label
  *   outside [0, K) leaves its slot unassigned.  order_out (slots): the slots
@@ -313,6 +316,11 @@ GMMXX_API int gmmxx_grouped_matmul_backward(int dtype, const void* grad_out, con
                                             const void* weight, int weight_transposed, void* grad_x,
                                             void* grad_weight, void* grad_bias, void* workspace,
                                             size_t workspace_bytes, void* stream);
+
+/* GMMXX_OK, or GMMXX_ERR_TIMEOUT when a bounded device-side wait ran out in a
+ * product or orthogonalisation kernel of the current device since the last
+ * call (those kernels' results are undefined).  Synchronises the stream. */
+GMMXX_API int gmmxx_products_status(int* status_out, void* stream);
 
 /* Newton-Schulz orthogonalisation of a stack of matrices g (batch, m, n):
  * X = g / (|g|_F + eps), then `steps` times X <- a X + (b P + c P^2) X with
