@@ -40,15 +40,16 @@ __device__ __forceinline__ void split3(float x, uint32_t* h) {
   h[2] = __float_as_uint(r - __uint_as_float(rb & 0xffff0000u)) >> 16;
 }
 
-// [rows][cols] of any type -> 1 plane (16-bit types, copied) or 3 (fp32) of rows of ld elements
+// [rows][cols] of any type -> 1 plane (16-bit types, copied) or 3 (fp32) of
+// rows of ld elements; with `order` row i is the source's row order[i] / div
 __global__ void __launch_bounds__(256) pack_kernel(const void* src, int f32, int64_t rows, int cols, int ld,
-                                                   uint16_t* dst, int64_t plane) {
+                                                   const int32_t* order, int div, uint16_t* dst, int64_t plane) {
   const int per = ld / 8;
   const int64_t n = rows * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / per;
     const int c = (int)(i % per) * 8;
-    const int64_t at = r * cols + c;
+    const int64_t at = (order != nullptr ? order[r] / div : r) * cols + c;
     uint32_t q[3][4] = {};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -75,7 +76,8 @@ struct Planes {
   int fp16;
 };
 
-int operand(int dt, const void* src, int64_t rows, int64_t cols, char*& ws, Planes* out, cudaStream_t st) {
+int operand(int dt, const void* src, int64_t rows, int64_t cols, const int32_t* order, int div, char*& ws, Planes* out,
+            cudaStream_t st) {
   out->fp16 = dt == GMMXX_FLOAT16;
   out->n = planes_of(dt);
   if (direct(dt, cols)) {
@@ -88,16 +90,20 @@ int operand(int dt, const void* src, int64_t rows, int64_t cols, char*& ws, Plan
   for (int p = 0; p < out->n; ++p) out->base[p] = ws + p * plane;
   const int64_t blocks = std::min<int64_t>(148 * 16, ceil_div(rows * out->ld / 8, 256));
   if (blocks > 0)
-    pack_kernel<<<(unsigned)blocks, 256, 0, st>>>(src, dt == GMMXX_FLOAT32, rows, (int)cols, (int)out->ld,
+    pack_kernel<<<(unsigned)blocks, 256, 0, st>>>(src, dt == GMMXX_FLOAT32, rows, (int)cols, (int)out->ld, order, div,
                                                   reinterpret_cast<uint16_t*>(ws), plane / 2);
   ws += plane * out->n;
   return check_launch("pack_kernel");
 }
 
-int rows_maps(const Planes& p, int64_t cols, int64_t rows, CUtensorMap* maps) {
-  for (int i = 0; i < p.n; ++i)
-    if (int rc = encode_rows(&maps[i], p.base[i], p.fp16, cols, rows, p.ld)) return rc;
-  return GMMXX_OK;
+// routed rows: fp32 ones as sorted planes (slots rows), 16-bit ones where they lie
+int routed(int dt, const void* src, int64_t rows, int64_t cols, const Groups& g, int div, char*& ws, Planes* out,
+           cudaStream_t st) {
+  if (dt == GMMXX_FLOAT32) return operand(dt, src, g.slots(), cols, g.order, div, ws, out, st);
+  return operand(dt, src, rows, cols, nullptr, 1, ws, out, st);
+}
+int64_t routed_bytes(int dt, int64_t rows, int64_t cols, const Groups& g) {
+  return pack_bytes(dt, dt == GMMXX_FLOAT32 ? g.slots() : rows, cols);
 }
 
 int stack_maps(const Planes& p, int64_t cols, int64_t rows, int64_t stack, int box_rows, CUtensorMap* maps) {
@@ -126,11 +132,12 @@ bool vec_ok(const void* p, int dt, int64_t ld) {
 // ---------------------------------------------------------------------------
 
 // out[slot] = src[slot / div] . W, W (K, k_dim, n) when !b_kmajor, (K, n, k_dim) when b_kmajor
-int rows_product(int dt, const Planes& src, int64_t src_rows, int div, const Groups& g, int64_t k_dim, int64_t n,
+int rows_product(int dt, const Planes& src, int div, const Groups& g, int64_t k_dim, int64_t n,
                  const Planes& w, bool b_kmajor, const void* bias, void* out, int out_dt, cudaStream_t st) {
   const int bn = tile_columns(ceil_div(g.slots(), kTileRows), n, src.n, 256);
   ProductMaps maps;
-  if (int rc = rows_maps(src, k_dim, src_rows, maps.a)) return rc;
+  if (src.n > 1)
+    if (int rc = stack_maps(src, k_dim, g.slots(), 1, kTileRows, maps.a)) return rc;
   if (int rc = b_kmajor ? stack_maps(w, k_dim, n, g.K, bn, maps.b) : stack_maps(w, n, k_dim, g.K, kBlockK, maps.b))
     return rc;
   ProductArgs a{};
@@ -143,6 +150,8 @@ int rows_product(int dt, const Planes& src, int64_t src_rows, int div, const Gro
   a.b_mn = b_kmajor ? 0 : 1;
   a.idesc = product_idesc(src.fp16, bn, 0, a.b_mn);
   a.order = g.order;
+  a.src_a = static_cast<const char*>(src.base[0]);
+  a.ld_a = src.ld;
   a.table = g.tiles;
   a.div_a = div;
   a.div_b = 1;
@@ -391,21 +400,21 @@ int stack_operand(const Stack& s, int planes, int64_t batch, int box_rows, CUten
 size_t grouped_matmul_ws(int dt, const Groups& g, int64_t n_in, int64_t n_out) {
   // the weight's inner length is n_out or (transposed) n_in: room for either
   const int64_t w = std::max(pack_bytes(dt, g.K * n_in, n_out), pack_bytes(dt, g.K * n_out, n_in));
-  return (size_t)(256 + pack_bytes(dt, g.rows, n_in) + w);
+  return (size_t)(256 + routed_bytes(dt, g.rows, n_in, g) + w);
 }
 
 int launch_grouped_matmul(int dt, const void* x, const Groups& g, int64_t n_in, int64_t n_out, const void* w, int wt,
                           const void* bias, void* out, char* ws, cudaStream_t st) {
   Planes px, pw;
-  if (int rc = operand(dt, x, g.rows, n_in, ws, &px, st)) return rc;
-  if (int rc = operand(dt, w, g.K * (wt ? n_out : n_in), wt ? n_in : n_out, ws, &pw, st)) return rc;
-  return rows_product(dt, px, g.rows, g.top, g, n_in, n_out, pw, wt != 0, bias, out, dt, st);
+  if (int rc = routed(dt, x, g.rows, n_in, g, g.top, ws, &px, st)) return rc;
+  if (int rc = operand(dt, w, g.K * (wt ? n_out : n_in), wt ? n_in : n_out, nullptr, 1, ws, &pw, st)) return rc;
+  return rows_product(dt, px, g.top, g, n_in, n_out, pw, wt != 0, bias, out, dt, st);
 }
 
 size_t grouped_backward_ws(int dt, const Groups& g, int64_t n_in, int64_t n_out) {
   const SegPlan p = seg_plan(g, n_in, n_out);
   const int64_t w = std::max(pack_bytes(dt, g.K * n_in, n_out), pack_bytes(dt, g.K * n_out, n_in));
-  return (size_t)(256 + pack_bytes(dt, g.slots(), n_out) + w + pack_bytes(dt, g.rows, n_in) +
+  return (size_t)(256 + pack_bytes(dt, g.slots(), n_out) + w + routed_bytes(dt, g.rows, n_in, g) +
                   (g.top > 1 ? al256(g.slots() * n_in * 4) : 0) + al256((kSegHeader + kSegInts * p.max_segs) * 4) +
                   al256(p.max_split * 16) + al256(p.max_slots * n_in * n_out * 4) + al256(p.max_slots * n_out * 4));
 }
@@ -415,15 +424,15 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
   Planes pg, pw, px;
   const int64_t slots = g.slots();
   if (slots > 0 && (gx != nullptr || gw != nullptr))
-    if (int rc = operand(dt, gy, slots, n_out, ws, &pg, st)) return rc;
+    if (int rc = routed(dt, gy, slots, n_out, g, 1, ws, &pg, st)) return rc;
   if (slots > 0 && gx != nullptr) {
-    if (int rc = operand(dt, w, g.K * (wt ? n_out : n_in), wt ? n_in : n_out, ws, &pw, st)) return rc;
+    if (int rc = operand(dt, w, g.K * (wt ? n_out : n_in), wt ? n_in : n_out, nullptr, 1, ws, &pw, st)) return rc;
     void* to = gx;
     if (g.top > 1) {
       to = ws;
       ws += al256(slots * n_in * 4);
     }
-    if (int rc = rows_product(dt, pg, slots, 1, g, n_out, n_in, pw, wt == 0, nullptr, to,
+    if (int rc = rows_product(dt, pg, 1, g, n_out, n_in, pw, wt == 0, nullptr, to,
                               g.top > 1 ? GMMXX_FLOAT32 : dt, st))
       return rc;
     if (g.top > 1) {
@@ -451,14 +460,16 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
   segments_kernel<<<1, 1024, 0, st>>>(g.offsets, g.K, (int)p.seg, table, split);
   if (int rc = check_launch("segments_kernel")) return rc;
   if (gw != nullptr) {
-    if (int rc = operand(dt, x, g.rows, n_in, ws, &px, st)) return rc;
+    if (int rc = routed(dt, x, g.rows, n_in, g, g.top, ws, &px, st)) return rc;
     // (n_in x n_out) = x^T gy; for a transposed weight (n_out x n_in) = gy^T x
     const int64_t m = wt ? n_out : n_in, n = wt ? n_in : n_out;
     const int planes = planes_of(dt);
     const int bn = tile_columns(p.max_segs * ceil_div(m, 128), n, planes, 256);
     ProductMaps maps;
-    if (int rc = rows_maps(px, n_in, g.rows, wt ? maps.b : maps.a)) return rc;
-    if (int rc = rows_maps(pg, n_out, slots, wt ? maps.a : maps.b)) return rc;
+    if (planes > 1) {
+      if (int rc = stack_maps(px, n_in, slots, 1, kBlockK, wt ? maps.b : maps.a)) return rc;
+      if (int rc = stack_maps(pg, n_out, slots, 1, kBlockK, wt ? maps.a : maps.b)) return rc;
+    }
     ProductArgs a{};
     a.m = (int)m;
     a.n = (int)n;
@@ -469,6 +480,11 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
     a.a_mn = a.b_mn = 1;
     a.idesc = product_idesc(px.fp16, bn, 1, 1);
     a.order = g.order;
+    const Planes &pa = wt ? pg : px, &pb = wt ? px : pg;
+    a.src_a = static_cast<const char*>(pa.base[0]);
+    a.src_b = static_cast<const char*>(pb.base[0]);
+    a.ld_a = pa.ld;
+    a.ld_b = pb.ld;
     a.table = table;
     a.div_a = wt ? 1 : g.top;
     a.div_b = wt ? g.top : 1;

@@ -8,16 +8,18 @@
 // thread issues tcgen05.mma, and eight epilogue warps drain one accumulator
 // from tensor memory while the next tile's products go to the other.
 //
-// Routed rows are never copied: the TMA's gather (tile::gather4, four rows of
-// 128 bytes per instruction) fetches each row where it lies, for kRows as the
+// Routed rows of 16-bit types are never copied: four warps fetch each row where
+// it lies with 16-byte cp.async into the swizzled stage, for kRows as the
 // K-major A operand, for kWeights -- where the rows are the contraction -- as
-// MN-major A and B operands.  Both are the same bytes in shared memory (rows
-// of 64 elements, swizzled), read through different descriptors.
-//
-// Ragged ends.  kRows: rows behind the tile's last are fetched as copies of
-// its first and not stored.  kWeights: the last stage of a segment issues only
-// the 16-row steps that hold rows, and the rest of its last step is zeroed in
-// both operands first (zeroing one would leave NaN * 0).
+// MN-major A and B operands.  (TMA's gather of four rows per instruction took
+// about 80 cycles an instruction, 6 B per cycle and SM, and held the tensor pipe
+// at 18 % and 7 %.)  The copies complete on the stage's mbarrier; the thread that
+// issues the products fences the proxies after it has waited.  Rows behind a
+// segment's last are filled with zeros; kRows fetches copies of the tile's first
+// row there and does not store them.  Planes of fp32 rows are laid out sorted
+// before the launch and loaded as TMA tiles; there the last stage of a kWeights
+// segment also holds the next group's rows, which are zeroed in both operands
+// before the products (zeroing one would leave NaN * 0).
 //
 // Sums.  The tensor core adds to an accumulator by cutting, not rounding: an
 // addition costs about 3.4e-8 of the sum, always towards zero (measured: 8e-7
@@ -50,7 +52,7 @@ __device__ int g_status = 0;  // sticky: 1 when a bounded wait ran out (gmmxx_pr
 namespace {
 
 constexpr int kBM = 128;
-constexpr int kThreadsTc = 384;
+constexpr int kGatherWarp0 = 12, kGatherThreads = 128;
 constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
 constexpr int kABytes = kBM * 128;  // one plane of A per stage
 constexpr int kMaxStages = 8;
@@ -64,12 +66,13 @@ struct Bars {
   int abort;
 };
 
-__device__ __forceinline__ void gather4(void* dst, const CUtensorMap* map, int x, const int* r, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-      "%4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(smem_u32(bar))
-      : "memory");
+// 16 bytes to shared memory, or zeros
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+// arrives on the barrier when this thread's copies so far have landed
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
@@ -223,8 +226,17 @@ __device__ __forceinline__ void batch32(const ProductArgs& a, const Tile& t, int
 }
 
 template <int KIND, int PLANES>
-__global__ void __launch_bounds__(kThreadsTc, 1)
+struct Roles {
+  static constexpr bool kGather = KIND != kBatch && PLANES == 1;      // rows by cp.async
+  static constexpr bool kTma = !(KIND == kWeights && PLANES == 1);    // something by TMA
+  static constexpr int kThreads = kGather ? 512 : 384;
+  static constexpr int kFullCount = (kGather ? kGatherThreads : 0) + (kTma ? 1 : 0);
+};
+
+template <int KIND, int PLANES>
+__global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
     product_kernel(const __grid_constant__ ProductMaps maps, const ProductArgs a) {
+  using R = Roles<KIND, PLANES>;
   extern __shared__ __align__(1024) char smem_raw[];
   __shared__ Bars bars;
   char* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -238,7 +250,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
-      mbar_init(&bars.full[i], 1);
+      mbar_init(&bars.full[i], R::kFullCount);
       mbar_init(&bars.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -254,69 +266,47 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
   const uint32_t tmem = bars.tmem_base;
   const int64_t total = tile_count<KIND>(a);
 
-  if (warp == 0) {
-    // ---- loads ----
+  if (R::kTma && warp == 0) {
+    // ---- tiled loads: kRows' matrices, sorted planes, stacks ----
     if (lane < PLANES) {
-      prefetch_tmap(&maps.a[lane]);
+      if (!R::kGather) prefetch_tmap(&maps.a[lane]);
       prefetch_tmap(&maps.b[lane]);
     }
     int64_t fill = 0;  // stages filled so far
     bool ok = true;
-    const int quad = lane & 15, half = lane >> 4;
+    const uint32_t bytes = (uint32_t)(R::kGather ? bbytes : stage_bytes);
     for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
       const Tile t = decode<KIND>(a, it);
-      if (t.kb == 0) continue;
-      int ra[4], rb[4], next[4];
-      if (KIND == kRows) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 4 * lane + i;
-          ra[i] = __ldg(a.order + t.pos + (r < t.rows ? r : 0)) / a.div_a;
-        }
-      } else if (KIND == kWeights) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) next[i] = __ldg(a.order + t.pos + min(4 * quad + i, t.rows - 1));
-      }
       for (int kb = 0; kb < t.kb; ++kb, ++fill) {
         const int s = (int)(fill % a.stages);
-        const uint32_t ph = (uint32_t)((fill / a.stages) & 1);
-        if (KIND == kWeights) {  // this stage's rows; the next stage's are fetched meanwhile
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            ra[i] = next[i] / a.div_a;
-            rb[i] = next[i] / a.div_b;
-            next[i] = __ldg(a.order + t.pos + min((kb + 1) * kBlockK + 4 * quad + i, t.rows - 1));
-          }
-        }
-        ok = mbar_wait_warp(&bars.empty[s], ph ^ 1, abort);
+        ok = mbar_wait_warp(&bars.empty[s], (uint32_t)((fill / a.stages) & 1) ^ 1, abort);
         if (!ok) break;
         char* sa = sm + s * stage_bytes;
         char* sb = sa + PLANES * kABytes;
         uint64_t* bar = &bars.full[s];
-        if (lane == 0) mbar_expect_tx(bar, (uint32_t)stage_bytes);
+        if (lane == 0) mbar_expect_tx(bar, bytes);
         __syncwarp();
         const int k0 = kb * kBlockK;
 #pragma unroll
         for (int p = 0; p < PLANES; ++p) {
           char* pa = sa + p * kABytes;
           char* pb = sb + p * bbytes;
+          if (KIND == kWeights) {  // 64 sorted rows x 64 columns per box
+            if (lane < 2) tma_load_3d(pa + lane * 8192, &maps.a[p], t.m0 + lane * 64, t.pos + k0, 0, bar);
+            if (lane < a.bn / 64) tma_load_3d(pb + lane * 8192, &maps.b[p], t.n0 + lane * 64, t.pos + k0, 0, bar);
+            continue;
+          }
           if (KIND == kRows) {
-            gather4(pa + lane * 512, &maps.a[p], k0, ra, bar);
-          } else if (KIND == kWeights) {
-            gather4(pa + half * 8192 + quad * 512, &maps.a[p], t.m0 + half * 64, ra, bar);
-            for (int j = half; j < a.bn / 64; j += 2)
-              gather4(pb + j * 8192 + quad * 512, &maps.b[p], t.n0 + j * 64, rb, bar);
+            if (!R::kGather && lane == 0) tma_load_3d(pa, &maps.a[p], k0, t.pos, 0, bar);
           } else if (a.a_mn) {
             if (lane < 2) tma_load_3d(pa + lane * 8192, &maps.a[p], t.m0 + lane * 64, k0, t.g, bar);
           } else {
             if (lane == 0) tma_load_3d(pa, &maps.a[p], k0, t.m0, t.g, bar);
           }
-          if (KIND != kWeights) {
-            if (a.b_mn) {
-              if (lane < a.bn / 64) tma_load_3d(pb + lane * 8192, &maps.b[p], t.n0 + lane * 64, k0, t.g, bar);
-            } else {
-              if (lane == 0) tma_load_3d(pb, &maps.b[p], k0, t.n0, t.g, bar);
-            }
+          if (a.b_mn) {
+            if (lane < a.bn / 64) tma_load_3d(pb + lane * 8192, &maps.b[p], t.n0 + lane * 64, k0, t.g, bar);
+          } else {
+            if (lane == 0) tma_load_3d(pb, &maps.b[p], k0, t.n0, t.g, bar);
           }
         }
       }
@@ -354,8 +344,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         int steps = 4;
         if (KIND == kWeights) {
           const int left = t.rows - kb * kBlockK;
-          if (left < kBlockK) {
-            steps = (left + 15) >> 4;
+          if (left < kBlockK) steps = (left + 15) >> 4;
+          if (!R::kGather && left < kBlockK) {
             const int zero = steps * 16 - left;  // rows to clear, of 128 bytes in each 64-column group
             if (zero > 0) {
               const int groups = PLANES * (2 + a.bn / 64);
@@ -370,6 +360,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
           }
         }
         if (lane == 0) {
+          if (R::kGather) fence_proxy_async();  // cp.async wrote through the generic proxy
           tmem_fence_after();
           constexpr int kPairs = PLANES == 1 ? 1 : PLANES == 2 ? 3 : 6;
 #pragma unroll
@@ -393,7 +384,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       const int64_t first = use > a.stages ? use - a.stages : 0;
       for (int64_t u = first; u < use; ++u) mbar_wait_warp(&bars.empty[u % a.stages], (uint32_t)((u / a.stages) & 1), nullptr);
     }
-  } else if (warp >= kEpiWarp0) {
+  } else if (warp >= kEpiWarp0 && warp < kEpiWarp0 + kEpiWarps) {
     // ---- results ----
     const int w = warp - kEpiWarp0;
     const int row = (w & 3) * 32 + lane;            // row of the tile: the accumulator's lane
@@ -492,6 +483,74 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
       }
     }
   }
+  if (R::kGather && warp >= kGatherWarp0) {
+    // ---- gathered rows: thread = 16-byte piece `q` of every 16th row ----
+    const int tid = threadIdx.x - kGatherWarp0 * 32, q = tid & 7, r0 = tid >> 3;
+    const uint32_t at = (uint32_t)(r0 * 128 + ((q ^ (r0 & 7)) << 4));  // 128-byte swizzle; rows r0 + 16 i: + 2048 i
+    int64_t fill = 0;
+    bool ok = true;
+    for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
+      const Tile t = decode<KIND>(a, it);
+      if (t.kb == 0) continue;
+      if (KIND == kRows) {
+        const char* src[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = r0 + 16 * i;
+          src[i] = a.src_a + ((int64_t)(__ldg(a.order + t.pos + (r < t.rows ? r : 0)) / a.div_a) * a.ld_a + q * 8) * 2;
+        }
+        for (int kb = 0; kb < t.kb; ++kb, ++fill) {
+          const int s = (int)(fill % a.stages);
+          ok = mbar_wait_warp(&bars.empty[s], (uint32_t)((fill / a.stages) & 1) ^ 1, abort);
+          if (!ok) break;
+          const uint32_t sa = smem_u32(sm) + s * stage_bytes + at;
+          const bool live = kb * kBlockK + q * 8 < a.k;
+          const int64_t k0 = live ? (int64_t)kb * (kBlockK * 2) : 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) copy16(sa + 2048 * i, src[i] + k0, live);
+          copies_arrive(&bars.full[s]);
+        }
+      } else {
+        int next[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) next[i] = __ldg(a.order + t.pos + min(r0 + 16 * i, t.rows - 1));
+        for (int kb = 0; kb < t.kb; ++kb, ++fill) {
+          const int s = (int)(fill % a.stages);
+          const char *pa[4], *pb[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {  // this stage's rows; the next stage's are fetched meanwhile
+            pa[i] = a.src_a + ((int64_t)(next[i] / a.div_a) * a.ld_a + q * 8 + t.m0) * 2;
+            pb[i] = a.src_b + ((int64_t)(next[i] / a.div_b) * a.ld_b + q * 8 + t.n0) * 2;
+            next[i] = __ldg(a.order + t.pos + min((kb + 1) * kBlockK + r0 + 16 * i, t.rows - 1));
+          }
+          ok = mbar_wait_warp(&bars.empty[s], (uint32_t)((fill / a.stages) & 1) ^ 1, abort);
+          if (!ok) break;
+          const uint32_t sa = smem_u32(sm) + s * stage_bytes + at, sb = sa + kABytes;
+          const int left = t.rows - kb * kBlockK - r0;  // rows r0 + 16 i < left are the segment's
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const bool in = t.m0 + g * 64 + q * 8 < a.m;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool live = in && 16 * i < left;
+              copy16(sa + g * 8192 + 2048 * i, live ? pa[i] + g * 128 : a.src_a, live);
+            }
+          }
+          for (int g = 0; g < a.bn / 64; ++g) {
+            const bool in = t.n0 + g * 64 + q * 8 < a.n;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool live = in && 16 * i < left;
+              copy16(sb + g * 8192 + 2048 * i, live ? pb[i] + g * 128 : a.src_b, live);
+            }
+          }
+          copies_arrive(&bars.full[s]);
+        }
+      }
+    }
+    if (!ok && lane == 0) give_up(&bars, lane);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
   __syncwarp();
   tmem_fence_before();
   __syncthreads();
@@ -525,19 +584,11 @@ template <int KIND, int PLANES>
 int launch_one(const ProductMaps& maps, const ProductArgs& a, unsigned grid, cudaStream_t st) {
   const int smem = a.stages * PLANES * (kABytes + a.bn * 128) + 1024;
   if (int rc = allow_smem((const void*)product_kernel<KIND, PLANES>, smem)) return rc;
-  product_kernel<KIND, PLANES><<<grid, kThreadsTc, smem, st>>>(maps, a);
+  product_kernel<KIND, PLANES><<<grid, Roles<KIND, PLANES>::kThreads, smem, st>>>(maps, a);
   return check_launch("product_kernel");
 }
 
 }  // namespace
-
-// rows to gather: boxes of one row of 64 elements
-int encode_rows(CUtensorMap* map, const void* base, int fp16, int64_t cols, int64_t rows, int64_t ld) {
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {kBlockK, 1};
-  return encode(map, base, fp16, 2, dims, strides, box);
-}
 
 // a stack of matrices: boxes of 64 elements x box_rows rows of one matrix; what lies beyond a matrix reads as zero
 int encode_stack(CUtensorMap* map, const void* base, int fp16, int64_t cols, int64_t rows, int64_t ld, int64_t stack,

@@ -30,6 +30,8 @@ struct ProductArgs {
   int64_t items;   // kBatch: matrices; otherwise read from the tables
   // routing
   const int32_t* order;
+  const char *src_a, *src_b;  // 16-bit rows fetched by cp.async (one plane): 16-byte aligned,
+  int64_t ld_a, ld_b;         // rows of ld elements (a multiple of 8)
   const int32_t* table;  // kRows: tiles; kWeights: segments
   int div_a, div_b;      // gathered row = order[position] / div
   int groups;
@@ -58,7 +60,6 @@ struct ProductMaps {
 constexpr int kSegHeader = 4;
 constexpr int kSegInts = 4;
 
-int encode_rows(CUtensorMap* map, const void* base, int fp16, int64_t cols, int64_t rows, int64_t ld);
 int encode_stack(CUtensorMap* map, const void* base, int fp16, int64_t cols, int64_t rows, int64_t ld, int64_t stack,
                  int64_t stride, int box_rows);
 uint32_t product_idesc(int fp16, int bn, int a_mn, int b_mn);
