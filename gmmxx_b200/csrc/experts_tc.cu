@@ -93,6 +93,18 @@ __device__ __forceinline__ void give_up(Bars* bars, int lane) {
   }
 }
 
+// position in the ring of stages (or of the two accumulators): index and phase, counted without divisions
+struct Ring {
+  int i = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void step(int n) {
+    if (++i == n) {
+      i = 0;
+      phase ^= 1;
+    }
+  }
+};
+
 // one output tile
 struct Tile {
   int g;       // group / matrix
@@ -272,14 +284,15 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
       if (!R::kGather) prefetch_tmap(&maps.a[lane]);
       prefetch_tmap(&maps.b[lane]);
     }
-    int64_t fill = 0;  // stages filled so far
+    Ring ring;
+    int64_t filled = 0;
     bool ok = true;
     const uint32_t bytes = (uint32_t)(R::kGather ? bbytes : stage_bytes);
     for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
       const Tile t = decode<KIND>(a, it);
-      for (int kb = 0; kb < t.kb; ++kb, ++fill) {
-        const int s = (int)(fill % a.stages);
-        ok = mbar_wait_warp(&bars.empty[s], (uint32_t)((fill / a.stages) & 1) ^ 1, abort);
+      for (int kb = 0; kb < t.kb; ++kb, ring.step(a.stages), ++filled) {
+        const int s = ring.i;
+        ok = mbar_wait_warp(&bars.empty[s], ring.phase ^ 1, abort);
         if (!ok) break;
         char* sa = sm + s * stage_bytes;
         char* sb = sa + PLANES * kABytes;
@@ -313,34 +326,38 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
     }
     if (!ok) {  // the copies in flight still write shared memory: wait for them before the block ends
       give_up(&bars, lane);
-      const int64_t first = fill > a.stages ? fill - a.stages : 0;
-      for (int64_t f = first; f < fill; ++f) mbar_wait_warp(&bars.full[f % a.stages], (uint32_t)((f / a.stages) & 1), nullptr);
+      const int64_t first = filled > a.stages ? filled - a.stages : 0;
+      for (int64_t f = first; f < filled; ++f) mbar_wait_warp(&bars.full[f % a.stages], (uint32_t)((f / a.stages) & 1), nullptr);
     }
   } else if (warp == 1) {
     // ---- products ----
-    int64_t use = 0, sums = 0;
+    Ring ring, sums;
+    int64_t use = 0;
     bool ok = true;
-    const uint32_t step_a = a.a_mn ? 2048 : 32, step_b = a.b_mn ? 2048 : 32;  // bytes per 16 contraction elements
+    // descriptor units (16 bytes) per 16 contraction elements
+    const uint32_t step_a = (a.a_mn ? 2048 : 32) >> 4, step_b = (a.b_mn ? 2048 : 32) >> 4;
+    const uint64_t desc_a = a.a_mn ? desc_mnmajor(smem_u32(sm), 8192) : desc_kmajor(smem_u32(sm));
+    const uint32_t sb0 = smem_u32(sm) + PLANES * kABytes;
+    const uint64_t desc_b = a.b_mn ? desc_mnmajor(sb0, 8192) : desc_kmajor(sb0);
+    const uint32_t stage_units = (uint32_t)stage_bytes >> 4, b_units = (uint32_t)bbytes >> 4;
+    const uint32_t idesc = a.idesc;
     for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
       const Tile t = decode<KIND>(a, it);
-      if (t.kb == 0) continue;
       int buf = 0;
       uint32_t d = 0;
-      for (int kb = 0; kb < t.kb; ++kb, ++use) {
+      for (int kb = 0; kb < t.kb; ++kb, ring.step(a.stages), ++use) {
         const int in_sum = PLANES > 1 ? kb % kChunk : kb;  // stages already in this accumulator
         if (in_sum == 0) {
-          buf = (int)(sums & 1);
-          ok = mbar_wait_warp(&bars.accempty[buf], (uint32_t)(((sums >> 1) & 1) ^ 1), abort);
+          buf = sums.i;
+          ok = mbar_wait_warp(&bars.accempty[buf], sums.phase ^ 1, abort);
           if (!ok) break;
           tmem_fence_after();
           d = tmem + buf * kAccs * a.bn;
-          ++sums;
+          sums.step(2);
         }
-        const int s = (int)(use % a.stages);
-        ok = mbar_wait_warp(&bars.full[s], (uint32_t)((use / a.stages) & 1), abort);
+        const int s = ring.i;
+        ok = mbar_wait_warp(&bars.full[s], ring.phase, abort);
         if (!ok) break;
-        char* sa = sm + s * stage_bytes;
-        char* sb = sa + PLANES * kABytes;
         int steps = 4;
         if (KIND == kWeights) {
           const int left = t.rows - kb * kBlockK;
@@ -348,6 +365,8 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
           if (!R::kGather && left < kBlockK) {
             const int zero = steps * 16 - left;  // rows to clear, of 128 bytes in each 64-column group
             if (zero > 0) {
+              char* sa = sm + s * stage_bytes;
+              char* sb = sa + PLANES * kABytes;
               const int groups = PLANES * (2 + a.bn / 64);
               for (int i = lane; i < groups * zero * 8; i += 32) {
                 const int grp = i / (zero * 8), r = left + (i % (zero * 8)) / 8, q = i % 8;
@@ -366,12 +385,16 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
 #pragma unroll
           for (int c = 0; c < kPairs; ++c) {
             constexpr int pa[6] = {0, 0, 1, 1, 0, 2}, pb[6] = {0, 1, 0, 1, 2, 0};
-            const uint32_t ua = smem_u32(sa) + pa[c] * kABytes, ub = smem_u32(sb) + pb[c] * bbytes;
-            const uint64_t da = a.a_mn ? desc_mnmajor(ua, 8192) : desc_kmajor(ua);
-            const uint64_t db = a.b_mn ? desc_mnmajor(ub, 8192) : desc_kmajor(ub);
-            for (int k = 0; k < steps; ++k)
-              mma_16(c == 0 ? d : d + a.bn, da + ((k * step_a) >> 4), db + ((k * step_b) >> 4), a.idesc,
-                     (in_sum | k) != 0 || c > 1);
+            const uint64_t da = desc_a + (uint32_t)s * stage_units + pa[c] * (kABytes >> 4);
+            const uint64_t db = desc_b + (uint32_t)s * stage_units + pb[c] * b_units;
+            const uint32_t dc = c == 0 ? d : d + a.bn;
+            const bool add = in_sum != 0 || c > 1;
+            if (steps == 4) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mma_16(dc, da + k * step_a, db + k * step_b, idesc, k != 0 || add);
+            } else {
+              for (int k = 0; k < steps; ++k) mma_16(dc, da + k * step_a, db + k * step_b, idesc, k != 0 || add);
+            }
           }
           mma_commit(&bars.empty[s]);
           if (kb == t.kb - 1 || (PLANES > 1 && in_sum == kChunk - 1)) mma_commit(&bars.accfull[buf]);
@@ -389,7 +412,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
     const int w = warp - kEpiWarp0;
     const int row = (w & 3) * 32 + lane;            // row of the tile: the accumulator's lane
     const int c_lo = (w >> 2) * (a.bn / 2), c_hi = c_lo + a.bn / 2;
-    int64_t sums = 0;
+    Ring sums;
     bool ok = true;
     for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
       const Tile t = decode<KIND>(a, it);
@@ -397,9 +420,9 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
       if (PLANES > 1) {
 #pragma unroll
         for (int i = 0; i < 64; ++i) held[i] = 0.f;
-        for (int kb = 0; kb < t.kb; kb += kChunk, ++sums) {
-          const int buf = (int)(sums & 1);
-          ok = mbar_wait_warp(&bars.accfull[buf], (uint32_t)((sums >> 1) & 1), abort);
+        for (int kb = 0; kb < t.kb; kb += kChunk, sums.step(2)) {
+          const int buf = sums.i;
+          ok = mbar_wait_warp(&bars.accfull[buf], sums.phase, abort);
           if (!ok) break;
           tmem_fence_after();
           const uint32_t acc = tmem + buf * 2 * a.bn + c_lo + ((uint32_t)((w & 3) * 32) << 16);
@@ -418,15 +441,15 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
           if (lane == 0) mbar_arrive(&bars.accempty[buf]);
         }
       } else if (t.kb > 0) {
-        ok = mbar_wait_warp(&bars.accfull[sums & 1], (uint32_t)((sums >> 1) & 1), abort);
+        ok = mbar_wait_warp(&bars.accfull[sums.i], sums.phase, abort);
         tmem_fence_after();
       }
       if (!ok) {
         give_up(&bars, lane);
         break;
       }
-      const int buf = (int)(sums & 1);
-      if (PLANES == 1 && t.kb > 0) ++sums;
+      const int buf = sums.i;
+      if (PLANES == 1 && t.kb > 0) sums.step(2);
       // where this thread's row goes
       const int valid_rows = KIND == kWeights ? min(kBM, a.m - t.m0) : t.rows;
       const bool live = row < valid_rows;
@@ -487,45 +510,56 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
     // ---- gathered rows: thread = 16-byte piece `q` of every 16th row ----
     const int tid = threadIdx.x - kGatherWarp0 * 32, q = tid & 7, r0 = tid >> 3;
     const uint32_t at = (uint32_t)(r0 * 128 + ((q ^ (r0 & 7)) << 4));  // 128-byte swizzle; rows r0 + 16 i: + 2048 i
-    int64_t fill = 0;
+    Ring ring;
     bool ok = true;
-    for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
-      const Tile t = decode<KIND>(a, it);
-      if (t.kb == 0) continue;
-      if (KIND == kRows) {
-        const char* src[8];
+    constexpr int kR = KIND == kRows ? 8 : 4;  // rows of a stage per thread
+    // The next tile's place and rows are fetched while this tile's stages are
+    // in flight: each of these loads waits for the one before.
+    Tile t{};
+    if (blockIdx.x < total) t = decode<KIND>(a, blockIdx.x);
+    int next[kR];
+    auto first_rows = [&](const Tile& u) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = r0 + 16 * i;
-          src[i] = a.src_a + ((int64_t)(__ldg(a.order + t.pos + (r < t.rows ? r : 0)) / a.div_a) * a.ld_a + q * 8) * 2;
+      for (int i = 0; i < kR; ++i) {
+        const int r = r0 + 16 * i;
+        if (u.kb > 0) next[i] = __ldg(a.order + u.pos + (r < u.rows ? r : 0));
+      }
+    };
+    first_rows(t);
+    for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
+      const int64_t ahead = it + gridDim.x < total ? it + gridDim.x : it;
+      Tile u = t;
+      if (t.kb == 0) {
+        t = decode<KIND>(a, ahead);
+        first_rows(t);
+        continue;
+      }
+      const char* src[8];
+      if (KIND == kRows) {
+#pragma unroll
+        for (int i = 0; i < kR; ++i) src[i] = a.src_a + ((int64_t)(next[i] / a.div_a) * a.ld_a + q * 8) * 2;
+      }
+      for (int kb = 0; kb < t.kb; ++kb, ring.step(a.stages)) {
+        const bool last = kb == t.kb - 1;
+        const int s = ring.i;
+        if (KIND == kWeights) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            src[i] = a.src_a + ((int64_t)(next[i] / a.div_a) * a.ld_a + q * 8 + t.m0) * 2;
+            src[4 + i] = a.src_b + ((int64_t)(next[i] / a.div_b) * a.ld_b + q * 8 + t.n0) * 2;
+            if (!last) next[i] = __ldg(a.order + t.pos + min((kb + 1) * kBlockK + r0 + 16 * i, t.rows - 1));
+          }
         }
-        for (int kb = 0; kb < t.kb; ++kb, ++fill) {
-          const int s = (int)(fill % a.stages);
-          ok = mbar_wait_warp(&bars.empty[s], (uint32_t)((fill / a.stages) & 1) ^ 1, abort);
-          if (!ok) break;
-          const uint32_t sa = smem_u32(sm) + s * stage_bytes + at;
+        ok = mbar_wait_warp(&bars.empty[s], ring.phase ^ 1, abort);
+        if (!ok) break;
+        const uint32_t sa = smem_u32(sm) + s * stage_bytes + at;
+        if (KIND == kRows) {
           const bool live = kb * kBlockK + q * 8 < a.k;
           const int64_t k0 = live ? (int64_t)kb * (kBlockK * 2) : 0;
 #pragma unroll
           for (int i = 0; i < 8; ++i) copy16(sa + 2048 * i, src[i] + k0, live);
-          copies_arrive(&bars.full[s]);
-        }
-      } else {
-        int next[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) next[i] = __ldg(a.order + t.pos + min(r0 + 16 * i, t.rows - 1));
-        for (int kb = 0; kb < t.kb; ++kb, ++fill) {
-          const int s = (int)(fill % a.stages);
-          const char *pa[4], *pb[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {  // this stage's rows; the next stage's are fetched meanwhile
-            pa[i] = a.src_a + ((int64_t)(next[i] / a.div_a) * a.ld_a + q * 8 + t.m0) * 2;
-            pb[i] = a.src_b + ((int64_t)(next[i] / a.div_b) * a.ld_b + q * 8 + t.n0) * 2;
-            next[i] = __ldg(a.order + t.pos + min((kb + 1) * kBlockK + r0 + 16 * i, t.rows - 1));
-          }
-          ok = mbar_wait_warp(&bars.empty[s], (uint32_t)((fill / a.stages) & 1) ^ 1, abort);
-          if (!ok) break;
-          const uint32_t sa = smem_u32(sm) + s * stage_bytes + at, sb = sa + kABytes;
+        } else {
+          const uint32_t sb = sa + kABytes;
           const int left = t.rows - kb * kBlockK - r0;  // rows r0 + 16 i < left are the segment's
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
@@ -533,20 +567,25 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const bool live = in && 16 * i < left;
-              copy16(sa + g * 8192 + 2048 * i, live ? pa[i] + g * 128 : a.src_a, live);
+              copy16(sa + g * 8192 + 2048 * i, live ? src[i] + g * 128 : a.src_a, live);
             }
           }
-          for (int g = 0; g < a.bn / 64; ++g) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            if (g >= a.bn / 64) break;
             const bool in = t.n0 + g * 64 + q * 8 < a.n;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const bool live = in && 16 * i < left;
-              copy16(sb + g * 8192 + 2048 * i, live ? pb[i] + g * 128 : a.src_b, live);
+              copy16(sb + g * 8192 + 2048 * i, live ? src[4 + i] + g * 128 : a.src_b, live);
             }
           }
-          copies_arrive(&bars.full[s]);
         }
+        copies_arrive(&bars.full[s]);
+        if (kb == 0) u = decode<KIND>(a, ahead);
+        if (last) first_rows(u);
       }
+      t = u;
     }
     if (!ok && lane == 0) give_up(&bars, lane);
     asm volatile("cp.async.wait_all;" ::: "memory");
