@@ -13,8 +13,9 @@
 // K-major A operand, for kWeights -- where the rows are the contraction -- as
 // MN-major A and B operands.  (TMA's gather of four rows per instruction took
 // about 80 cycles an instruction, 6 B per cycle and SM, and held the tensor pipe
-// at 18 % and 7 %.)  The copies complete on the stage's mbarrier; the thread that
-// issues the products fences the proxies after it has waited.  Rows behind a
+// at 18 % and 7 %.)  The copies complete on the stage's mbarrier; a warp of its own
+// waits for it, fences the proxies and passes the stage on (the fence costs the
+// thread that issues the products 5 % of its time).  Rows behind a
 // segment's last are filled with zeros; kRows fetches copies of the tile's first
 // row there and does not store them.  Planes of fp32 rows are laid out sorted
 // before the launch and loaded as TMA tiles; there the last stage of a kWeights
@@ -60,7 +61,7 @@ constexpr int kChunk = 2;  // stages per accumulation where there are several pl
 constexpr int kSmemLimit = 232448 - 1024;
 
 struct Bars {
-  uint64_t full[kMaxStages], empty[kMaxStages];
+  uint64_t full[kMaxStages], ready[kMaxStages], empty[kMaxStages];  // ready: full, and the proxies fenced
   uint64_t accfull[2], accempty[2];
   uint32_t tmem_base;
   int abort;
@@ -91,6 +92,18 @@ __device__ __forceinline__ void give_up(Bars* bars, int lane) {
     *(volatile int*)&bars->abort = 1;
     atomicOr(&g_status, 1);
   }
+}
+
+// one poll, without waiting
+__device__ __forceinline__ bool mbar_test(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(smem_u32(b)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 // position in the ring of stages (or of the two accumulators): index and phase, counted without divisions
@@ -263,6 +276,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
       mbar_init(&bars.full[i], R::kFullCount);
+      mbar_init(&bars.ready[i], 1);
       mbar_init(&bars.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -329,7 +343,83 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
       const int64_t first = filled > a.stages ? filled - a.stages : 0;
       for (int64_t f = first; f < filled; ++f) mbar_wait_warp(&bars.full[f % a.stages], (uint32_t)((f / a.stages) & 1), nullptr);
     }
-  } else if (warp == 1) {
+  } else if (PLANES == 1 && warp == 1) {
+    // ---- products of one plane: one thread ----
+    if (lane == 0) {
+      Ring ring, sums;
+      int64_t use = 0;
+      bool ok = true, peeked = false;  // peeked: the stage at `ring` is known to be there
+      const uint32_t step_a = (a.a_mn ? 2048 : 32) >> 4, step_b = (a.b_mn ? 2048 : 32) >> 4;
+      const uint64_t desc_a = a.a_mn ? desc_mnmajor(smem_u32(sm), 8192) : desc_kmajor(smem_u32(sm));
+      const uint32_t sb0 = smem_u32(sm) + kABytes;
+      const uint64_t desc_b = a.b_mn ? desc_mnmajor(sb0, 8192) : desc_kmajor(sb0);
+      const uint32_t stage_units = (uint32_t)stage_bytes >> 4;
+      const uint32_t idesc = a.idesc;
+      uint64_t* there = R::kGather ? bars.ready : bars.full;
+      Tile t{};
+      if (blockIdx.x < total) t = decode<KIND>(a, blockIdx.x);
+      for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
+        const int64_t ahead = it + gridDim.x < total ? it + gridDim.x : it;
+        if (t.kb == 0) {
+          t = decode<KIND>(a, ahead);
+          continue;
+        }
+        ok = mbar_wait(&bars.accempty[sums.i], sums.phase ^ 1, abort);
+        if (!ok) break;
+        tmem_fence_after();
+        const uint32_t d = tmem + sums.i * a.bn;
+        Tile u = t;
+        for (int kb = 0; kb < t.kb; ++kb, ++use) {
+          if (!peeked) ok = mbar_wait(&there[ring.i], ring.phase, abort);
+          if (!ok) break;
+          tmem_fence_after();
+          const uint64_t da = desc_a + (uint32_t)ring.i * stage_units, db = desc_b + (uint32_t)ring.i * stage_units;
+          uint64_t* done = &bars.empty[ring.i];
+          const bool last = kb == t.kb - 1;
+          const int steps = KIND == kWeights && last ? min(4, (t.rows - kb * kBlockK + 15) >> 4) : 4;
+          ring.step(a.stages);
+          if (steps == 4) {
+            mma_16(d, da, db, idesc, kb != 0);
+            mma_16(d, da + step_a, db + step_b, idesc, 1);
+            // While these run: whether the next stage is there, or what comes after this tile.  The
+            // tensor core takes few products ahead, so what stands between two stages' products is idle time.
+            if (last) u = decode<KIND>(a, ahead);
+            peeked = mbar_test(&there[ring.i], ring.phase);
+            mma_16(d, da + 2 * step_a, db + 2 * step_b, idesc, 1);
+            mma_16(d, da + 3 * step_a, db + 3 * step_b, idesc, 1);
+          } else {
+            for (int k = 0; k < steps; ++k) mma_16(d, da + k * step_a, db + k * step_b, idesc, (kb | k) != 0);
+            u = decode<KIND>(a, ahead);
+            peeked = false;
+          }
+          mma_commit(done);
+          if (last) mma_commit(&bars.accfull[sums.i]);
+        }
+        sums.step(2);
+        t = u;
+      }
+      if (!ok) {  // products in flight still read shared and write tensor memory
+        give_up(&bars, 0);
+        const int64_t first = use > a.stages ? use - a.stages : 0;
+        for (int64_t f = first; f < use; ++f) mbar_wait(&bars.empty[f % a.stages], (uint32_t)((f / a.stages) & 1), nullptr);
+      }
+    }
+  } else if (R::kGather && warp == 3) {
+    // ---- stages whose copies have landed: fence the proxies (cp.async wrote through the generic one) ----
+    Ring ring;
+    bool ok = true;
+    for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
+      const int n = decode<KIND>(a, it).kb;
+      for (int kb = 0; kb < n; ++kb, ring.step(a.stages)) {
+        ok = mbar_wait_warp(&bars.full[ring.i], ring.phase, abort);
+        if (!ok) break;
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.ready[ring.i]);
+      }
+    }
+    if (!ok) give_up(&bars, lane);
+  } else if (PLANES > 1 && warp == 1) {
     // ---- products ----
     Ring ring, sums;
     int64_t use = 0;
@@ -362,7 +452,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
         if (KIND == kWeights) {
           const int left = t.rows - kb * kBlockK;
           if (left < kBlockK) steps = (left + 15) >> 4;
-          if (!R::kGather && left < kBlockK) {
+          if (left < kBlockK) {
             const int zero = steps * 16 - left;  // rows to clear, of 128 bytes in each 64-column group
             if (zero > 0) {
               char* sa = sm + s * stage_bytes;
@@ -379,7 +469,6 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
           }
         }
         if (lane == 0) {
-          if (R::kGather) fence_proxy_async();  // cp.async wrote through the generic proxy
           tmem_fence_after();
           constexpr int kPairs = PLANES == 1 ? 1 : PLANES == 2 ? 3 : 6;
 #pragma unroll
