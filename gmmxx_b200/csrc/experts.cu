@@ -123,8 +123,9 @@ int tile_columns(int64_t row_tiles, int64_t n, int planes, int max_bn) {
 }
 
 int elem_size(int dt) { return dt == GMMXX_FLOAT32 ? 4 : 2; }
+// four elements at a time: rows of a multiple of four elements
 bool vec_ok(const void* p, int dt, int64_t ld) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * elem_size(dt)) % 16 == 0;
+  return (reinterpret_cast<uintptr_t>(p) & (4 * elem_size(dt) - 1)) == 0 && ld % 4 == 0;
 }
 
 // ---------------------------------------------------------------------------
@@ -503,7 +504,7 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
   }
   if (gb != nullptr) {
     const dim3 grid((unsigned)ceil_div(n_out, 128), (unsigned)std::min<int64_t>(65535, p.max_segs));
-    bias_kernel<<<grid, 256, 0, st>>>(table, g.order, gy, dt, (int)n_out, vec_ok(gy, dt, n_out), part_b, gb);
+    bias_kernel<<<grid, 256, 0, st>>>(table, g.order, gy, dt, (int)n_out, n_out % 8 == 0, part_b, gb);
     if (int rc = check_launch("bias_kernel")) return rc;
     if (p.max_split > 0) {
       join_kernel<<<148, 256, 0, st>>>(table, split, part_b, n_out, gb, dt);

@@ -57,8 +57,9 @@ constexpr int kGatherWarp0 = 12, kGatherThreads = 128;
 constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
 constexpr int kABytes = kBM * 128;  // one plane of A per stage
 constexpr int kMaxStages = 8;
+constexpr int kStageEpi = 4096;     // staging of one epilogue warp: 32 rows x 32 fp32
 constexpr int kChunk = 2;  // stages per accumulation where there are several planes
-constexpr int kSmemLimit = 232448 - 1024;
+constexpr int kSmemLimit = 232448;
 
 struct Bars {
   uint64_t full[kMaxStages], ready[kMaxStages], empty[kMaxStages];  // ready: full, and the proxies fenced
@@ -168,85 +169,40 @@ __device__ __forceinline__ Tile decode(const ProductArgs& a, int64_t it) {
   return t;
 }
 
-__device__ __forceinline__ uint4 pack8(const float* v, int dt) {
-  uint4 q;
-  uint32_t* p = reinterpret_cast<uint32_t*>(&q);
+// One epilogue warp's 32 rows x 32 columns of fp32, staged in shared memory so
+// that global accesses run along rows: 16-byte piece j of row r at piece
+// j ^ (r & 7), which keeps both the row-wise writes (a lane per row) and the
+// reads (8 lanes per row, or a lane per column) free of bank conflicts.
+__device__ __forceinline__ void stage_row(char* st, int row, const float* v) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (dt == GMMXX_BFLOAT16) {
-      p[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-    } else {
-      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-      p[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-  }
-  return q;
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<float4*>(st + row * 128 + ((j ^ (row & 7)) << 4)) =
+        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+}
+__device__ __forceinline__ float4 staged4(const char* st, int row, int j) {
+  return *reinterpret_cast<const float4*>(st + row * 128 + ((j ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ float staged1(const char* st, int row, int c) {
+  return *reinterpret_cast<const float*>(st + row * 128 + (((c >> 2) ^ (row & 7)) << 4) + (c & 3) * 4);
 }
 
-// 32 values of one row to out[row0 + c], nv of them valid
-__device__ __forceinline__ void store32(void* out, int dt, int64_t at, const float* v, int nv, int vec) {
-  if (vec && nv >= 32) {
-    if (dt == GMMXX_FLOAT32) {
-      float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
-      uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = pack8(v + 8 * i, dt);
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (i < nv) store_y(out, at + i, dt, v[i]);
+__device__ __forceinline__ uint2 half4(float4 v) {
+  const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+__device__ __forceinline__ float4 float4_of(uint2 q) {
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&q.x));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&q.y));
+  return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// kBatch: 32 values of one row: combine with the planes e and write planes or the result
-template <int PLANES>
-__device__ __forceinline__ void batch32(const ProductArgs& a, const Tile& t, int row, int c, float* v, int nv) {
-  const int64_t at = t.g * a.p_stride + (int64_t)row * a.ldp + c;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] *= a.alpha;
-  if (a.e[0] != nullptr) {
-#pragma unroll
-    for (int i0 = 0; i0 < 32; i0 += 8) {  // ldp is a multiple of 8: whole 16-byte pieces (their tail is never used)
-      if (i0 >= nv) break;
-#pragma unroll
-      for (int p = PLANES - 1; p >= 0; --p) {
-        const uint4 q = *reinterpret_cast<const uint4*>(a.e[p] + at + i0);
-        const __half2* h = reinterpret_cast<const __half2*>(&q);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = __half22float2(h[i]);
-          v[i0 + 2 * i] = fmaf(a.beta, f.x, v[i0 + 2 * i]);
-          v[i0 + 2 * i + 1] = fmaf(a.beta, f.y, v[i0 + 2 * i + 1]);
-        }
-      }
-    }
-  }
-  if (a.out != nullptr) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] *= 1.f / kPlaneScale;
-    store32(a.out, a.out_dt, t.g * a.out_stride + (int64_t)row * a.ldo + c, v, nv, a.vec);
-    return;
-  }
-#pragma unroll
-  for (int i0 = 0; i0 < 32; i0 += 8) {
-    if (i0 >= nv) break;
-    uint4 q[2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = v[i0 + 2 * i], y = v[i0 + 2 * i + 1];
-      const __half2 hi = __floats2half2_rn(x, y);
-      reinterpret_cast<__half2*>(&q[0])[i] = hi;
-      if (PLANES > 1) {
-        const float2 f = __half22float2(hi);
-        reinterpret_cast<__half2*>(&q[1])[i] = __floats2half2_rn(x - f.x, y - f.y);
-      }
-    }
-#pragma unroll
-    for (int p = 0; p < PLANES; ++p) *reinterpret_cast<uint4*>(a.o[p] + at + i0) = q[p];
+// 4 values to out[at ..], aligned to 4 elements
+__device__ __forceinline__ void store4(void* out, int dt, int64_t at, float4 v) {
+  if (dt == GMMXX_FLOAT32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = v;
+  } else {
+    const uint2 q = dt == GMMXX_BFLOAT16 ? make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w)) : half4(v);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = q;
   }
 }
 
@@ -499,7 +455,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
   } else if (warp >= kEpiWarp0 && warp < kEpiWarp0 + kEpiWarps) {
     // ---- results ----
     const int w = warp - kEpiWarp0;
-    const int row = (w & 3) * 32 + lane;            // row of the tile: the accumulator's lane
+    char* stage = sm + a.stages * stage_bytes + w * kStageEpi;  // row = the accumulator's lane
     const int c_lo = (w >> 2) * (a.bn / 2), c_hi = c_lo + a.bn / 2;
     Ring sums;
     bool ok = true;
@@ -539,36 +495,55 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
       }
       const int buf = sums.i;
       if (PLANES == 1 && t.kb > 0) sums.step(2);
-      // where this thread's row goes
+      // Rows in store order: lane takes rows r8 + 4 i, four columns each (8 lanes per row)
+      const int n_left = a.n - t.n0;
       const int valid_rows = KIND == kWeights ? min(kBM, a.m - t.m0) : t.rows;
-      const bool live = row < valid_rows;
+      const int row0 = (w & 3) * 32, r8 = lane >> 3, c4 = (lane & 7) * 4;
       void* out = a.out;
       int dt = a.out_dt, vec = a.vec;
-      int64_t at = 0;
-      if (KIND == kRows && live) {
-        at = (int64_t)__ldg(a.order + t.pos + row) * a.ldo;
-      } else if (KIND == kWeights) {
-        if (t.slot >= 0) {
-          out = a.part;
-          dt = GMMXX_FLOAT32;
-          vec = (a.n & 3) == 0;
-          at = ((int64_t)t.slot * a.m + t.m0 + row) * a.n;
-        } else {
-          at = t.g * a.out_stride + (int64_t)(t.m0 + row) * a.ldo;
-        }
+      if (KIND == kWeights && t.slot >= 0) {
+        out = a.part;
+        dt = GMMXX_FLOAT32;
+        vec = (a.n & 3) == 0;
       }
-      const int n_left = a.n - t.n0;
+      // first element of tile row r
+      auto row_at = [&](int r) -> int64_t {
+        if (KIND == kRows) return (int64_t)__ldg(a.order + t.pos + r) * a.ldo;
+        if (KIND == kWeights && t.slot >= 0) return ((int64_t)t.slot * a.m + t.m0 + r) * a.n;
+        return t.g * a.out_stride + (int64_t)(t.m0 + r) * a.ldo;
+      };
+      int64_t at[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = row0 + r8 + 4 * i;
+        at[i] = r < valid_rows ? row_at(r) : -1;
+      }
 #pragma unroll
       for (int j = 0; j < (PLANES > 1 ? 2 : 4); ++j) {
         const int c = c_lo + 32 * j;
         if (c >= c_hi) break;
+        const int nv = n_left - c;  // columns left from c
+        // the planes to add, fetched while the accumulator is read
+        uint2 e[KIND == kBatch ? PLANES : 1][KIND == kBatch ? 8 : 1];
+        int64_t pat = 0;
+        auto fetch = [&]() {
+          pat = t.g * a.p_stride + (int64_t)(t.m0 + row0 + r8) * a.ldp + t.n0 + c + c4;
+          if (a.e[0] == nullptr) return;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int p = 0; p < PLANES; ++p)  // ldp is a multiple of 8: whole pieces, their tail is not used
+              e[p][i] = at[i] >= 0 && c4 < nv ? *reinterpret_cast<const uint2*>(a.e[p] + pat + 4 * i * a.ldp)
+                                              : make_uint2(0, 0);
+        };
+        if (KIND == kBatch && PLANES == 1) fetch();
         float v[32];
         __syncwarp();
         if (PLANES > 1) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = held[(32 * j + i) % (PLANES > 1 ? 64 : 1)];
         } else if (t.kb > 0) {
-          tmem_ld32(tmem + buf * a.bn + c + ((uint32_t)((w & 3) * 32) << 16), v);
+          tmem_ld32(tmem + buf * a.bn + c + ((uint32_t)row0 << 16), v);
           tmem_wait_ld();
           if (c + 32 == c_hi) {  // the accumulator is in registers: free it for the tile after next
             tmem_fence_before();
@@ -579,19 +554,70 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0.f;
         }
-        const int nv = n_left - c;
-        if (!live || nv <= 0) continue;
+        if (nv <= 0) continue;
+        stage_row(stage, lane, v);
+        if (KIND == kBatch && PLANES > 1) fetch();  // later: the sums hold the registers
+        __syncwarp();
         if (KIND == kBatch) {
-          batch32<PLANES>(a, t, t.m0 + row, t.n0 + c, v, nv);
-        } else {
-          if (KIND == kRows && a.bias != nullptr && t.kb > 0) {
-            const int64_t b0 = (int64_t)t.g * a.n + t.n0 + c;
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < nv) v[i] += load_x(a.bias, b0 + i, a.bias_dt);
+          for (int i = 0; i < 8; ++i) {
+            float4 x = staged4(stage, r8 + 4 * i, lane & 7);
+            x = make_float4(x.x * a.alpha, x.y * a.alpha, x.z * a.alpha, x.w * a.alpha);
+            if (a.e[0] != nullptr) {
+#pragma unroll
+              for (int p = PLANES - 1; p >= 0; --p) {
+                const float4 f = float4_of(e[p][i]);
+                x = make_float4(fmaf(a.beta, f.x, x.x), fmaf(a.beta, f.y, x.y), fmaf(a.beta, f.z, x.z),
+                                fmaf(a.beta, f.w, x.w));
+              }
+            }
+            if (at[i] < 0 || c4 >= nv) continue;
+            if (a.out != nullptr) {
+              constexpr float down = 1.f / kPlaneScale;
+              x = make_float4(x.x * down, x.y * down, x.z * down, x.w * down);
+              const int64_t o = at[i] + t.n0 + c + c4;
+              if (vec) {
+                store4(out, dt, o, x);
+              } else {
+                store_y(out, o, dt, x.x);
+                if (c4 + 1 < nv) store_y(out, o + 1, dt, x.y);
+                if (c4 + 2 < nv) store_y(out, o + 2, dt, x.z);
+                if (c4 + 3 < nv) store_y(out, o + 3, dt, x.w);
+              }
+            } else {
+              const uint2 hi = half4(x);
+              *reinterpret_cast<uint2*>(a.o[0] + pat + 4 * i * a.ldp) = hi;
+              if (PLANES > 1) {
+                const float4 f = float4_of(hi);
+                *reinterpret_cast<uint2*>(a.o[1] + pat + 4 * i * a.ldp) =
+                    half4(make_float4(x.x - f.x, x.y - f.y, x.z - f.z, x.w - f.w));
+              }
+            }
           }
-          store32(out, dt, at + t.n0 + c, v, nv, vec);
+        } else {
+          const bool biased = KIND == kRows && a.bias != nullptr && t.kb > 0;
+          const int64_t b0 = (int64_t)t.g * a.n + t.n0 + c;
+          if (vec) {  // a.n is a multiple of 4: a piece of four columns is whole or absent
+            float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (biased && c4 < nv)
+              b = make_float4(load_x(a.bias, b0 + c4, a.bias_dt), load_x(a.bias, b0 + c4 + 1, a.bias_dt),
+                              load_x(a.bias, b0 + c4 + 2, a.bias_dt), load_x(a.bias, b0 + c4 + 3, a.bias_dt));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 x = staged4(stage, r8 + 4 * i, lane & 7);
+              if (at[i] >= 0 && c4 < nv)
+                store4(out, dt, at[i] + t.n0 + c + c4, make_float4(x.x + b.x, x.y + b.y, x.z + b.z, x.w + b.w));
+            }
+          } else {  // a lane per column: whole lines although no row is aligned
+            const float b = biased && lane < nv ? load_x(a.bias, b0 + lane, a.bias_dt) : 0.f;
+#pragma unroll
+            for (int r = 0; r < 32; ++r) {
+              const int64_t base = __shfl_sync(0xffffffffu, at[r >> 2], (r & 3) * 8);
+              if (base >= 0 && lane < nv) store_y(out, base + t.n0 + c + lane, dt, staged1(stage, r, lane) + b);
+            }
+          }
         }
+        __syncwarp();
       }
     }
   }
@@ -710,7 +736,7 @@ int encode(CUtensorMap* map, const void* base, int fp16, int rank, const cuuint6
 
 template <int KIND, int PLANES>
 int launch_one(const ProductMaps& maps, const ProductArgs& a, unsigned grid, cudaStream_t st) {
-  const int smem = a.stages * PLANES * (kABytes + a.bn * 128) + 1024;
+  const int smem = a.stages * PLANES * (kABytes + a.bn * 128) + kEpiWarps * kStageEpi + 1024;
   if (int rc = allow_smem((const void*)product_kernel<KIND, PLANES>, smem)) return rc;
   product_kernel<KIND, PLANES><<<grid, Roles<KIND, PLANES>::kThreads, smem, st>>>(maps, a);
   return check_launch("product_kernel");
@@ -734,7 +760,7 @@ uint32_t product_idesc(int fp16, int bn, int a_mn, int b_mn) {
 }
 
 int product_stages(int planes, int bn) {
-  return std::min(kMaxStages, (kSmemLimit - 2048) / (planes * (kABytes + bn * 128)));
+  return std::min(kMaxStages, (kSmemLimit - 2048 - kEpiWarps * kStageEpi) / (planes * (kABytes + bn * 128)));
 }
 
 int device_sms(int* sms) {
