@@ -12,6 +12,7 @@ This module replaces the reference's lazy ``gmmxx._C`` import and its
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 from typing import Optional
@@ -206,21 +207,26 @@ def _size(name: str, *args) -> int:
     return v
 
 
+@functools.lru_cache(maxsize=1024)
 def group_tiles_len(slots: int, k: int) -> int:
     return _size("gmmxx_group_tiles_len", slots, k)
 
 
+@functools.lru_cache(maxsize=1024)
 def group_rows_workspace_bytes(slots: int, k: int) -> int:
     return _size("gmmxx_group_rows_workspace_bytes", slots, k)
 
 
+@functools.lru_cache(maxsize=1024)
 def grouped_matmul_workspace_bytes(dt: int, rows: int, top: int, k: int, n_in: int, n_out: int) -> int:
     return _size("gmmxx_grouped_matmul_workspace_bytes", dt, rows, top, k, n_in, n_out)
 
 
+@functools.lru_cache(maxsize=1024)
 def grouped_matmul_backward_workspace_bytes(dt: int, rows: int, top: int, k: int, n_in: int, n_out: int) -> int:
     return _size("gmmxx_grouped_matmul_backward_workspace_bytes", dt, rows, top, k, n_in, n_out)
 
 
+@functools.lru_cache(maxsize=1024)
 def orthogonalize_workspace_bytes(dt: int, batch: int, m: int, n: int) -> int:
     return _size("gmmxx_orthogonalize_workspace_bytes", dt, batch, m, n)

@@ -514,12 +514,22 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
   return GMMXX_OK;
 }
 
+int read_status(int* out, cudaStream_t st) {
+  int a = 0, b = 0;
+  if (int rc = product_status(&a, st)) return rc;
+  if (int rc = orth_small_status(&b, st)) return rc;
+  *out = a != 0 || b != 0 ? GMMXX_ERR_TIMEOUT : GMMXX_OK;
+  return GMMXX_OK;
+}
+
 size_t orthogonalize_ws(int dt, int64_t batch, int64_t m, int64_t n) {
+  if (orth_small_fits(m, n)) return 256;
   return (size_t)(ns_plan(dt, batch, m, n).bytes + 256);
 }
 
 int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_t n, int steps, float a, float b,
                          float c, float eps, void* q, char* ws, cudaStream_t st) {
+  if (orth_small_fits(m, n)) return launch_orth_small(dt, g, batch, m, n, steps, a, b, c, eps, q, st);
   const NsPlan s = ns_plan(dt, batch, m, n);
   const int64_t size = m * n;
   double* part = reinterpret_cast<double*>(ws + s.part);

@@ -4,6 +4,8 @@
 
 #include "gmm_common.cuh"
 
+#include <atomic>
+
 namespace gmmxx {
 namespace experts {
 
@@ -36,9 +38,24 @@ __device__ __forceinline__ void store_y(void* p, int64_t i, int dt, float v) {
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-inline int allow_smem(const void* kern, int bytes) {
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+// Lets `kern` have `bytes` of dynamic shared memory on the current device.
+// `done` (one per kernel) holds the largest size granted so far per device: the
+// call costs more than a launch's other host work.
+constexpr int kMaxDevices = 64;
+struct SmemGrants {
+  std::atomic<int> bytes[kMaxDevices] = {};
+};
+inline int allow_smem(const void* kern, int bytes, SmemGrants& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < kMaxDevices && done.bytes[dev].load(std::memory_order_relaxed) >= bytes) return GMMXX_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "kernel attributes: %s", cudaGetErrorString(e));
+  if (dev < kMaxDevices) {  // only ever grows: a smaller grant must not replace a larger one
+    int seen = done.bytes[dev].load(std::memory_order_relaxed);
+    while (seen < bytes && !done.bytes[dev].compare_exchange_weak(seen, bytes)) {
+    }
+  }
   return GMMXX_OK;
 }
 

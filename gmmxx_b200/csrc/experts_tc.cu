@@ -48,7 +48,7 @@ namespace experts {
 
 using namespace ptx;
 
-__device__ int g_status = 0;  // sticky: 1 when a bounded wait ran out (gmmxx_products_status)
+static __device__ int g_status = 0;  // sticky: 1 when a bounded wait ran out (gmmxx_products_status)
 
 namespace {
 
@@ -737,7 +737,8 @@ int encode(CUtensorMap* map, const void* base, int fp16, int rank, const cuuint6
 template <int KIND, int PLANES>
 int launch_one(const ProductMaps& maps, const ProductArgs& a, unsigned grid, cudaStream_t st) {
   const int smem = a.stages * PLANES * (kABytes + a.bn * 128) + kEpiWarps * kStageEpi + 1024;
-  if (int rc = allow_smem((const void*)product_kernel<KIND, PLANES>, smem)) return rc;
+  static SmemGrants grants;
+  if (int rc = allow_smem((const void*)product_kernel<KIND, PLANES>, kSmemLimit - 1024, grants)) return rc;
   product_kernel<KIND, PLANES><<<grid, Roles<KIND, PLANES>::kThreads, smem, st>>>(maps, a);
   return check_launch("product_kernel");
 }
@@ -753,21 +754,18 @@ int encode_stack(CUtensorMap* map, const void* base, int fp16, int64_t cols, int
   return encode(map, base, fp16, 3, dims, strides, box);
 }
 
-uint32_t product_idesc(int fp16, int bn, int a_mn, int b_mn) {
-  uint32_t d = idesc_bf16(kBM, bn, a_mn, b_mn);
-  if (fp16) d &= ~((1u << 7) | (1u << 10));  // A and B types: 0 = fp16, 1 = bf16
-  return d;
-}
-
 int product_stages(int planes, int bn) {
   return std::min(kMaxStages, (kSmemLimit - 2048 - kEpiWarps * kStageEpi) / (planes * (kABytes + bn * 128)));
 }
 
 int device_sms(int* sms) {
+  static std::atomic<int> known[kMaxDevices] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < kMaxDevices && (*sms = known[dev].load(std::memory_order_relaxed)) > 0) return GMMXX_OK;
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "device query: %s", cudaGetErrorString(e));
+  if (dev < kMaxDevices) known[dev].store(*sms, std::memory_order_relaxed);
   return GMMXX_OK;
 }
 
@@ -782,17 +780,18 @@ int launch_product(Kind kind, int planes, const ProductMaps& maps, const Product
   return planes == 1 ? launch_one<kBatch, 1>(maps, a, grid, st) : launch_one<kBatch, 2>(maps, a, grid, st);
 }
 
-int read_status(int* out, cudaStream_t st) {
-  int v = 0;
+int take_flag(const void* symbol, int* flag, cudaStream_t st) {
   const int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, g_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  cudaError_t e = cudaMemcpyFromSymbolAsync(flag, symbol, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  if (e == cudaSuccess && v != 0) e = cudaMemcpyToSymbolAsync(g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
-  if (e == cudaSuccess && v != 0) e = cudaStreamSynchronize(st);
-  if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "status read: %s", cudaGetErrorString(e));
-  *out = v != 0 ? GMMXX_ERR_TIMEOUT : GMMXX_OK;
-  return GMMXX_OK;
+  if (e == cudaSuccess && *flag != 0) {
+    e = cudaMemcpyToSymbolAsync(symbol, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  }
+  return e == cudaSuccess ? GMMXX_OK : set_error(GMMXX_ERR_CUDA, "status read: %s", cudaGetErrorString(e));
 }
+
+int product_status(int* flag, cudaStream_t st) { return take_flag((const void*)&g_status, flag, st); }
 
 }  // namespace experts
 }  // namespace gmmxx

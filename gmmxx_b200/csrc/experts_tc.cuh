@@ -62,11 +62,25 @@ constexpr int kSegInts = 4;
 
 int encode_stack(CUtensorMap* map, const void* base, int fp16, int64_t cols, int64_t rows, int64_t ld, int64_t stack,
                  int64_t stride, int box_rows);
-uint32_t product_idesc(int fp16, int bn, int a_mn, int b_mn);
+// instruction descriptor of kind::f16 with M = 128, N = bn, fp32 sums; types 0 = fp16, 1 = bf16 for both operands
+__host__ __device__ inline uint32_t product_idesc(int fp16, int bn, int a_mn, int b_mn) {
+  const uint32_t type = fp16 ? 0u : 1u;
+  return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
 int product_stages(int planes, int bn);
 int launch_product(Kind kind, int planes, const ProductMaps& maps, const ProductArgs& a, int64_t max_items,
                    cudaStream_t st);
 int device_sms(int* sms);
+// sticky flags of bounded waits that ran out: read on the stream, synchronise, clear
+int take_flag(const void* symbol, int* flag, cudaStream_t st);
+int product_status(int* flag, cudaStream_t st);
+int orth_small_status(int* flag, cudaStream_t st);
+
+// stacks of small matrices in one launch (orth_small.cu)
+bool orth_small_fits(int64_t m, int64_t n);
+int launch_orth_small(int dt, const void* g, int64_t batch, int64_t m, int64_t n, int steps, float a, float b, float c,
+                      float eps, void* q, cudaStream_t st);
 
 }  // namespace experts
 }  // namespace gmmxx

@@ -22,10 +22,10 @@ namespace {
 
 constexpr int kWarps = 32;                       // warps of the one-block kernel
 constexpr int64_t kSmallSlots = 32768;           // above, four launches over the whole GPU are faster
-constexpr int64_t kSmallSmem = 200 * 1024;
+constexpr int kSmallSmem = 200 * 1024;
 constexpr int64_t kChunk = 1024;                 // slots per warp of the large path, at least
 constexpr int64_t kMaxWarps = 148 * 32;
-constexpr int64_t kTableSmem = 200 * 1024;       // counters of one block's warps
+constexpr int kTableSmem = 200 * 1024;       // counters of one block's warps
 
 __device__ __forceinline__ int load_label(const void* labels, int wide, int64_t i, int K) {
   // clamped before the narrowing: a 64-bit label beyond 32 bits is unassigned too
@@ -281,7 +281,8 @@ int launch_group_rows(const void* labels, int wide, int64_t slots, int64_t K, in
                       int32_t* tiles, char* ws, cudaStream_t st) {
   const Plan p = make_plan(slots, K);
   if (p.small) {
-    if (int rc = allow_smem((const void*)group_rows_small_kernel, p.smem)) return rc;
+    static SmemGrants grants;
+    if (int rc = allow_smem((const void*)group_rows_small_kernel, kSmallSmem, grants)) return rc;
     group_rows_small_kernel<<<1, 1024, p.smem, st>>>(labels, wide, (int)slots, (int)K, order, offsets, tiles);
     return check_launch("group_rows_small_kernel");
   }
@@ -289,8 +290,9 @@ int launch_group_rows(const void* labels, int wide, int64_t slots, int64_t K, in
   int* total = reinterpret_cast<int*>(ws + p.total);
   int* start = reinterpret_cast<int*>(ws + p.start);
   int* first = reinterpret_cast<int*>(ws + p.first);
-  if (int rc = allow_smem((const void*)count_kernel, p.smem)) return rc;
-  if (int rc = allow_smem((const void*)place_kernel, p.smem)) return rc;
+  static SmemGrants count_grants, place_grants;
+  if (int rc = allow_smem((const void*)count_kernel, kTableSmem, count_grants)) return rc;
+  if (int rc = allow_smem((const void*)place_kernel, kTableSmem, place_grants)) return rc;
   count_kernel<<<p.blocks, p.warps * 32, p.smem, st>>>(labels, wide, slots, (int)K, p.chunk, p.nwarps, table);
   if (int rc = check_launch("count_kernel")) return rc;
   columns_kernel<<<(unsigned)ceil_div(K + 1, 32), 1024, 0, st>>>(table, p.nwarps, (int)K + 1, total);

@@ -1,0 +1,320 @@
+// orth_small.cu -- the whole Newton-Schulz iteration of a small matrix in one
+// block: iterates in shared memory, products on tcgen05, one launch for a stack
+// of any length.
+//
+// A matrix with short side <= 64 and long side <= 512, or both <= 128 (256), is
+// held as two fp16 planes of value * kPlaneScale (22 bits, see experts_tc.cu)
+// with its short side along the rows (a tall one is transposed on the way in and
+// out).  Per step, three products of 128 x N x K by one thread, each followed by
+// an epilogue of all warps that rounds the result back into planes:
+//
+//   P = X X^T            both operands K-major (rows of X)
+//   P <- b P + c P P     P is symmetric: its rows serve as both operands, in place
+//   X <- a X + P X       X as the MN-major B operand, column chunk by chunk, in place
+//
+// The leading planes' products and the others go to accumulators of their own,
+// and P's leading products to one per 128 columns of X: at most 8 additions in
+// an accumulator (the tensor core's additions truncate).  Shared memory and
+// tensor memory let 4 blocks of 64 x 64 run per SM, 1 of 128 x 128.
+//
+// Bound by the chain of 15 products (5 steps): each waits for the epilogue
+// before it, ~1 us.  The same work through the stacked products takes 17
+// launches of ~5 us.
+#include "experts_tc.cuh"
+#include "tc_ptx.cuh"
+
+#include <algorithm>
+
+namespace gmmxx {
+namespace experts {
+
+using namespace ptx;
+
+namespace {
+
+constexpr int kOrthThreads = 256;
+
+static __device__ int g_orth_status = 0;  // sticky: 1 when a bounded wait ran out
+
+struct OrthArgs {
+  const void* g;
+  void* q;
+  int dt;
+  int64_t batch;
+  int m, n;           // of g
+  int lo, hi;         // sides
+  int tall;           // m > n: rows of the held matrix are g's columns
+  int rows;           // rows of a block: 64 or 128 (lo rounded up)
+  int xb, pb;         // 64-column blocks of X and of P
+  int np, xn;         // accumulator columns: P (64 / 128), a column chunk of X (64 / 128)
+  int chunks;         // 128-column chunks of X
+  int tmem;           // tensor memory columns
+  int steps;
+  float a, b, c, eps;
+};
+
+__device__ __forceinline__ void load16(uint32_t addr, float* v) {
+  tmem_ld16(addr, v);
+  tmem_wait_ld();
+}
+
+// 8 values of a row to / from the planes
+__device__ __forceinline__ void put8(char* hi, char* lo, uint32_t off, const float* v) {
+  uint4 h, l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 x = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    const float2 f = __half22float2(x);
+    reinterpret_cast<__half2*>(&h)[i] = x;
+    reinterpret_cast<__half2*>(&l)[i] = __floats2half2_rn(v[2 * i] - f.x, v[2 * i + 1] - f.y);
+  }
+  *reinterpret_cast<uint4*>(hi + off) = h;
+  *reinterpret_cast<uint4*>(lo + off) = l;
+}
+__device__ __forceinline__ void add8(const char* hi, const char* lo, uint32_t off, float scale, float* v) {
+  const uint4 h = *reinterpret_cast<const uint4*>(hi + off), l = *reinterpret_cast<const uint4*>(lo + off);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 fl = __half22float2(reinterpret_cast<const __half2*>(&l)[i]);
+    const float2 fh = __half22float2(reinterpret_cast<const __half2*>(&h)[i]);
+    v[2 * i] = fmaf(scale, fh.x, fmaf(scale, fl.x, v[2 * i]));
+    v[2 * i + 1] = fmaf(scale, fh.y, fmaf(scale, fl.y, v[2 * i + 1]));
+  }
+}
+
+__global__ void __launch_bounds__(kOrthThreads) orth_small_kernel(const OrthArgs a) {
+  extern __shared__ __align__(1024) char smem_raw[];
+  __shared__ uint64_t bar;
+  __shared__ uint32_t tmem_base;
+  __shared__ double red[kOrthThreads / 32];
+  char* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rb = a.rows * 128;  // bytes of a block of 64 columns
+  char* x0 = sm;
+  char* x1 = x0 + a.xb * rb;
+  char* p0 = x1 + a.xb * rb;
+  char* p1 = p0 + a.pb * rb;
+  if (tid == 0) {
+    mbar_init(&bar, 1);
+    fence_barrier_init();
+  }
+  if (warp == 0) tmem_alloc(&tmem_base, a.tmem);
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = tmem_base;
+  // this thread's row of the accumulators and its half of their columns
+  const int row = (warp & 3) * 32 + lane, part = warp >> 2;
+  const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+  const bool active = (warp & 3) * 32 < a.rows;  // blocks of 64 rows: half of the warps have none
+  const int ksteps_x = (a.hi + 15) / 16, ksteps_p = (a.lo + 15) / 16;
+  const uint32_t idesc_p = product_idesc(1, a.np, 0, 0), idesc_x = product_idesc(1, a.xn, 0, 1);
+  constexpr float down = 1.f / kPlaneScale;
+  uint32_t phase = 0;
+  bool ok = true;
+
+  for (int64_t z = blockIdx.x; ok && z < a.batch; z += gridDim.x) {
+    const int64_t size = (int64_t)a.m * a.n, base = z * size;
+    double s = 0.0;
+    for (int64_t i = tid; i < size; i += kOrthThreads) {
+      const double v = load_x(a.g, base + i, a.dt);
+      s += v * v;
+    }
+    s = block_sum(s, red);
+    const double inv = 1.0 / (sqrt(s) + (double)a.eps);
+    if (a.steps == 0) {
+      for (int64_t i = tid; i < size; i += kOrthThreads)
+        store_y(a.q, base + i, a.dt, (float)(load_x(a.g, base + i, a.dt) * inv));
+      continue;
+    }
+    // X, zero outside lo x hi: the products then keep every padding zero
+    const int pieces = a.xb * 8;
+    for (int i = tid; i < a.rows * pieces; i += kOrthThreads) {
+      const int r = a.tall ? i % a.rows : i / pieces, c = (a.tall ? i / a.rows : i % pieces) * 8;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool in = r < a.lo && c + j < a.hi;
+        const int64_t at = base + (a.tall ? (int64_t)(c + j) * a.n + r : (int64_t)r * a.n + c + j);
+        v[j] = in ? (float)(load_x(a.g, at, a.dt) * inv * kPlaneScale) : 0.f;
+      }
+      put8(x0, x1, (c >> 6) * rb + sw128(r, c & 63), v);
+    }
+    fence_proxy_async();
+    __syncthreads();
+
+    for (int step = 0; ok && step < a.steps; ++step) {
+      // ---- P = X X^T ----
+      const uint32_t corr_p = tmem + a.chunks * a.np;
+      if (tid == 0) {
+        tmem_fence_after();
+        for (int pair = 0; pair < 3; ++pair) {
+          const uint64_t da = desc_kmajor(smem_u32(pair == 2 ? x1 : x0)), db = desc_kmajor(smem_u32(pair == 1 ? x1 : x0));
+          for (int k = 0; k < ksteps_x; ++k) {
+            const uint32_t off = (uint32_t)((k >> 2) * rb + (k & 3) * 32) >> 4;
+            const uint32_t d = pair == 0 ? tmem + (k >> 3) * a.np : corr_p;
+            mma_bf16(d, da + off, db + off, idesc_p, pair == 0 ? (k & 7) != 0 : (pair == 2 || k != 0));
+          }
+        }
+        mma_commit(&bar);
+      }
+      ok = mbar_wait(&bar, phase, nullptr);
+      phase ^= 1;
+      tmem_fence_after();
+      if (active)
+        for (int c = part * (a.np / 2); c < (part + 1) * (a.np / 2); c += 16) {
+          float v[16], u[16];
+          load16(corr_p + c + lanes, v);
+          for (int i = 0; i < a.chunks; ++i) {
+            load16(tmem + i * a.np + c + lanes, u);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] += u[j];
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] *= down;
+          put8(p0, p1, (c >> 6) * rb + sw128(row, c & 63), v);
+          put8(p0, p1, (c >> 6) * rb + sw128(row, (c & 63) + 8), v + 8);
+        }
+      tmem_fence_before();
+      fence_proxy_async();
+      ok = __syncthreads_and(ok);
+      if (!ok) break;
+      // ---- P <- b P + c P P ----
+      if (tid == 0) {
+        tmem_fence_after();
+        for (int pair = 0; pair < 3; ++pair) {
+          const uint64_t da = desc_kmajor(smem_u32(pair == 2 ? p1 : p0)), db = desc_kmajor(smem_u32(pair == 1 ? p1 : p0));
+          for (int k = 0; k < ksteps_p; ++k) {
+            const uint32_t off = (uint32_t)((k >> 2) * rb + (k & 3) * 32) >> 4;
+            mma_bf16(pair == 0 ? tmem : tmem + a.np, da + off, db + off, idesc_p, pair == 2 || k != 0);
+          }
+        }
+        mma_commit(&bar);
+      }
+      ok = mbar_wait(&bar, phase, nullptr);
+      phase ^= 1;
+      tmem_fence_after();
+      if (active)
+        for (int c = part * (a.np / 2); c < (part + 1) * (a.np / 2); c += 16) {
+          float v[16], u[16];
+          load16(tmem + a.np + c + lanes, v);
+          load16(tmem + c + lanes, u);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = (v[j] + u[j]) * (a.c * down);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t off = (c >> 6) * rb + sw128(row, (c & 63) + 8 * h);
+            add8(p0, p1, off, a.b, v + 8 * h);
+            put8(p0, p1, off, v + 8 * h);
+          }
+        }
+      tmem_fence_before();
+      fence_proxy_async();
+      ok = __syncthreads_and(ok);
+      if (!ok) break;
+      // ---- X <- a X + P X, by column chunks ----
+      const bool last = step == a.steps - 1;
+      for (int ch = 0; ch < a.chunks; ++ch) {
+        if (tid == 0) {
+          tmem_fence_after();
+          for (int pair = 0; pair < 3; ++pair) {
+            const uint64_t da = desc_kmajor(smem_u32(pair == 2 ? p1 : p0));
+            const uint64_t db = desc_mnmajor(smem_u32(pair == 1 ? x1 : x0) + 2 * ch * rb, rb);
+            for (int k = 0; k < ksteps_p; ++k)
+              mma_bf16(pair == 0 ? tmem : tmem + a.xn, da + ((uint32_t)((k >> 2) * rb + (k & 3) * 32) >> 4),
+                       db + ((uint32_t)(k * 2048) >> 4), idesc_x, pair == 2 || k != 0);
+          }
+          mma_commit(&bar);
+        }
+        ok = mbar_wait(&bar, phase, nullptr);
+        phase ^= 1;
+        tmem_fence_after();
+        if (active)
+          for (int c = part * (a.xn / 2); c < (part + 1) * (a.xn / 2); c += 16) {
+            const int col = ch * 128 + c;
+            if (col >= a.xb * 64) break;
+            float v[16], u[16];
+            load16(tmem + a.xn + c + lanes, v);
+            load16(tmem + c + lanes, u);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = (v[j] + u[j]) * down;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t off = (col >> 6) * rb + sw128(row, (col & 63) + 8 * h);
+              add8(x0, x1, off, a.a, v + 8 * h);
+              if (!last) put8(x0, x1, off, v + 8 * h);
+            }
+            if (last && row < a.lo) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (col + j < a.hi)
+                  store_y(a.q, base + (a.tall ? (int64_t)(col + j) * a.n + row : (int64_t)row * a.n + col + j), a.dt,
+                          v[j] * down);
+            }
+          }
+        tmem_fence_before();
+        fence_proxy_async();
+        ok = __syncthreads_and(ok);
+        if (!ok) break;
+      }
+    }
+  }
+  if (!ok) {  // a product may still be running: wait for it once more, then report
+    mbar_wait(&bar, phase ^ 1, nullptr);
+    if (tid == 0) atomicOr(&g_orth_status, 1);
+  }
+  tmem_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, a.tmem);
+}
+
+}  // namespace
+
+int orth_small_status(int* flag, cudaStream_t st) { return take_flag((const void*)&g_orth_status, flag, st); }
+
+bool orth_small_fits(int64_t m, int64_t n) {
+  const int64_t lo = std::min(m, n), hi = std::max(m, n);
+  return lo <= 64 ? hi <= 512 : lo <= 128 && hi <= 256;
+}
+
+int launch_orth_small(int dt, const void* g, int64_t batch, int64_t m, int64_t n, int steps, float a, float b, float c,
+                      float eps, void* q, cudaStream_t st) {
+  OrthArgs t{};
+  t.g = g;
+  t.q = q;
+  t.dt = dt;
+  t.batch = batch;
+  t.m = (int)m;
+  t.n = (int)n;
+  t.lo = (int)std::min(m, n);
+  t.hi = (int)std::max(m, n);
+  t.tall = m > n;
+  t.rows = t.lo <= 64 ? 64 : 128;
+  t.xb = (t.hi + 63) / 64;
+  t.pb = t.rows / 64;
+  t.np = t.rows;
+  t.xn = t.hi <= 64 ? 64 : 128;
+  t.chunks = (t.hi + 127) / 128;
+  const int cols = std::max((t.chunks + 1) * t.np, 2 * t.xn);
+  t.tmem = 128;
+  while (t.tmem < cols) t.tmem *= 2;
+  t.steps = steps;
+  t.a = a;
+  t.b = b;
+  t.c = c;
+  t.eps = eps;
+  // 128 operand rows are read from blocks of 64: 8 KB behind the last block, and 1 KB of alignment
+  int smem = 2 * (t.xb + t.pb) * t.rows * 128 + 8192 + 1024;
+  // as many blocks per SM as tensor memory serves (an SM that held more would let them wait for it)
+  const int per_sm = std::min(512 / t.tmem, std::max(1, (232448 - 4096) / (smem + 2048)));
+  smem = std::max(smem, 226 * 1024 / per_sm - 3072);
+  static SmemGrants grants;
+  if (int rc = allow_smem((const void*)orth_small_kernel, 231424, grants)) return rc;
+  int sms = 0;
+  if (int rc = device_sms(&sms)) return rc;
+  const unsigned grid = (unsigned)std::min<int64_t>(batch, (int64_t)sms * per_sm);
+  orth_small_kernel<<<grid, kOrthThreads, smem, st>>>(t);
+  return check_launch("orth_small_kernel");
+}
+
+}  // namespace experts
+}  // namespace gmmxx

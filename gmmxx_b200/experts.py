@@ -26,8 +26,9 @@ chain with :func:`grouped_matmul_backward`).
 
 from __future__ import annotations
 
+import functools
 import math
-from typing import NamedTuple, Optional, Sequence, Tuple
+from typing import Dict, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -74,10 +75,38 @@ def _same_device(dev: torch.device, **tensors) -> None:
             raise ValueError(f"{name} is on {t.device}, expected {dev}")
 
 
+_NO_WORKSPACE: Dict[torch.device, torch.Tensor] = {}
+
+
 def _workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
     # of its own per call, from the caching allocator: calls on several streams
-    # and captured graphs never share one
-    return torch.empty(max(256, nbytes), dtype=torch.uint8, device=dev)
+    # and captured graphs never share one.  Calls that need none (the 256 bytes
+    # every size starts from are alignment) pass one block that no kernel touches.
+    if nbytes > 256:
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = _NO_WORKSPACE.get(dev)
+    if ws is None:
+        ws = torch.empty(256, dtype=torch.uint8, device=dev)
+        if not torch.cuda.is_current_stream_capturing():  # a capture's memory is its graph's
+            _NO_WORKSPACE[dev] = ws
+    return ws
+
+
+# the current stream's handle without building a torch.cuda.Stream (2 us of a call's host time)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(dev: torch.device) -> int:
+    return _raw_stream(dev.index) if _raw_stream is not None else engine._stream_ptr(dev)
+
+
+def _call(name: str, dev: torch.device, *args) -> None:
+    """A C entry point on dev's current stream, with dev current."""
+    if torch.cuda.current_device() == dev.index:
+        nat.call(name, *args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            nat.call(name, *args, _stream(dev))
 
 
 def check_products_status(device=None) -> None:
@@ -114,13 +143,12 @@ def group_rows(labels: torch.Tensor, n_groups: int) -> RowGroups:
         raise ValueError("labels must have at least one choice per row")
     slots, dev = labels.numel(), labels.device
     tiles_len = nat.group_tiles_len(slots, n_groups)
-    order = torch.empty((slots,), dtype=torch.int32, device=dev)
-    offsets = torch.empty((n_groups + 1,), dtype=torch.int32, device=dev)
-    tiles = torch.empty((tiles_len,), dtype=torch.int32, device=dev)
+    # one block for the three results
+    order, offsets, tiles = torch.empty((slots + n_groups + 1 + tiles_len,), dtype=torch.int32,
+                                        device=dev).split((slots, n_groups + 1, tiles_len))
     ws = _workspace(nat.group_rows_workspace_bytes(slots, n_groups), dev)
-    with torch.cuda.device(dev):
-        nat.call("gmmxx_group_rows", labels.data_ptr(), labels.element_size(), slots, n_groups, order.data_ptr(),
-                 offsets.data_ptr(), tiles.data_ptr(), ws.data_ptr(), ws.numel(), engine._stream_ptr(dev))
+    _call("gmmxx_group_rows", dev, labels.data_ptr(), labels.element_size(), slots, n_groups, order.data_ptr(),
+          offsets.data_ptr(), tiles.data_ptr(), ws.data_ptr(), ws.numel())
     return RowGroups(order, offsets, tiles, labels.shape[0], top, n_groups, tuple(labels.shape))
 
 
@@ -181,10 +209,9 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups,
     dt = engine._X_DTYPES[x.dtype]
     out = torch.empty((*groups.shape, n_out), dtype=x.dtype, device=dev)
     ws = _workspace(nat.grouped_matmul_workspace_bytes(dt, groups.n_rows, groups.top_k, k, n_in, n_out), dev)
-    with torch.cuda.device(dev):
-        nat.call("gmmxx_grouped_matmul", dt, x.data_ptr(), groups.n_rows, groups.top_k, k, n_in, n_out,
-                 groups.order.data_ptr(), groups.offsets.data_ptr(), groups.tiles.data_ptr(), w.data_ptr(), wt,
-                 engine._p(bias), out.data_ptr(), ws.data_ptr(), ws.numel(), engine._stream_ptr(dev))
+    _call("gmmxx_grouped_matmul", dev, dt, x.data_ptr(), groups.n_rows, groups.top_k, k, n_in, n_out,
+          groups.order.data_ptr(), groups.offsets.data_ptr(), groups.tiles.data_ptr(), w.data_ptr(), wt,
+          engine._p(bias), out.data_ptr(), ws.data_ptr(), ws.numel())
     return out
 
 
@@ -209,28 +236,37 @@ def grouped_matmul_backward(grad_out: torch.Tensor, x: torch.Tensor, weight: tor
     grad_w = torch.empty_like(w) if need_weight else None
     grad_b = torch.empty((k, n_out), dtype=x.dtype, device=dev) if bias else None
     ws = _workspace(nat.grouped_matmul_backward_workspace_bytes(dt, groups.n_rows, groups.top_k, k, n_in, n_out), dev)
-    with torch.cuda.device(dev):
-        nat.call("gmmxx_grouped_matmul_backward", dt, grad_out.data_ptr(), x.data_ptr(), groups.n_rows, groups.top_k,
-                 k, n_in, n_out, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.tiles.data_ptr(),
-                 w.data_ptr(), wt, engine._p(grad_x), engine._p(grad_w), engine._p(grad_b), ws.data_ptr(),
-                 ws.numel(), engine._stream_ptr(dev))
+    _call("gmmxx_grouped_matmul_backward", dev, dt, grad_out.data_ptr(), x.data_ptr(), groups.n_rows, groups.top_k, k,
+          n_in, n_out, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.tiles.data_ptr(), w.data_ptr(), wt,
+          engine._p(grad_x), engine._p(grad_w), engine._p(grad_b), ws.data_ptr(), ws.numel())
     if grad_w is not None and wt:
         grad_w = grad_w.transpose(1, 2)
     return grad_x, grad_w, grad_b
 
 
+def _largest(points, f) -> float:
+    return max(abs(f(p)) for p in points)
+
+
+@functools.lru_cache(maxsize=64)
 def _check_polynomial(a: float, b: float, c: float, steps: int) -> None:
     """Refuse coefficients that carry a singular value of [0, 1] beyond what the
     kernels' 16-bit planes hold: with |X|_F <= 1 at the start, the iterates'
     singular values are those of the scalar polynomial."""
     if not all(math.isfinite(v) for v in (a, b, c)):
         raise ValueError("coefficients must be finite")
+    # where a s + b s^3 + c s^5 and b s^2 + c s^4 turn (in s^2)
+    turns = [-b / (2.0 * c)] if c != 0.0 else []
+    disc = 9.0 * b * b - 20.0 * a * c
+    if c != 0.0 and disc >= 0.0:
+        turns += [(-3.0 * b + r * math.sqrt(disc)) / (10.0 * c) for r in (1.0, -1.0)]
+    elif c == 0.0 and b != 0.0:
+        turns.append(-a / (3.0 * b))
     top = 1.0
     for _ in range(steps):
-        # |a s + b s^3 + c s^5| over [0, top], and the products on the way
-        grid = [top * i / 512.0 for i in range(513)]
-        inner = max(abs(b * s * s + c * s**4) for s in grid)
-        top = max(abs(a * s + b * s**3 + c * s**5) for s in grid)
+        points = [top] + [math.sqrt(q) for q in turns if 0.0 < q < top * top]
+        inner = _largest(points, lambda s: b * s * s + c * s**4)
+        top = _largest(points, lambda s: a * s + b * s**3 + c * s**5)
         if top > 2.0 or inner > 8.0:
             raise ValueError("coefficients make the iteration diverge: a singular value of [0, 1] leaves [-2, 2]")
 
@@ -263,7 +299,6 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients: Sequence[float]
         return q
     dev, dt = g.device, engine._X_DTYPES[g.dtype]
     ws = _workspace(nat.orthogonalize_workspace_bytes(dt, batch, m, n), dev)
-    with torch.cuda.device(dev):
-        nat.call("gmmxx_orthogonalize", dt, g.data_ptr(), batch, m, n, steps, a, b, c, eps, q.data_ptr(),
-                 ws.data_ptr(), ws.numel(), engine._stream_ptr(dev))
+    _call("gmmxx_orthogonalize", dev, dt, g.data_ptr(), batch, m, n, steps, a, b, c, eps, q.data_ptr(), ws.data_ptr(),
+          ws.numel())
     return q
