@@ -122,6 +122,12 @@ int tile_columns(int64_t row_tiles, int64_t n, int planes, int max_bn) {
   return bn;
 }
 
+// Pairs of blocks on tiles of 256 x 256: one plane, and enough tiles of at
+// least half a pair's rows to give every pair one (a ragged group's last tile
+// wastes 128 rows on average, which the pair's faster stages pay for from
+// groups of about 256 rows on).
+int pair_of(int planes, int bn, int64_t pair_tiles) { return planes == 1 && bn == 256 && pair_tiles >= 74 ? 2 : 1; }
+
 int elem_size(int dt) { return dt == GMMXX_FLOAT32 ? 4 : 2; }
 // four elements at a time: rows of a multiple of four elements
 bool vec_ok(const void* p, int dt, int64_t ld) {
@@ -136,24 +142,27 @@ bool vec_ok(const void* p, int dt, int64_t ld) {
 int rows_product(int dt, const Planes& src, int div, const Groups& g, int64_t k_dim, int64_t n,
                  const Planes& w, bool b_kmajor, const void* bias, void* out, int out_dt, cudaStream_t st) {
   const int bn = tile_columns(ceil_div(g.slots(), kTileRows), n, src.n, 256);
+  const int pair = g.slots() >= (int64_t)kPairRows * g.K ? pair_of(src.n, bn, g.slots() / kPairRows * ceil_div(n, bn)) : 1;
+  const int rows_per = pair * kTileRows;
   ProductMaps maps;
   if (src.n > 1)
     if (int rc = stack_maps(src, k_dim, g.slots(), 1, kTileRows, maps.a)) return rc;
-  if (int rc = b_kmajor ? stack_maps(w, k_dim, n, g.K, bn, maps.b) : stack_maps(w, n, k_dim, g.K, kBlockK, maps.b))
+  if (int rc = b_kmajor ? stack_maps(w, k_dim, n, g.K, bn / pair, maps.b) : stack_maps(w, n, k_dim, g.K, kBlockK, maps.b))
     return rc;
   ProductArgs a{};
   a.n = (int)n;
   a.k = (int)k_dim;
   a.bn = bn;
-  a.stages = product_stages(src.n, bn);
+  a.stages = product_stages(src.n, bn, pair);
   a.mt = 1;
   a.nt = (int)ceil_div(n, bn);
   a.b_mn = b_kmajor ? 0 : 1;
-  a.idesc = product_idesc(src.fp16, bn, 0, a.b_mn);
+  a.idesc = product_idesc(src.fp16, bn, 0, a.b_mn, pair);
   a.order = g.order;
   a.src_a = static_cast<const char*>(src.base[0]);
   a.ld_a = src.ld;
-  a.table = g.tiles;
+  a.count = g.tiles + (pair == 2 ? 1 : 0);
+  a.table = g.tile_table(rows_per);
   a.div_a = div;
   a.div_b = 1;
   a.groups = g.K;
@@ -163,7 +172,7 @@ int rows_product(int dt, const Planes& src, int div, const Groups& g, int64_t k_
   a.vec = vec_ok(out, out_dt, n);
   a.bias = bias;
   a.bias_dt = dt;
-  return launch_product(kRows, src.n, maps, a, g.max_tiles(), st);
+  return launch_product(kRows, src.n, pair, maps, a, g.max_tiles(rows_per), st);
 }
 
 // gx[row] = sum over the row's slots, rounded once
@@ -466,6 +475,7 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
     const int64_t m = wt ? n_out : n_in, n = wt ? n_in : n_out;
     const int planes = planes_of(dt);
     const int bn = tile_columns(p.max_segs * ceil_div(m, 128), n, planes, 256);
+    const int pair = m > 128 ? pair_of(planes, bn, p.max_segs * ceil_div(m, 256) * ceil_div(n, bn)) : 1;
     ProductMaps maps;
     if (planes > 1) {
       if (int rc = stack_maps(px, n_in, slots, 1, kBlockK, wt ? maps.b : maps.a)) return rc;
@@ -475,18 +485,19 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
     a.m = (int)m;
     a.n = (int)n;
     a.bn = bn;
-    a.stages = product_stages(planes, bn);
-    a.mt = (int)ceil_div(m, 128);
+    a.stages = product_stages(planes, bn, pair);
+    a.mt = (int)ceil_div(m, 128 * pair);
     a.nt = (int)ceil_div(n, bn);
     a.a_mn = a.b_mn = 1;
-    a.idesc = product_idesc(px.fp16, bn, 1, 1);
+    a.idesc = product_idesc(px.fp16, bn, 1, 1, pair);
     a.order = g.order;
     const Planes &pa = wt ? pg : px, &pb = wt ? px : pg;
     a.src_a = static_cast<const char*>(pa.base[0]);
     a.src_b = static_cast<const char*>(pb.base[0]);
     a.ld_a = pa.ld;
     a.ld_b = pb.ld;
-    a.table = table;
+    a.count = table;
+    a.table = table + kSegHeader;
     a.div_a = wt ? 1 : g.top;
     a.div_b = wt ? g.top : 1;
     a.groups = g.K;
@@ -496,7 +507,7 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
     a.out_stride = m * n;
     a.vec = vec_ok(gw, dt, n);
     a.part = part;
-    if (int rc = launch_product(kWeights, planes, maps, a, p.max_segs, st)) return rc;
+    if (int rc = launch_product(kWeights, planes, pair, maps, a, p.max_segs, st)) return rc;
     if (p.max_split > 0) {
       join_kernel<<<148 * 8, 256, 0, st>>>(table, split, part, m * n, gw, dt);
       if (int rc = check_launch("join_kernel")) return rc;
@@ -553,20 +564,21 @@ int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_
   auto product = [&](const Stack& A, bool a_mn, const Stack& B, bool b_mn, int64_t rows, int64_t cols, int64_t k,
                      float alpha, float beta, const Stack* E, const Stack& O, void* out) {
     const int bn = tile_columns(batch * ceil_div(rows, 128), cols, s.planes, max_bn);
+    const int pair = rows > 128 ? pair_of(s.planes, bn, batch * ceil_div(rows, 256) * ceil_div(cols, bn)) : 1;
     ProductMaps maps;
     if (int rc = stack_operand(A, s.planes, batch, a_mn ? kBlockK : 128, maps.a)) return rc;
-    if (int rc = stack_operand(B, s.planes, batch, b_mn ? kBlockK : bn, maps.b)) return rc;
+    if (int rc = stack_operand(B, s.planes, batch, b_mn ? kBlockK : bn / pair, maps.b)) return rc;
     ProductArgs t{};
     t.m = (int)rows;
     t.n = (int)cols;
     t.k = (int)k;
     t.bn = bn;
-    t.stages = product_stages(s.planes, bn);
-    t.mt = (int)ceil_div(rows, 128);
+    t.stages = product_stages(s.planes, bn, pair);
+    t.mt = (int)ceil_div(rows, 128 * pair);
     t.nt = (int)ceil_div(cols, bn);
     t.a_mn = a_mn;
     t.b_mn = b_mn;
-    t.idesc = product_idesc(1, bn, a_mn, b_mn);
+    t.idesc = product_idesc(1, bn, a_mn, b_mn, pair);
     t.items = batch;
     t.alpha = alpha / kPlaneScale;
     t.beta = beta;
@@ -581,7 +593,7 @@ int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_
     t.ldo = cols;
     t.out_stride = rows * cols;
     t.vec = vec_ok(out, dt, cols) && vec_ok(out, dt, rows * cols);
-    return launch_product(kBatch, s.planes, maps, t, batch, st);
+    return launch_product(kBatch, s.planes, pair, maps, t, batch, st);
   };
   for (int i = 0; i < steps; ++i) {
     void* out = i == steps - 1 ? q : nullptr;

@@ -10,7 +10,8 @@ namespace gmmxx {
 namespace experts {
 
 constexpr int kTileRows = 128;   // rows of one tile: the M extent of a tcgen05 tile
-constexpr int kTileHeader = 4;   // tiles[0]: number of tiles
+constexpr int kPairRows = 256;   // and of a pair of blocks' tile
+constexpr int kTileHeader = 4;   // tiles[0]: number of 128-row tiles, tiles[1]: of 256-row tiles
 constexpr int kTileInts = 3;     // per tile: group, first position in the sorted order, rows
 constexpr int64_t kMaxGroups = 32768;
 
@@ -23,8 +24,16 @@ struct Groups {
   int top;
   int K;
   int64_t slots() const { return rows * top; }
-  int64_t max_tiles() const { return slots() / kTileRows + (K + 1 < slots() ? K + 1 : slots()); }
+  int64_t max_tiles(int rows_per = kTileRows) const;
+  const int32_t* tile_table(int rows_per) const;  // its first entry
 };
+
+// most tiles of `per` rows that K groups and the unassigned slots can take
+inline int64_t most_tiles(int64_t slots, int64_t K, int per) { return slots / per + (K + 1 < slots ? K + 1 : slots); }
+inline int64_t Groups::max_tiles(int per) const { return most_tiles(slots(), K, per); }
+inline const int32_t* Groups::tile_table(int per) const {
+  return tiles + kTileHeader + (per == kPairRows ? kTileInts * most_tiles(slots(), K, kTileRows) : 0);
+}
 
 int64_t tiles_len(int64_t slots, int64_t K);
 size_t group_rows_ws(int64_t slots, int64_t K);

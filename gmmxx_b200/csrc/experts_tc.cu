@@ -16,11 +16,15 @@
 // at 18 % and 7 %.)  The copies complete on the stage's mbarrier; a warp of its own
 // waits for it, fences the proxies and passes the stage on (the fence costs the
 // thread that issues the products 5 % of its time).  Rows behind a
-// segment's last are filled with zeros; kRows fetches copies of the tile's first
-// row there and does not store them.  Planes of fp32 rows are laid out sorted
+// segment's or tile's last are filled with zeros.  Planes of fp32 rows are laid out sorted
 // before the launch and loaded as TMA tiles; there the last stage of a kWeights
 // segment also holds the next group's rows, which are zeroed in both operands
 // before the products (zeroing one would leave NaN * 0).
+//
+// Pairs.  Where there are enough full tiles two blocks (a cluster of two SMs)
+// share one of 256 x 256 (cta_group::2): each loads its 128 rows of A and half
+// of B, 32 KB per stage instead of 48, which the six stages that then fit hide
+// the latency of (four stages of 48 KB keep the tensor pipe at 64 %).
 //
 // Sums.  The tensor core adds to an accumulator by cutting, not rounding: an
 // addition costs about 3.4e-8 of the sum, always towards zero (measured: 8e-7
@@ -83,8 +87,60 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
+// kind::f16: the types are the descriptor's
+template <int CG>
 __device__ __forceinline__ void mma_16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  mma_bf16(d, a, b, idesc, acc);  // kind::f16: the types are the descriptor's
+  if (CG == 1) {
+    mma_bf16(d, a, b, idesc, acc);
+  } else {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  }
+}
+// arrives on the barrier (in both blocks of a pair) when the products issued so far are done
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if (CG == 1) {
+    mma_commit(bar);
+  } else {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  }
+}
+// arrives on the leading block's barrier
+template <int CG>
+__device__ __forceinline__ void arrive_leader(uint64_t* bar) {
+  if (CG == 1) {
+    mbar_arrive(bar);
+  } else {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(map_shared(smem_u32(bar), 0))
+                 : "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_take(uint32_t* dst, uint32_t cols) {
+  if (CG == 1) {
+    tmem_alloc(dst, cols);
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_give(uint32_t addr, uint32_t cols) {
+  if (CG == 1) tmem_dealloc(addr, cols);
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void block_or_pair_sync() {
+  if (CG == 1) __syncthreads();
+  else cluster_sync();
 }
 
 // a bounded wait ran out: every warp of the block stops at its next wait
@@ -99,7 +155,7 @@ __device__ __forceinline__ void give_up(Bars* bars, int lane) {
 __device__ __forceinline__ bool mbar_test(uint64_t* b, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
       " selp.u32 %0, 1, 0, p;\n}"
       : "=r"(ok)
       : "r"(smem_u32(b)), "r"(parity)
@@ -131,29 +187,30 @@ struct Tile {
 
 template <int KIND>
 __device__ __forceinline__ int64_t tile_count(const ProductArgs& a) {
-  const int64_t items = KIND == kBatch ? a.items : (int64_t)__ldg(a.table);
+  const int64_t items = KIND == kBatch ? a.items : (int64_t)__ldg(a.count);
   return items * a.mt * a.nt;
 }
 
-template <int KIND>
-__device__ __forceinline__ Tile decode(const ProductArgs& a, int64_t it) {
+// this block's part (its 128 rows) of tile `it` of CG * 128 rows
+template <int KIND, int CG>
+__device__ __forceinline__ Tile decode(const ProductArgs& a, int64_t it, int rank) {
   Tile t;
   t.n0 = (int)(it % a.nt) * a.bn;
   it /= a.nt;
   if (KIND == kRows) {
-    const int32_t* e = a.table + kTileHeader + it * kTileInts;
+    const int32_t* e = a.table + it * kTileInts;
     t.g = __ldg(e);
-    t.pos = __ldg(e + 1);
-    t.rows = __ldg(e + 2);
+    t.pos = __ldg(e + 1) + rank * kBM;
+    t.rows = max(0, min(kBM, __ldg(e + 2) - rank * kBM));
     t.m0 = 0;
     t.slot = -1;
     t.kb = t.g < a.groups ? (a.k + kBlockK - 1) / kBlockK : 0;
     return t;
   }
-  t.m0 = (int)(it % a.mt) * kBM;
+  t.m0 = ((int)(it % a.mt) * CG + rank) * kBM;
   it /= a.mt;
   if (KIND == kWeights) {
-    const int32_t* e = a.table + kSegHeader + it * kSegInts;
+    const int32_t* e = a.table + it * kSegInts;
     t.g = __ldg(e);
     t.pos = __ldg(e + 1);
     t.rows = __ldg(e + 2);
@@ -206,23 +263,27 @@ __device__ __forceinline__ void store4(void* out, int dt, int64_t at, float4 v) 
   }
 }
 
-template <int KIND, int PLANES>
+template <int KIND, int PLANES, int CG>
 struct Roles {
   static constexpr bool kGather = KIND != kBatch && PLANES == 1;      // rows by cp.async
   static constexpr bool kTma = !(KIND == kWeights && PLANES == 1);    // something by TMA
   static constexpr int kThreads = kGather ? 512 : 384;
+  static constexpr bool kRelay = kGather || CG > 1;                   // stages reach the products through `ready`
   static constexpr int kFullCount = (kGather ? kGatherThreads : 0) + (kTma ? 1 : 0);
 };
 
-template <int KIND, int PLANES>
-__global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
+template <int KIND, int PLANES, int CG>
+__global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
     product_kernel(const __grid_constant__ ProductMaps maps, const ProductArgs a) {
-  using R = Roles<KIND, PLANES>;
+  using R = Roles<KIND, PLANES, CG>;
   extern __shared__ __align__(1024) char smem_raw[];
   __shared__ Bars bars;
   char* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int bbytes = a.bn * 128;  // one plane of B per stage
+  const int rank = CG == 1 ? 0 : (int)cluster_rank();
+  const int bcols = a.bn / CG;     // columns of B that this block loads
+  const int bbytes = bcols * 128;  // one plane of B per stage
+  const int64_t first = blockIdx.x / CG, stride = gridDim.x / CG;
   const int stage_bytes = PLANES * (kABytes + bbytes);
   volatile int* abort = &bars.abort;
   // two buffers of one accumulator, or of two (leading products, others)
@@ -232,18 +293,18 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
       mbar_init(&bars.full[i], R::kFullCount);
-      mbar_init(&bars.ready[i], 1);
+      mbar_init(&bars.ready[i], CG);
       mbar_init(&bars.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.accfull[i], 1);
-      mbar_init(&bars.accempty[i], kEpiWarps);
+      mbar_init(&bars.accempty[i], CG * kEpiWarps);
     }
     bars.abort = 0;
     fence_barrier_init();
   }
-  if (warp == 2) tmem_alloc(&bars.tmem_base, tmem_cols);
-  __syncthreads();
+  if (warp == 2) tmem_take<CG>(&bars.tmem_base, tmem_cols);
+  block_or_pair_sync<CG>();
   tmem_fence_after();
   const uint32_t tmem = bars.tmem_base;
   const int64_t total = tile_count<KIND>(a);
@@ -258,25 +319,25 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
     int64_t filled = 0;
     bool ok = true;
     const uint32_t bytes = (uint32_t)(R::kGather ? bbytes : stage_bytes);
-    for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
-      const Tile t = decode<KIND>(a, it);
+    for (int64_t it = first; ok && it < total; it += stride) {
+      const Tile t = decode<KIND, CG>(a, it, rank);
       for (int kb = 0; kb < t.kb; ++kb, ring.step(a.stages), ++filled) {
         const int s = ring.i;
-        ok = mbar_wait_warp(&bars.empty[s], ring.phase ^ 1, abort);
+        ok = wait_phase_warp(&bars.empty[s], ring.phase ^ 1, abort);
         if (!ok) break;
         char* sa = sm + s * stage_bytes;
         char* sb = sa + PLANES * kABytes;
         uint64_t* bar = &bars.full[s];
         if (lane == 0) mbar_expect_tx(bar, bytes);
         __syncwarp();
-        const int k0 = kb * kBlockK;
+        const int k0 = kb * kBlockK, nb = t.n0 + rank * bcols;
 #pragma unroll
         for (int p = 0; p < PLANES; ++p) {
           char* pa = sa + p * kABytes;
           char* pb = sb + p * bbytes;
           if (KIND == kWeights) {  // 64 sorted rows x 64 columns per box
             if (lane < 2) tma_load_3d(pa + lane * 8192, &maps.a[p], t.m0 + lane * 64, t.pos + k0, 0, bar);
-            if (lane < a.bn / 64) tma_load_3d(pb + lane * 8192, &maps.b[p], t.n0 + lane * 64, t.pos + k0, 0, bar);
+            if (lane < bcols / 64) tma_load_3d(pb + lane * 8192, &maps.b[p], nb + lane * 64, t.pos + k0, 0, bar);
             continue;
           }
           if (KIND == kRows) {
@@ -287,21 +348,21 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
             if (lane == 0) tma_load_3d(pa, &maps.a[p], k0, t.m0, t.g, bar);
           }
           if (a.b_mn) {
-            if (lane < a.bn / 64) tma_load_3d(pb + lane * 8192, &maps.b[p], t.n0 + lane * 64, k0, t.g, bar);
+            if (lane < bcols / 64) tma_load_3d(pb + lane * 8192, &maps.b[p], nb + lane * 64, k0, t.g, bar);
           } else {
-            if (lane == 0) tma_load_3d(pb, &maps.b[p], k0, t.n0, t.g, bar);
+            if (lane == 0) tma_load_3d(pb, &maps.b[p], k0, nb, t.g, bar);
           }
         }
       }
     }
     if (!ok) {  // the copies in flight still write shared memory: wait for them before the block ends
       give_up(&bars, lane);
-      const int64_t first = filled > a.stages ? filled - a.stages : 0;
-      for (int64_t f = first; f < filled; ++f) mbar_wait_warp(&bars.full[f % a.stages], (uint32_t)((f / a.stages) & 1), nullptr);
+      const int64_t oldest = filled > a.stages ? filled - a.stages : 0;
+      for (int64_t f = oldest; f < filled; ++f) wait_phase_warp(&bars.full[f % a.stages], (uint32_t)((f / a.stages) & 1), nullptr);
     }
   } else if (PLANES == 1 && warp == 1) {
-    // ---- products of one plane: one thread ----
-    if (lane == 0) {
+    // ---- products of one plane: one thread (of the leading block) ----
+    if (lane == 0 && rank == 0) {
       Ring ring, sums;
       int64_t use = 0;
       bool ok = true, peeked = false;  // peeked: the stage at `ring` is known to be there
@@ -311,22 +372,22 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
       const uint64_t desc_b = a.b_mn ? desc_mnmajor(sb0, 8192) : desc_kmajor(sb0);
       const uint32_t stage_units = (uint32_t)stage_bytes >> 4;
       const uint32_t idesc = a.idesc;
-      uint64_t* there = R::kGather ? bars.ready : bars.full;
+      uint64_t* there = R::kRelay ? bars.ready : bars.full;
       Tile t{};
-      if (blockIdx.x < total) t = decode<KIND>(a, blockIdx.x);
-      for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
-        const int64_t ahead = it + gridDim.x < total ? it + gridDim.x : it;
+      if (first < total) t = decode<KIND, CG>(a, first, rank);
+      for (int64_t it = first; ok && it < total; it += stride) {
+        const int64_t ahead = it + stride < total ? it + stride : it;
         if (t.kb == 0) {
-          t = decode<KIND>(a, ahead);
+          t = decode<KIND, CG>(a, ahead, rank);
           continue;
         }
-        ok = mbar_wait(&bars.accempty[sums.i], sums.phase ^ 1, abort);
+        ok = wait_phase(&bars.accempty[sums.i], sums.phase ^ 1, abort);
         if (!ok) break;
         tmem_fence_after();
         const uint32_t d = tmem + sums.i * a.bn;
         Tile u = t;
         for (int kb = 0; kb < t.kb; ++kb, ++use) {
-          if (!peeked) ok = mbar_wait(&there[ring.i], ring.phase, abort);
+          if (!peeked) ok = wait_phase(&there[ring.i], ring.phase, abort);
           if (!ok) break;
           tmem_fence_after();
           const uint64_t da = desc_a + (uint32_t)ring.i * stage_units, db = desc_b + (uint32_t)ring.i * stage_units;
@@ -335,43 +396,44 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
           const int steps = KIND == kWeights && last ? min(4, (t.rows - kb * kBlockK + 15) >> 4) : 4;
           ring.step(a.stages);
           if (steps == 4) {
-            mma_16(d, da, db, idesc, kb != 0);
-            mma_16(d, da + step_a, db + step_b, idesc, 1);
+            mma_16<CG>(d, da, db, idesc, kb != 0);
+            mma_16<CG>(d, da + step_a, db + step_b, idesc, 1);
             // While these run: whether the next stage is there, or what comes after this tile.  The
             // tensor core takes few products ahead, so what stands between two stages' products is idle time.
-            if (last) u = decode<KIND>(a, ahead);
+            if (last) u = decode<KIND, CG>(a, ahead, rank);
             peeked = mbar_test(&there[ring.i], ring.phase);
-            mma_16(d, da + 2 * step_a, db + 2 * step_b, idesc, 1);
-            mma_16(d, da + 3 * step_a, db + 3 * step_b, idesc, 1);
+            mma_16<CG>(d, da + 2 * step_a, db + 2 * step_b, idesc, 1);
+            mma_16<CG>(d, da + 3 * step_a, db + 3 * step_b, idesc, 1);
           } else {
-            for (int k = 0; k < steps; ++k) mma_16(d, da + k * step_a, db + k * step_b, idesc, (kb | k) != 0);
-            u = decode<KIND>(a, ahead);
+            for (int k = 0; k < steps; ++k) mma_16<CG>(d, da + k * step_a, db + k * step_b, idesc, (kb | k) != 0);
+            u = decode<KIND, CG>(a, ahead, rank);
             peeked = false;
           }
-          mma_commit(done);
-          if (last) mma_commit(&bars.accfull[sums.i]);
+          commit<CG>(done);
+          if (last) commit<CG>(&bars.accfull[sums.i]);
         }
         sums.step(2);
         t = u;
       }
       if (!ok) {  // products in flight still read shared and write tensor memory
         give_up(&bars, 0);
-        const int64_t first = use > a.stages ? use - a.stages : 0;
-        for (int64_t f = first; f < use; ++f) mbar_wait(&bars.empty[f % a.stages], (uint32_t)((f / a.stages) & 1), nullptr);
+        const int64_t oldest = use > a.stages ? use - a.stages : 0;
+        for (int64_t f = oldest; f < use; ++f) wait_phase(&bars.empty[f % a.stages], (uint32_t)((f / a.stages) & 1), nullptr);
       }
     }
-  } else if (R::kGather && warp == 3) {
-    // ---- stages whose copies have landed: fence the proxies (cp.async wrote through the generic one) ----
+  } else if (R::kRelay && warp == 3) {
+    // ---- stages whose copies have landed: fence the proxies (cp.async wrote through the generic one), tell the
+    // thread that issues the products ----
     Ring ring;
     bool ok = true;
-    for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
-      const int n = decode<KIND>(a, it).kb;
+    for (int64_t it = first; ok && it < total; it += stride) {
+      const int n = decode<KIND, CG>(a, it, rank).kb;
       for (int kb = 0; kb < n; ++kb, ring.step(a.stages)) {
-        ok = mbar_wait_warp(&bars.full[ring.i], ring.phase, abort);
+        ok = wait_phase_warp(&bars.full[ring.i], ring.phase, abort);
         if (!ok) break;
-        fence_proxy_async();
+        if (R::kGather) fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.ready[ring.i]);
+        if (lane == 0) arrive_leader<CG>(&bars.ready[ring.i]);
       }
     }
     if (!ok) give_up(&bars, lane);
@@ -387,22 +449,22 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
     const uint64_t desc_b = a.b_mn ? desc_mnmajor(sb0, 8192) : desc_kmajor(sb0);
     const uint32_t stage_units = (uint32_t)stage_bytes >> 4, b_units = (uint32_t)bbytes >> 4;
     const uint32_t idesc = a.idesc;
-    for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
-      const Tile t = decode<KIND>(a, it);
+    for (int64_t it = first; ok && it < total; it += stride) {
+      const Tile t = decode<KIND, CG>(a, it, rank);
       int buf = 0;
       uint32_t d = 0;
       for (int kb = 0; kb < t.kb; ++kb, ring.step(a.stages), ++use) {
         const int in_sum = PLANES > 1 ? kb % kChunk : kb;  // stages already in this accumulator
         if (in_sum == 0) {
           buf = sums.i;
-          ok = mbar_wait_warp(&bars.accempty[buf], sums.phase ^ 1, abort);
+          ok = wait_phase_warp(&bars.accempty[buf], sums.phase ^ 1, abort);
           if (!ok) break;
           tmem_fence_after();
           d = tmem + buf * kAccs * a.bn;
           sums.step(2);
         }
         const int s = ring.i;
-        ok = mbar_wait_warp(&bars.full[s], ring.phase, abort);
+        ok = wait_phase_warp(&bars.full[s], ring.phase, abort);
         if (!ok) break;
         int steps = 4;
         if (KIND == kWeights) {
@@ -436,9 +498,9 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
             const bool add = in_sum != 0 || c > 1;
             if (steps == 4) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) mma_16(dc, da + k * step_a, db + k * step_b, idesc, k != 0 || add);
+              for (int k = 0; k < 4; ++k) mma_16<CG>(dc, da + k * step_a, db + k * step_b, idesc, k != 0 || add);
             } else {
-              for (int k = 0; k < steps; ++k) mma_16(dc, da + k * step_a, db + k * step_b, idesc, k != 0 || add);
+              for (int k = 0; k < steps; ++k) mma_16<CG>(dc, da + k * step_a, db + k * step_b, idesc, k != 0 || add);
             }
           }
           mma_commit(&bars.empty[s]);
@@ -449,8 +511,8 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
     }
     if (!ok) {  // products in flight still read shared and write tensor memory
       give_up(&bars, lane);
-      const int64_t first = use > a.stages ? use - a.stages : 0;
-      for (int64_t u = first; u < use; ++u) mbar_wait_warp(&bars.empty[u % a.stages], (uint32_t)((u / a.stages) & 1), nullptr);
+      const int64_t oldest = use > a.stages ? use - a.stages : 0;
+      for (int64_t u = oldest; u < use; ++u) wait_phase_warp(&bars.empty[u % a.stages], (uint32_t)((u / a.stages) & 1), nullptr);
     }
   } else if (warp >= kEpiWarp0 && warp < kEpiWarp0 + kEpiWarps) {
     // ---- results ----
@@ -459,15 +521,15 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
     const int c_lo = (w >> 2) * (a.bn / 2), c_hi = c_lo + a.bn / 2;
     Ring sums;
     bool ok = true;
-    for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
-      const Tile t = decode<KIND>(a, it);
+    for (int64_t it = first; ok && it < total; it += stride) {
+      const Tile t = decode<KIND, CG>(a, it, rank);
       float held[PLANES > 1 ? 64 : 1];  // sums of the finished accumulations (bn <= 128: 64 columns at most)
       if (PLANES > 1) {
 #pragma unroll
         for (int i = 0; i < 64; ++i) held[i] = 0.f;
         for (int kb = 0; kb < t.kb; kb += kChunk, sums.step(2)) {
           const int buf = sums.i;
-          ok = mbar_wait_warp(&bars.accfull[buf], sums.phase, abort);
+          ok = wait_phase_warp(&bars.accfull[buf], sums.phase, abort);
           if (!ok) break;
           tmem_fence_after();
           const uint32_t acc = tmem + buf * 2 * a.bn + c_lo + ((uint32_t)((w & 3) * 32) << 16);
@@ -483,10 +545,10 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
             }
           tmem_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.accempty[buf]);
+          if (lane == 0) arrive_leader<CG>(&bars.accempty[buf]);
         }
       } else if (t.kb > 0) {
-        ok = mbar_wait_warp(&bars.accfull[sums.i], sums.phase, abort);
+        ok = wait_phase_warp(&bars.accfull[sums.i], sums.phase, abort);
         tmem_fence_after();
       }
       if (!ok) {
@@ -548,7 +610,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
           if (c + 32 == c_hi) {  // the accumulator is in registers: free it for the tile after next
             tmem_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.accempty[buf]);
+            if (lane == 0) arrive_leader<CG>(&bars.accempty[buf]);
           }
         } else {
 #pragma unroll
@@ -631,21 +693,21 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
     // The next tile's place and rows are fetched while this tile's stages are
     // in flight: each of these loads waits for the one before.
     Tile t{};
-    if (blockIdx.x < total) t = decode<KIND>(a, blockIdx.x);
+    if (first < total) t = decode<KIND, CG>(a, first, rank);
     int next[kR];
     auto first_rows = [&](const Tile& u) {
 #pragma unroll
       for (int i = 0; i < kR; ++i) {
         const int r = r0 + 16 * i;
-        if (u.kb > 0) next[i] = __ldg(a.order + u.pos + (r < u.rows ? r : 0));
+        next[i] = u.kb > 0 && r < u.rows ? __ldg(a.order + u.pos + r) : 0;
       }
     };
     first_rows(t);
-    for (int64_t it = blockIdx.x; ok && it < total; it += gridDim.x) {
-      const int64_t ahead = it + gridDim.x < total ? it + gridDim.x : it;
+    for (int64_t it = first; ok && it < total; it += stride) {
+      const int64_t ahead = it + stride < total ? it + stride : it;
       Tile u = t;
       if (t.kb == 0) {
-        t = decode<KIND>(a, ahead);
+        t = decode<KIND, CG>(a, ahead, rank);
         first_rows(t);
         continue;
       }
@@ -656,23 +718,23 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
       }
       for (int kb = 0; kb < t.kb; ++kb, ring.step(a.stages)) {
         const bool last = kb == t.kb - 1;
-        const int s = ring.i;
+        const int s = ring.i, nb = t.n0 + rank * bcols;
         if (KIND == kWeights) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             src[i] = a.src_a + ((int64_t)(next[i] / a.div_a) * a.ld_a + q * 8 + t.m0) * 2;
-            src[4 + i] = a.src_b + ((int64_t)(next[i] / a.div_b) * a.ld_b + q * 8 + t.n0) * 2;
+            src[4 + i] = a.src_b + ((int64_t)(next[i] / a.div_b) * a.ld_b + q * 8 + nb) * 2;
             if (!last) next[i] = __ldg(a.order + t.pos + min((kb + 1) * kBlockK + r0 + 16 * i, t.rows - 1));
           }
         }
-        ok = mbar_wait_warp(&bars.empty[s], ring.phase ^ 1, abort);
+        ok = wait_phase_warp(&bars.empty[s], ring.phase ^ 1, abort);
         if (!ok) break;
         const uint32_t sa = smem_u32(sm) + s * stage_bytes + at;
         if (KIND == kRows) {
           const bool live = kb * kBlockK + q * 8 < a.k;
           const int64_t k0 = live ? (int64_t)kb * (kBlockK * 2) : 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) copy16(sa + 2048 * i, src[i] + k0, live);
+          for (int i = 0; i < 8; ++i) copy16(sa + 2048 * i, src[i] + k0, live && r0 + 16 * i < t.rows);
         } else {
           const uint32_t sb = sa + kABytes;
           const int left = t.rows - kb * kBlockK - r0;  // rows r0 + 16 i < left are the segment's
@@ -686,9 +748,9 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
             }
           }
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            if (g >= a.bn / 64) break;
-            const bool in = t.n0 + g * 64 + q * 8 < a.n;
+          for (int g = 0; g < 4 / CG; ++g) {
+            if (g >= bcols / 64) break;
+            const bool in = nb + g * 64 + q * 8 < a.n;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const bool live = in && 16 * i < left;
@@ -697,7 +759,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
           }
         }
         copies_arrive(&bars.full[s]);
-        if (kb == 0) u = decode<KIND>(a, ahead);
+        if (kb == 0) u = decode<KIND, CG>(a, ahead, rank);
         if (last) first_rows(u);
       }
       t = u;
@@ -707,8 +769,12 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES>::kThreads, 1)
   }
   __syncwarp();
   tmem_fence_before();
-  __syncthreads();
-  if (warp == 2) tmem_dealloc(tmem, tmem_cols);
+  block_or_pair_sync<CG>();
+  if (warp == 2) tmem_give<CG>(tmem, tmem_cols);
+  if (CG > 1) {  // the other block's shared and tensor memory stay until both are done
+    __syncwarp();
+    cluster_sync();
+  }
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -734,13 +800,32 @@ int encode(CUtensorMap* map, const void* base, int fp16, int rank, const cuuint6
   return GMMXX_OK;
 }
 
-template <int KIND, int PLANES>
+template <int KIND, int PLANES, int CG>
 int launch_one(const ProductMaps& maps, const ProductArgs& a, unsigned grid, cudaStream_t st) {
-  const int smem = a.stages * PLANES * (kABytes + a.bn * 128) + kEpiWarps * kStageEpi + 1024;
+  using R = Roles<KIND, PLANES, CG>;
+  const int smem = a.stages * PLANES * (kABytes + a.bn / CG * 128) + kEpiWarps * kStageEpi + 1024;
+  const auto kern = product_kernel<KIND, PLANES, CG>;
   static SmemGrants grants;
-  if (int rc = allow_smem((const void*)product_kernel<KIND, PLANES>, kSmemLimit - 1024, grants)) return rc;
-  product_kernel<KIND, PLANES><<<grid, Roles<KIND, PLANES>::kThreads, smem, st>>>(maps, a);
-  return check_launch("product_kernel");
+  if (int rc = allow_smem((const void*)kern, kSmemLimit - 1024, grants)) return rc;
+  if (CG == 1) {
+    kern<<<grid, R::kThreads, smem, st>>>(maps, a);
+    return check_launch("product_kernel");
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(R::kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, maps, a);
+  if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "product_kernel launch: %s", cudaGetErrorString(e));
+  return GMMXX_OK;
 }
 
 }  // namespace
@@ -754,8 +839,8 @@ int encode_stack(CUtensorMap* map, const void* base, int fp16, int64_t cols, int
   return encode(map, base, fp16, 3, dims, strides, box);
 }
 
-int product_stages(int planes, int bn) {
-  return std::min(kMaxStages, (kSmemLimit - 2048 - kEpiWarps * kStageEpi) / (planes * (kABytes + bn * 128)));
+int product_stages(int planes, int bn, int pair) {
+  return std::min(kMaxStages, (kSmemLimit - 2048 - kEpiWarps * kStageEpi) / (planes * (kABytes + bn / pair * 128)));
 }
 
 int device_sms(int* sms) {
@@ -769,15 +854,22 @@ int device_sms(int* sms) {
   return GMMXX_OK;
 }
 
-int launch_product(Kind kind, int planes, const ProductMaps& maps, const ProductArgs& a, int64_t max_items,
+int launch_product(Kind kind, int planes, int pair, const ProductMaps& maps, const ProductArgs& a, int64_t max_items,
                    cudaStream_t st) {
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
-  const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(sms, max_items * a.mt * a.nt));
-  if (kind == kRows) return planes == 1 ? launch_one<kRows, 1>(maps, a, grid, st) : launch_one<kRows, 3>(maps, a, grid, st);
+  const int64_t tiles = std::max<int64_t>(1, max_items * a.mt * a.nt);
+  const unsigned grid = (unsigned)(std::min<int64_t>(sms / pair, tiles) * pair);
+  if (pair == 2) {
+    if (kind == kRows) return launch_one<kRows, 1, 2>(maps, a, grid, st);
+    if (kind == kWeights) return launch_one<kWeights, 1, 2>(maps, a, grid, st);
+    return launch_one<kBatch, 1, 2>(maps, a, grid, st);
+  }
+  if (kind == kRows)
+    return planes == 1 ? launch_one<kRows, 1, 1>(maps, a, grid, st) : launch_one<kRows, 3, 1>(maps, a, grid, st);
   if (kind == kWeights)
-    return planes == 1 ? launch_one<kWeights, 1>(maps, a, grid, st) : launch_one<kWeights, 3>(maps, a, grid, st);
-  return planes == 1 ? launch_one<kBatch, 1>(maps, a, grid, st) : launch_one<kBatch, 2>(maps, a, grid, st);
+    return planes == 1 ? launch_one<kWeights, 1, 1>(maps, a, grid, st) : launch_one<kWeights, 3, 1>(maps, a, grid, st);
+  return planes == 1 ? launch_one<kBatch, 1, 1>(maps, a, grid, st) : launch_one<kBatch, 2, 1>(maps, a, grid, st);
 }
 
 int take_flag(const void* symbol, int* flag, cudaStream_t st) {

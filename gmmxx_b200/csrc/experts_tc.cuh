@@ -3,6 +3,7 @@
 #pragma once
 
 #include "experts_api.cuh"
+#include "tc_ptx.cuh"
 
 #include <cuda.h>
 
@@ -32,6 +33,7 @@ struct ProductArgs {
   const int32_t* order;
   const char *src_a, *src_b;  // 16-bit rows fetched by cp.async (one plane): 16-byte aligned,
   int64_t ld_a, ld_b;         // rows of ld elements (a multiple of 8)
+  const int32_t* count;  // number of entries of the table (device)
   const int32_t* table;  // kRows: tiles; kWeights: segments
   int div_a, div_b;      // gathered row = order[position] / div
   int groups;
@@ -55,6 +57,43 @@ struct ProductMaps {
   CUtensorMap a[3], b[3];
 };
 
+#ifdef __CUDACC__
+// Bounded waits of the product kernels: until the phase, the block's abort flag
+// (may be null), or about two seconds of SM cycles.
+// The barriers' scope is left at its default (the block): the data they
+// guard is shared memory of the block that waits, or is read and written by the
+// tensor core and TMA, whose order the proxy fences and commits give.  Cluster
+// scope costs a wait for all the thread's memory accesses: ~1300 cycles for an
+// arrival, more than a stage's products.
+constexpr long long kWaitCycles = 4000000000ll;
+__device__ __forceinline__ bool try_phase(uint32_t b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(b), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait_phase(uint64_t* b, uint32_t parity, volatile int* abort) {
+  const uint32_t a = ptx::smem_u32(b);
+  if (try_phase(a, parity)) return true;
+  const long long t0 = clock64();
+  for (uint32_t i = 1;; ++i) {
+    if (try_phase(a, parity)) return true;
+    if ((i & 31) == 0) {
+      if (abort != nullptr && *abort) return false;
+      if (clock64() - t0 > kWaitCycles) return false;
+    }
+  }
+}
+// by a whole warp, the result uniform
+__device__ __forceinline__ bool wait_phase_warp(uint64_t* b, uint32_t parity, volatile int* abort) {
+  const bool ok = wait_phase(b, parity, abort);
+  return __all_sync(0xffffffffu, ok) != 0;
+}
+#endif
+
 // segments of the matrices' gradient (device table): [0] their number, then
 // per segment {group, first position, rows, partial slot or -1}
 constexpr int kSegHeader = 4;
@@ -63,13 +102,14 @@ constexpr int kSegInts = 4;
 int encode_stack(CUtensorMap* map, const void* base, int fp16, int64_t cols, int64_t rows, int64_t ld, int64_t stack,
                  int64_t stride, int box_rows);
 // instruction descriptor of kind::f16 with M = 128, N = bn, fp32 sums; types 0 = fp16, 1 = bf16 for both operands
-__host__ __device__ inline uint32_t product_idesc(int fp16, int bn, int a_mn, int b_mn) {
+// (M = 256 for a pair of blocks)
+__host__ __device__ inline uint32_t product_idesc(int fp16, int bn, int a_mn, int b_mn, int pair = 1) {
   const uint32_t type = fp16 ? 0u : 1u;
   return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-         ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+         ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(128 * pair >> 4) << 24);
 }
-int product_stages(int planes, int bn);
-int launch_product(Kind kind, int planes, const ProductMaps& maps, const ProductArgs& a, int64_t max_items,
+int product_stages(int planes, int bn, int pair);
+int launch_product(Kind kind, int planes, int pair, const ProductMaps& maps, const ProductArgs& a, int64_t max_items,
                    cudaStream_t st);
 int device_sms(int* sms);
 // sticky flags of bounded waits that ran out: read on the stream, synchronise, clear

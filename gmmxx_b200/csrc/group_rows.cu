@@ -10,7 +10,7 @@
 // nothing depends on the order in which warps run, so the result is the same
 // in every run.
 //
-// Small problems (kSmallSlots slots and a [32][K + 1] table in shared memory)
+// Small problems (kSmallSlots slots and a [35][K + 1] table in shared memory)
 // run in a single block and launch; larger ones in four launches.
 #include "experts_api.cuh"
 
@@ -101,52 +101,68 @@ __device__ __forceinline__ int block_exclusive(int v, int* red, int* total) {
 // k, k == K the unassigned.  One block of 1024 threads; start[k] (may be the
 // caller's shared memory) and first[k] receive K + 1 values each.
 template <typename Size>
-__device__ __forceinline__ void scan_groups(int K, Size size, int* start, int* first, int32_t* offsets, int32_t* tiles,
-                                            int* red) {
-  int row0 = 0, tile0 = 0;
+__device__ __forceinline__ void scan_groups(int K, Size size, int* start, int* first, int* first2, int32_t* offsets,
+                                            int32_t* tiles, int* red) {
+  int row0 = 0, tile0 = 0, pair0 = 0;
   for (int k0 = 0; k0 <= K; k0 += 1024) {
     const int k = k0 + threadIdx.x;
     const int c = k <= K ? size(k) : 0;
     const int nt = (c + kTileRows - 1) / kTileRows;
-    int rows, ntiles;
+    int rows, ntiles, npairs;
     const int r = row0 + block_exclusive(c, red, &rows);
     const int t = tile0 + block_exclusive(nt, red, &ntiles);
+    const int p = pair0 + block_exclusive((c + kPairRows - 1) / kPairRows, red, &npairs);
     if (k <= K) {
       start[k] = r;
       first[k] = t;
+      first2[k] = p;
       offsets[k] = r;  // offsets[K]: end of the last group, start of the unassigned slots
     }
     row0 += rows;
     tile0 += ntiles;
+    pair0 += npairs;
   }
-  if (threadIdx.x == 0) tiles[0] = tile0;
+  if (threadIdx.x == 0) {
+    tiles[0] = tile0;
+    tiles[1] = pair0;
+  }
 }
 
-// tile table: tiles[0] their number, then per tile {group, first position,
-// rows}; the unassigned slots' tiles have group K and come last
-__device__ __forceinline__ void fill_tiles(int K, const int* first, const int* start, int slots, int32_t* tiles,
-                                           int64_t t, int ntiles) {
-  int lo = 0, hi = K;  // last k with first[k] <= t and a tile of its own
+// Tile table: per tile of `per` rows {group, first position, rows}; the
+// unassigned slots' tiles have group K and come last.  Entry t of `table`:
+__device__ __forceinline__ void fill_tile(int K, const int* first, const int* start, int slots, int per, int32_t* table,
+                                          int64_t t) {
+  int lo = 0, hi = K;  // last k with first[k] <= t: the one whose tiles t falls in
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (first[mid] <= t) lo = mid; else hi = mid - 1;
   }
-  const int pos = start[lo] + (int)(t - first[lo]) * kTileRows;
+  const int pos = start[lo] + (int)(t - first[lo]) * per;
   const int end = lo < K ? start[lo + 1] : slots;
-  int32_t* e = tiles + kTileHeader + t * kTileInts;
+  int32_t* e = table + t * kTileInts;
   e[0] = lo;
   e[1] = pos;
-  e[2] = min(kTileRows, end - pos);
+  e[2] = min(per, end - pos);
+}
+
+// both tables, the tiles [begin, ...) in steps of `step`; pairs: offset of the second
+__device__ __forceinline__ void fill_tables(int K, const int* first, const int* first2, const int* start, int slots,
+                                            int32_t* tiles, int64_t pairs, int64_t begin, int64_t step) {
+  const int n1 = tiles[0], n2 = tiles[1];
+  for (int64_t t = begin; t < n1; t += step) fill_tile(K, first, start, slots, kTileRows, tiles + kTileHeader, t);
+  for (int64_t t = begin; t < n2; t += step) fill_tile(K, first2, start, slots, kPairRows, tiles + kTileHeader + pairs, t);
 }
 
 __global__ void __launch_bounds__(1024) group_rows_small_kernel(const void* labels, int wide, int slots, int K,
-                                                                int32_t* order, int32_t* offsets, int32_t* tiles) {
+                                                                int32_t* order, int32_t* offsets, int32_t* tiles,
+                                                                int64_t pairs) {
   extern __shared__ int sm[];
   __shared__ int red[32];
   const int K1 = K + 1, warp = threadIdx.x >> 5;
   int* table = sm;                // [kWarps][K1]
   int* start = sm + kWarps * K1;  // [K1]
   int* first = start + K1;        // [K1]
+  int* first2 = first + K1;       // [K1]
   for (int i = threadIdx.x; i < kWarps * K1; i += 1024) table[i] = 0;
   __syncthreads();
   // whole 128-slot steps per warp
@@ -164,13 +180,12 @@ __global__ void __launch_bounds__(1024) group_rows_small_kernel(const void* labe
     first[k] = run;
   }
   __syncthreads();
-  scan_groups(K, [&](int k) { return first[k]; }, start, first, offsets, tiles, red);
+  scan_groups(K, [&](int k) { return first[k]; }, start, first, first2, offsets, tiles, red);
   __syncthreads();
   for (int i = threadIdx.x; i < kWarps * K1; i += 1024) table[i] += start[i % K1];
   __syncthreads();
   walk<false>(labels, wide, begin, end, K, table + warp * K1, order);
-  const int ntiles = tiles[0];
-  for (int t = threadIdx.x; t < ntiles; t += 1024) fill_tiles(K, first, start, slots, tiles, t, ntiles);
+  fill_tables(K, first, first2, start, slots, tiles, pairs, threadIdx.x, 1024);
 }
 
 // rows of the table: warp w of the grid counts slots [w * chunk, (w + 1) * chunk)
@@ -214,13 +229,14 @@ __global__ void __launch_bounds__(1024) columns_kernel(int* table, int nwarps, i
 }
 
 __global__ void __launch_bounds__(1024) totals_kernel(const int* total, int K, int* start, int* first,
-                                                      int32_t* offsets, int32_t* tiles) {
+                                                      int* first2, int32_t* offsets, int32_t* tiles) {
   __shared__ int red[32];
-  scan_groups(K, [&](int k) { return total[k]; }, start, first, offsets, tiles, red);
+  scan_groups(K, [&](int k) { return total[k]; }, start, first, first2, offsets, tiles, red);
 }
 
 __global__ void place_kernel(const void* labels, int wide, int64_t slots, int K, int64_t chunk, int nwarps,
-                             const int* table, const int* start, const int* first, int32_t* order, int32_t* tiles) {
+                             const int* table, const int* start, const int* first, const int* first2, int32_t* order,
+                             int32_t* tiles, int64_t pairs) {
   extern __shared__ int sm[];
   const int K1 = K + 1, warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
   const int rows = min(warps, nwarps - (int)blockIdx.x * warps);
@@ -230,9 +246,8 @@ __global__ void place_kernel(const void* labels, int wide, int64_t slots, int K,
   const int64_t w = (int64_t)blockIdx.x * warps + warp;
   const int64_t begin = min(slots, w * chunk), end = min(slots, begin + chunk);
   walk<false>(labels, wide, begin, end, K, sm + warp * K1, order);
-  const int ntiles = tiles[0];
-  for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < ntiles; t += (int64_t)gridDim.x * blockDim.x)
-    fill_tiles(K, first, start, (int)slots, tiles, t, ntiles);
+  fill_tables(K, first, first2, start, (int)slots, tiles, pairs, (int64_t)blockIdx.x * blockDim.x + threadIdx.x,
+              (int64_t)gridDim.x * blockDim.x);
 }
 
 struct Plan {
@@ -241,13 +256,13 @@ struct Plan {
   int warps, blocks;    // per block, grid
   int nwarps;           // rows of the table
   int64_t chunk;
-  int64_t table, total, start, first, bytes;  // workspace offsets (large path)
+  int64_t table, total, start, first, first2, bytes;  // workspace offsets (large path)
 };
 
 Plan make_plan(int64_t slots, int64_t K) {
   Plan p{};
   const int64_t K1 = K + 1;
-  const int64_t small = (kWarps + 2) * K1 * 4;
+  const int64_t small = (kWarps + 3) * K1 * 4;
   p.small = slots <= kSmallSlots && small <= kSmallSmem;
   if (p.small) {
     p.smem = (int)small;
@@ -265,6 +280,7 @@ Plan make_plan(int64_t slots, int64_t K) {
   p.total = off; off += round_up(K1 * 4, 256);
   p.start = off; off += round_up(K1 * 4, 256);
   p.first = off; off += round_up(K1 * 4, 256);
+  p.first2 = off; off += round_up(K1 * 4, 256);
   p.bytes = off;
   return p;
 }
@@ -272,7 +288,7 @@ Plan make_plan(int64_t slots, int64_t K) {
 }  // namespace
 
 int64_t tiles_len(int64_t slots, int64_t K) {
-  return kTileHeader + kTileInts * (slots / kTileRows + std::min<int64_t>(K + 1, slots));
+  return kTileHeader + kTileInts * (most_tiles(slots, K, kTileRows) + most_tiles(slots, K, kPairRows));
 }
 
 size_t group_rows_ws(int64_t slots, int64_t K) { return (size_t)make_plan(slots, K).bytes; }
@@ -280,16 +296,18 @@ size_t group_rows_ws(int64_t slots, int64_t K) { return (size_t)make_plan(slots,
 int launch_group_rows(const void* labels, int wide, int64_t slots, int64_t K, int32_t* order, int32_t* offsets,
                       int32_t* tiles, char* ws, cudaStream_t st) {
   const Plan p = make_plan(slots, K);
+  const int64_t pairs = kTileInts * most_tiles(slots, K, kTileRows);
   if (p.small) {
     static SmemGrants grants;
     if (int rc = allow_smem((const void*)group_rows_small_kernel, kSmallSmem, grants)) return rc;
-    group_rows_small_kernel<<<1, 1024, p.smem, st>>>(labels, wide, (int)slots, (int)K, order, offsets, tiles);
+    group_rows_small_kernel<<<1, 1024, p.smem, st>>>(labels, wide, (int)slots, (int)K, order, offsets, tiles, pairs);
     return check_launch("group_rows_small_kernel");
   }
   int* table = reinterpret_cast<int*>(ws + p.table);
   int* total = reinterpret_cast<int*>(ws + p.total);
   int* start = reinterpret_cast<int*>(ws + p.start);
   int* first = reinterpret_cast<int*>(ws + p.first);
+  int* first2 = reinterpret_cast<int*>(ws + p.first2);
   static SmemGrants count_grants, place_grants;
   if (int rc = allow_smem((const void*)count_kernel, kTableSmem, count_grants)) return rc;
   if (int rc = allow_smem((const void*)place_kernel, kTableSmem, place_grants)) return rc;
@@ -297,10 +315,10 @@ int launch_group_rows(const void* labels, int wide, int64_t slots, int64_t K, in
   if (int rc = check_launch("count_kernel")) return rc;
   columns_kernel<<<(unsigned)ceil_div(K + 1, 32), 1024, 0, st>>>(table, p.nwarps, (int)K + 1, total);
   if (int rc = check_launch("columns_kernel")) return rc;
-  totals_kernel<<<1, 1024, 0, st>>>(total, (int)K, start, first, offsets, tiles);
+  totals_kernel<<<1, 1024, 0, st>>>(total, (int)K, start, first, first2, offsets, tiles);
   if (int rc = check_launch("totals_kernel")) return rc;
   place_kernel<<<p.blocks, p.warps * 32, p.smem, st>>>(labels, wide, slots, (int)K, p.chunk, p.nwarps, table, start,
-                                                       first, order, tiles);
+                                                       first, first2, order, tiles, pairs);
   return check_launch("place_kernel");
 }
 

@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kOrthThreads) orth_small_kernel(const OrthArgs
         }
         mma_commit(&bar);
       }
-      ok = mbar_wait(&bar, phase, nullptr);
+      ok = wait_phase(&bar, phase, nullptr);
       phase ^= 1;
       tmem_fence_after();
       if (active)
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kOrthThreads) orth_small_kernel(const OrthArgs
         }
         mma_commit(&bar);
       }
-      ok = mbar_wait(&bar, phase, nullptr);
+      ok = wait_phase(&bar, phase, nullptr);
       phase ^= 1;
       tmem_fence_after();
       if (active)
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kOrthThreads) orth_small_kernel(const OrthArgs
           }
           mma_commit(&bar);
         }
-        ok = mbar_wait(&bar, phase, nullptr);
+        ok = wait_phase(&bar, phase, nullptr);
         phase ^= 1;
         tmem_fence_after();
         if (active)
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kOrthThreads) orth_small_kernel(const OrthArgs
     }
   }
   if (!ok) {  // a product may still be running: wait for it once more, then report
-    mbar_wait(&bar, phase ^ 1, nullptr);
+    wait_phase(&bar, phase ^ 1, nullptr);
     if (tid == 0) atomicOr(&g_orth_status, 1);
   }
   tmem_fence_before();

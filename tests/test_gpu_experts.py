@@ -102,15 +102,18 @@ def _check_groups(labels, k, groups):
     counts = torch.bincount(key, minlength=k + 1)
     offsets = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)[:k]])
     assert torch.equal(groups.offsets.cpu().long(), offsets)
-    # the tile table covers every position once, in order, within the groups
+    # the tile tables cover every position once, in order, within the groups
     t = groups.tiles.cpu().long()
-    rows = t[4:4 + 3 * int(t[0])].reshape(-1, 3)
-    assert torch.equal(rows[:, 1], torch.cat([torch.zeros(1, dtype=torch.int64), rows[:, 2].cumsum(0)])[:-1])
-    assert int(rows[:, 2].sum()) == flat.numel()
-    if flat.numel():
-        assert torch.equal(key[want][rows[:, 1]], rows[:, 0])
-        assert torch.equal(key[want][rows[:, 1] + rows[:, 2] - 1], rows[:, 0])
-        assert int(rows[:, 2].min()) >= 1 and int(rows[:, 2].max()) <= 128
+    at = 4
+    for i, per in enumerate((128, 256)):
+        rows = t[at:at + 3 * int(t[i])].reshape(-1, 3)
+        assert torch.equal(rows[:, 1], torch.cat([torch.zeros(1, dtype=torch.int64), rows[:, 2].cumsum(0)])[:-1])
+        assert int(rows[:, 2].sum()) == flat.numel()
+        if flat.numel():
+            assert torch.equal(key[want][rows[:, 1]], rows[:, 0])
+            assert torch.equal(key[want][rows[:, 1] + rows[:, 2] - 1], rows[:, 0])
+            assert int(rows[:, 2].min()) >= 1 and int(rows[:, 2].max()) <= per
+        at += 3 * (flat.numel() // per + min(k + 1, flat.numel()))
 
 
 @pytest.mark.parametrize("n,top,k", [(1, 1, 1), (31, 1, 3), (129, 2, 16), (4097, 8, 64), (32768, 1, 1500),
@@ -183,6 +186,30 @@ def test_products_and_gradients(cuda_device, n, top, k, n_in, n_out, kind, dtype
     if kind in ("dropped", "none"):
         lost = ((labels < 0) | (labels >= k)).cpu()
         assert not y.cpu()[lost].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,top,k,n_in,n_out,kind", [(6000, 1, 5, 136, 1000, "skewed"), (5000, 2, 3, 264, 776, "dropped"),
+                                                     (20000, 1, 4, 520, 300, "even")])
+def test_pairs_of_blocks(cuda_device, n, top, k, n_in, n_out, kind, dtype):
+    """Sizes whose products run on pairs of blocks: ragged last tiles, columns
+    and contractions that are no multiple of anything."""
+    import gmmxx_b200 as gm
+
+    labels, x, w, b, gy = _case(cuda_device, n, top, k, n_in, n_out, dtype, kind)
+    groups = gm.group_rows(labels, k)
+    y = gm.grouped_matmul(x, w, groups, bias=b)
+    wt = w.transpose(1, 2).contiguous().transpose(1, 2)
+    gx, gw, gb = gm.grouped_matmul_backward(gy, x, w, groups, bias=True)
+    hx, hw, _ = gm.grouped_matmul_backward(gy, x, wt, groups)
+    ref, mag = _reference(x, w, b, labels.cpu(), gy)
+    most = int((groups.offsets[1:] - groups.offsets[:-1]).max())
+    _close(y.reshape(n, top, n_out), ref["y"], mag["y"], n_in + 1, dtype)
+    _close(gm.grouped_matmul(x, wt, groups, bias=b).reshape(n, top, n_out), ref["y"], mag["y"], n_in + 1, dtype)
+    for got in ((gx, gw), (hx, hw)):
+        _close(got[0], ref["gx"], mag["gx"], n_out + top, dtype)
+        _close(got[1], ref["gw"], mag["gw"], most, dtype)
+    _close(gb, ref["gb"], mag["gb"], most, dtype)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -341,6 +368,7 @@ def _ns_check(q, g, steps=5, coef=(3.4445, -4.7750, 2.0315), eps=1e-7):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(1, 1, 1), (3, 1, 9), (2, 5, 3), (4, 64, 64), (3, 33, 100), (2, 130, 64),
                                    (1, 128, 128), (2, 129, 200), (1, 300, 257), (2, 256, 520), (1, 520, 256),
+                                   (24, 520, 776), (20, 1000, 536), (3, 60, 500), (2, 90, 250), (2, 250, 100),
                                    (260, 16, 16), (2, 3, 24, 40)])
 def test_orthogonalize(cuda_device, shape, dtype):
     import gmmxx_b200 as gm
