@@ -143,6 +143,15 @@ __device__ __forceinline__ void block_or_pair_sync() {
   else cluster_sync();
 }
 
+// One thread of a converged warp, always the same.  The warp's values stay
+// uniform around it, which the tensor core's instructions take their operands
+// from; under `lane == 0` each of them cost ~70 cycles more.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
+
 // a bounded wait ran out: every warp of the block stops at its next wait
 __device__ __forceinline__ void give_up(Bars* bars, int lane) {
   if (lane == 0) {
@@ -279,7 +288,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
   extern __shared__ __align__(1024) char smem_raw[];
   __shared__ Bars bars;
   char* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = CG == 1 ? 0 : (int)cluster_rank();
   const int bcols = a.bn / CG;     // columns of B that this block loads
   const int bbytes = bcols * 128;  // one plane of B per stage
@@ -361,8 +370,8 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
       for (int64_t f = oldest; f < filled; ++f) wait_phase_warp(&bars.full[f % a.stages], (uint32_t)((f / a.stages) & 1), nullptr);
     }
   } else if (PLANES == 1 && warp == 1) {
-    // ---- products of one plane: one thread (of the leading block) ----
-    if (lane == 0 && rank == 0) {
+    // ---- products of one plane (the leading block's) ----
+    if (rank == 0) {
       Ring ring, sums;
       int64_t use = 0;
       bool ok = true, peeked = false;  // peeked: the stage at `ring` is known to be there
@@ -381,13 +390,13 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
           t = decode<KIND, CG>(a, ahead, rank);
           continue;
         }
-        ok = wait_phase(&bars.accempty[sums.i], sums.phase ^ 1, abort);
+        ok = wait_phase_warp(&bars.accempty[sums.i], sums.phase ^ 1, abort);
         if (!ok) break;
         tmem_fence_after();
         const uint32_t d = tmem + sums.i * a.bn;
         Tile u = t;
         for (int kb = 0; kb < t.kb; ++kb, ++use) {
-          if (!peeked) ok = wait_phase(&there[ring.i], ring.phase, abort);
+          if (!peeked) ok = wait_phase_warp(&there[ring.i], ring.phase, abort);
           if (!ok) break;
           tmem_fence_after();
           const uint64_t da = desc_a + (uint32_t)ring.i * stage_units, db = desc_b + (uint32_t)ring.i * stage_units;
@@ -395,30 +404,38 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
           const bool last = kb == t.kb - 1;
           const int steps = KIND == kWeights && last ? min(4, (t.rows - kb * kBlockK + 15) >> 4) : 4;
           ring.step(a.stages);
+          peeked = false;
           if (steps == 4) {
-            mma_16<CG>(d, da, db, idesc, kb != 0);
-            mma_16<CG>(d, da + step_a, db + step_b, idesc, 1);
+            if (elect_one()) {
+              mma_16<CG>(d, da, db, idesc, kb != 0);
+              mma_16<CG>(d, da + step_a, db + step_b, idesc, 1);
+            }
             // While these run: whether the next stage is there, or what comes after this tile.  The
             // tensor core takes few products ahead, so what stands between two stages' products is idle time.
             if (last) u = decode<KIND, CG>(a, ahead, rank);
-            peeked = mbar_test(&there[ring.i], ring.phase);
-            mma_16<CG>(d, da + 2 * step_a, db + 2 * step_b, idesc, 1);
-            mma_16<CG>(d, da + 3 * step_a, db + 3 * step_b, idesc, 1);
+            peeked = __all_sync(0xffffffffu, mbar_test(&there[ring.i], ring.phase));
+            if (elect_one()) {
+              mma_16<CG>(d, da + 2 * step_a, db + 2 * step_b, idesc, 1);
+              mma_16<CG>(d, da + 3 * step_a, db + 3 * step_b, idesc, 1);
+              commit<CG>(done);
+              if (last) commit<CG>(&bars.accfull[sums.i]);
+            }
           } else {
-            for (int k = 0; k < steps; ++k) mma_16<CG>(d, da + k * step_a, db + k * step_b, idesc, (kb | k) != 0);
-            u = decode<KIND, CG>(a, ahead, rank);
-            peeked = false;
+            if (elect_one()) {
+              for (int k = 0; k < steps; ++k) mma_16<CG>(d, da + k * step_a, db + k * step_b, idesc, (kb | k) != 0);
+              commit<CG>(done);
+              if (last) commit<CG>(&bars.accfull[sums.i]);
+            }
+            if (last) u = decode<KIND, CG>(a, ahead, rank);
           }
-          commit<CG>(done);
-          if (last) commit<CG>(&bars.accfull[sums.i]);
         }
         sums.step(2);
         t = u;
       }
       if (!ok) {  // products in flight still read shared and write tensor memory
-        give_up(&bars, 0);
+        give_up(&bars, lane);
         const int64_t oldest = use > a.stages ? use - a.stages : 0;
-        for (int64_t f = oldest; f < use; ++f) wait_phase(&bars.empty[f % a.stages], (uint32_t)((f / a.stages) & 1), nullptr);
+        for (int64_t f = oldest; f < use; ++f) wait_phase_warp(&bars.empty[f % a.stages], (uint32_t)((f / a.stages) & 1), nullptr);
       }
     }
   } else if (R::kRelay && warp == 3) {
@@ -486,8 +503,8 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
             }
           }
         }
-        if (lane == 0) {
-          tmem_fence_after();
+        tmem_fence_after();
+        if (elect_one()) {
           constexpr int kPairs = PLANES == 1 ? 1 : PLANES == 2 ? 3 : 6;
 #pragma unroll
           for (int c = 0; c < kPairs; ++c) {
