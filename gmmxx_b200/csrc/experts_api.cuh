@@ -13,7 +13,7 @@ constexpr int kTileRows = 128;   // rows of one tile: the M extent of a tcgen05 
 constexpr int kPairRows = 256;   // and of a pair of blocks' tile
 constexpr int kTileHeader = 4;   // tiles[0]: number of 128-row tiles, tiles[1]: of 256-row tiles
 constexpr int kTileInts = 3;     // per tile: group, first position in the sorted order, rows
-constexpr int64_t kMaxGroups = 32768;
+constexpr int64_t kMaxGroups = 16384;  // three scans of them fit a block's shared memory (group_rows.cu)
 
 // the routed rows of one call
 struct Groups {

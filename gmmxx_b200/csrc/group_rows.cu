@@ -1,18 +1,32 @@
 // group_rows.cu -- routing: slots sorted by the component they are assigned to
-// (gmmxx_group_rows), and the table of row tiles that the grouped products walk.
+// (gmmxx_group_rows), and the tables of row tiles that the grouped products walk.
 //
-// A stable counting sort.  The slots are cut into one contiguous chunk per
-// warp; every warp counts its chunk's labels into its own row of a
-// [warps][K + 1] table (column K: unassigned slots), the columns are scanned
-// over the warps and the totals over the components, and every warp walks its
-// chunk again and places each slot at (group start) + (earlier warps' slots of
-// that label) + (rank inside the warp).  Equal labels keep their slot order and
-// nothing depends on the order in which warps run, so the result is the same
-// in every run.
+// A stable counting sort in one launch.  The slots are cut into one contiguous
+// chunk per warp.  Every warp counts its chunk's labels in shared memory (column
+// K: unassigned slots); the warps' counts become their exclusive prefixes within
+// the block, the blocks' totals go to a [blocks][K + 1] table; after a barrier
+// every block knows what comes before it and how many slots each component has;
+// every warp walks its chunk again and places each slot at (group start) +
+// (earlier blocks') + (earlier warps') + (its rank in the warp).  Equal labels
+// keep their slot order and nothing depends on the order in which warps run, so
+// the result is the same in every run.
 //
-// Small problems (kSmallSlots slots and a [35][K + 1] table in shared memory)
-// run in a single block and launch; larger ones in four launches.
+// The barrier is none for one block, a cluster's for up to 8 blocks, and for
+// more a counter in the workspace of a cooperative launch (bounded waits).  With
+// a small table every block sums the rows it needs; a large one (blocks x
+// components) is scanned by columns, one block a share of the columns, between
+// two barriers.
+//
+// A rank in a warp takes a match over the warp only where a label occurs twice:
+// each lane reads its label's counter and then adds to it, and if every lane's
+// addition found what it had read, no label is there twice.
+//
+// Bound by latency up to ~10^5 slots (launch, two walks, a barrier), above by
+// the scattered 4-byte stores of `order` and the walks' occupancy: counters of
+// 8192 components are held in 16 bits (a block's chunk is below 2^16 slots), 12
+// warps per SM instead of 6.
 #include "experts_api.cuh"
+#include "experts_tc.cuh"
 
 #include <algorithm>
 
@@ -20,14 +34,31 @@ namespace gmmxx {
 namespace experts {
 namespace {
 
-constexpr int kWarps = 32;                       // warps of the one-block kernel
-constexpr int64_t kSmallSlots = 32768;           // above, four launches over the whole GPU are faster
-constexpr int kSmallSmem = 200 * 1024;
-constexpr int64_t kChunk = 1024;                 // slots per warp of the large path, at least
-constexpr int64_t kMaxWarps = 148 * 32;
-constexpr int kTableSmem = 200 * 1024;       // counters of one block's warps
+constexpr int kMaxSmem = 216 * 1024;
+constexpr int kMaxWarps = 32;
+constexpr int kDirectTable = 32768;  // table entries up to which every block reads the rows it needs itself
 
-__device__ __forceinline__ int load_label(const void* labels, int wide, int64_t i, int K) {
+static __device__ int g_route_status = 0;  // sticky: 1 when the bounded barrier ran out
+
+enum Sync { kOneBlock = 0, kCluster = 1, kGrid = 2 };
+
+struct RouteArgs {
+  const void* labels;
+  int wide;       // int64 labels
+  int slots, K;
+  int chunk;      // slots per warp, a multiple of 32
+  int* table;     // [blocks][K + 1]
+  int* total;     // [K + 1]
+  int* barrier;   // kGrid: zero at launch
+  int32_t* order;
+  int32_t* offsets;
+  int32_t* tiles;
+  int64_t pairs;  // offset of the second tile table
+  int keep;       // the scans of rows and tiles have shared memory of their own
+  int direct;     // every block sums the table's rows itself
+};
+
+__device__ __forceinline__ int load_label(const void* labels, int wide, int i, int K) {
   // clamped before the narrowing: a 64-bit label beyond 32 bits is unassigned too
   if (wide) {
     const long long v = static_cast<const long long*>(labels)[i];
@@ -37,289 +68,402 @@ __device__ __forceinline__ int load_label(const void* labels, int wide, int64_t 
   return (v < 0 || v >= K) ? K : v;
 }
 
-// Slots [begin, end) of one warp, four groups of 32 in flight.  COUNT: adds
-// each label to cnt.  Otherwise cnt holds the next free position per label and
-// the slots are placed.
-template <bool COUNT>
-__device__ __forceinline__ void walk(const void* labels, int wide, int64_t begin, int64_t end, int K, int* cnt,
-                                     int32_t* order) {
+// one warp's counters: 32 bits each, or (PACK) two of 16 bits per word
+template <bool PACK>
+struct Counters {
+  int* w;
+  static __host__ __device__ int words(int K1) { return PACK ? (K1 + 1) / 2 : K1; }
+  __device__ __forceinline__ int get(int k) const {
+    return PACK ? (w[k >> 1] >> ((k & 1) * 16)) & 0xffff : w[k];
+  }
+  __device__ __forceinline__ int add(int k) const {  // returns what was there
+    if (!PACK) return atomicAdd(&w[k], 1);
+    const int sh = (k & 1) * 16;
+    return (atomicAdd(&w[k >> 1], 1 << sh) >> sh) & 0xffff;
+  }
+};
+
+// Slots [begin, end) of one warp, 128 in flight and the next 128 behind them.
+// COUNT: counts them; otherwise places them behind base.
+template <bool PACK, bool COUNT>
+__device__ __forceinline__ void walk(const RouteArgs& a, int begin, int end, Counters<PACK> cnt, const int* base) {
   const int lane = threadIdx.x & 31;
+  int next[4];
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = (int64_t)i0 + u * 32 + lane;
+      next[u] = i < end ? load_label(a.labels, a.wide, (int)i, a.K) : -1;
+    }
+  };
+  fetch(begin);
   for (int64_t i0 = begin; i0 < end; i0 += 128) {
     int lab[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t i = i0 + u * 32 + lane;
-      lab[u] = i < end ? load_label(labels, wide, i, K) : -1;
-    }
+    for (int u = 0; u < 4; ++u) lab[u] = next[u];
+    if (i0 + 128 < end) fetch((int)(i0 + 128));
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
+      if (i0 + u * 32 >= end) break;
       if (COUNT) {
-        if (lab[u] >= 0) atomicAdd(&cnt[lab[u]], 1);
-      } else {
-        const unsigned same = __match_any_sync(0xffffffffu, lab[u]);
-        const int rank = __popc(same & ((1u << lane) - 1u));
-        int base = 0;
-        if (lab[u] >= 0) base = cnt[lab[u]];
-        __syncwarp();
-        if (lab[u] >= 0) {
-          order[base + rank] = (int32_t)(i0 + u * 32 + lane);
-          if (rank == 0) cnt[lab[u]] = base + __popc(same);
-        }
-        __syncwarp();
+        if (lab[u] >= 0) cnt.add(lab[u]);
+        continue;
       }
+      const int seen = lab[u] >= 0 ? cnt.get(lab[u]) : 0;
+      __syncwarp();
+      const int had = lab[u] >= 0 ? cnt.add(lab[u]) : 0;
+      int rank = 0;
+      if (__any_sync(0xffffffffu, had != seen)) {
+        const unsigned same = __match_any_sync(0xffffffffu, lab[u]);
+        rank = __popc(same & ((1u << lane) - 1u));
+      }
+      if (lab[u] >= 0) a.order[base[lab[u]] + seen + rank] = (int32_t)(i0 + u * 32 + lane);
+      __syncwarp();
     }
   }
 }
 
-// exclusive scan over the block of one value per thread (1024 threads); *total gets the sum
-__device__ __forceinline__ int block_exclusive(int v, int* red, int* total) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int s = v;
+// exclusive scans over the block of three values per thread; red: 3 x 32 ints
+struct Three {
+  int a, b, c;
+};
+__device__ __forceinline__ Three block_exclusive3(Three v, int* red, Three* total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  Three s = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int t = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += t;
-  }
-  __syncthreads();
-  if (lane == 31) red[w] = s;
-  __syncthreads();
-  if (w == 0) {
-    int t = red[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, t, o);
-      if (lane >= o) t += u;
+    const int x = __shfl_up_sync(0xffffffffu, s.a, o), y = __shfl_up_sync(0xffffffffu, s.b, o),
+              z = __shfl_up_sync(0xffffffffu, s.c, o);
+    if (lane >= o) {
+      s.a += x;
+      s.b += y;
+      s.c += z;
     }
-    red[lane] = t;
   }
   __syncthreads();
-  *total = red[31];
-  return s - v + (w ? red[w - 1] : 0);
+  if (lane == 31) {
+    red[w] = s.a;
+    red[32 + w] = s.b;
+    red[64 + w] = s.c;
+  }
+  __syncthreads();
+  Three before = {0, 0, 0}, all = {0, 0, 0};
+  for (int i = 0; i < nw; ++i) {
+    const int x = red[i], y = red[32 + i], z = red[64 + i];
+    if (i < w) {
+      before.a += x;
+      before.b += y;
+      before.c += z;
+    }
+    all.a += x;
+    all.b += y;
+    all.c += z;
+  }
+  *total = all;
+  return {before.a + s.a - v.a, before.b + s.b - v.b, before.c + s.c - v.c};
 }
 
-// Group starts and tile starts from the group sizes.  size(k): slots of group
-// k, k == K the unassigned.  One block of 1024 threads; start[k] (may be the
-// caller's shared memory) and first[k] receive K + 1 values each.
-template <typename Size>
-__device__ __forceinline__ void scan_groups(int K, Size size, int* start, int* first, int* first2, int32_t* offsets,
-                                            int32_t* tiles, int* red) {
-  int row0 = 0, tile0 = 0, pair0 = 0;
-  for (int k0 = 0; k0 <= K; k0 += 1024) {
+// Starts of the groups' rows, 128-row tiles and 256-row tiles from the sizes:
+// out(k, rows, tiles, pairs) for k = 0 .. K.  Returns the totals.
+template <typename Size, typename Out>
+__device__ __forceinline__ Three scan_groups(int K, int* red, Size size, Out out) {
+  Three at = {0, 0, 0};
+  for (int k0 = 0; k0 <= K; k0 += blockDim.x) {
     const int k = k0 + threadIdx.x;
     const int c = k <= K ? size(k) : 0;
-    const int nt = (c + kTileRows - 1) / kTileRows;
-    int rows, ntiles, npairs;
-    const int r = row0 + block_exclusive(c, red, &rows);
-    const int t = tile0 + block_exclusive(nt, red, &ntiles);
-    const int p = pair0 + block_exclusive((c + kPairRows - 1) / kPairRows, red, &npairs);
-    if (k <= K) {
-      start[k] = r;
-      first[k] = t;
-      first2[k] = p;
-      offsets[k] = r;  // offsets[K]: end of the last group, start of the unassigned slots
-    }
-    row0 += rows;
-    tile0 += ntiles;
-    pair0 += npairs;
+    Three all;
+    const Three v = block_exclusive3({c, (c + kTileRows - 1) / kTileRows, (c + kPairRows - 1) / kPairRows}, red, &all);
+    if (k <= K) out(k, at.a + v.a, at.b + v.b, at.c + v.c);
+    at.a += all.a;
+    at.b += all.b;
+    at.c += all.c;
   }
-  if (threadIdx.x == 0) {
-    tiles[0] = tile0;
-    tiles[1] = pair0;
-  }
+  return at;
 }
 
-// Tile table: per tile of `per` rows {group, first position, rows}; the
-// unassigned slots' tiles have group K and come last.  Entry t of `table`:
+// tile t of the tiles of `per` rows: {group, first position, rows}; the
+// unassigned slots' tiles have group K and come last
 __device__ __forceinline__ void fill_tile(int K, const int* first, const int* start, int slots, int per, int32_t* table,
-                                          int64_t t) {
+                                          int t) {
   int lo = 0, hi = K;  // last k with first[k] <= t: the one whose tiles t falls in
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (first[mid] <= t) lo = mid; else hi = mid - 1;
   }
-  const int pos = start[lo] + (int)(t - first[lo]) * per;
+  const int pos = start[lo] + (t - first[lo]) * per;
   const int end = lo < K ? start[lo + 1] : slots;
-  int32_t* e = table + t * kTileInts;
+  int32_t* e = table + (int64_t)t * kTileInts;
   e[0] = lo;
   e[1] = pos;
   e[2] = min(per, end - pos);
 }
 
-// both tables, the tiles [begin, ...) in steps of `step`; pairs: offset of the second
-__device__ __forceinline__ void fill_tables(int K, const int* first, const int* first2, const int* start, int slots,
-                                            int32_t* tiles, int64_t pairs, int64_t begin, int64_t step) {
-  const int n1 = tiles[0], n2 = tiles[1];
-  for (int64_t t = begin; t < n1; t += step) fill_tile(K, first, start, slots, kTileRows, tiles + kTileHeader, t);
-  for (int64_t t = begin; t < n2; t += step) fill_tile(K, first2, start, slots, kPairRows, tiles + kTileHeader + pairs, t);
-}
-
-__global__ void __launch_bounds__(1024) group_rows_small_kernel(const void* labels, int wide, int slots, int K,
-                                                                int32_t* order, int32_t* offsets, int32_t* tiles,
-                                                                int64_t pairs) {
-  extern __shared__ int sm[];
-  __shared__ int red[32];
-  const int K1 = K + 1, warp = threadIdx.x >> 5;
-  int* table = sm;                // [kWarps][K1]
-  int* start = sm + kWarps * K1;  // [K1]
-  int* first = start + K1;        // [K1]
-  int* first2 = first + K1;       // [K1]
-  for (int i = threadIdx.x; i < kWarps * K1; i += 1024) table[i] = 0;
-  __syncthreads();
-  // whole 128-slot steps per warp
-  const int chunk = ((slots + kWarps - 1) / kWarps + 127) / 128 * 128;
-  const int begin = min(slots, warp * chunk), end = min(slots, begin + chunk);
-  walk<true>(labels, wide, begin, end, K, table + warp * K1, nullptr);
-  __syncthreads();
-  for (int k = threadIdx.x; k < K1; k += 1024) {
-    int run = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      const int c = table[w * K1 + k];
-      table[w * K1 + k] = run;
-      run += c;
-    }
-    first[k] = run;
+// All blocks' writes before it are visible after it.  False when the bounded
+// wait ran out (kGrid).
+template <int SYNC>
+__device__ __forceinline__ bool barrier(const RouteArgs& a, int round) {
+  if (SYNC == kOneBlock) {
+    __syncthreads();
+    return true;
+  }
+  if (SYNC == kCluster) {
+    __syncthreads();
+    ptx::cluster_sync();
+    return true;
   }
   __syncthreads();
-  scan_groups(K, [&](int k) { return first[k]; }, start, first, first2, offsets, tiles, red);
-  __syncthreads();
-  for (int i = threadIdx.x; i < kWarps * K1; i += 1024) table[i] += start[i % K1];
-  __syncthreads();
-  walk<false>(labels, wide, begin, end, K, table + warp * K1, order);
-  fill_tables(K, first, first2, start, slots, tiles, pairs, threadIdx.x, 1024);
+  int ok = 1;
+  if (threadIdx.x == 0) {
+    __threadfence();
+    atomicAdd(a.barrier, 1);
+    const int want = (int)gridDim.x * round;
+    const long long t0 = clock64();
+    while (*(volatile int*)a.barrier < want) {
+      if (clock64() - t0 > kWaitCycles) {
+        ok = 0;
+        atomicOr(&g_route_status, 1);
+        break;
+      }
+    }
+    __threadfence();
+  }
+  return __syncthreads_and(ok) != 0;
 }
 
-// rows of the table: warp w of the grid counts slots [w * chunk, (w + 1) * chunk)
-__global__ void count_kernel(const void* labels, int wide, int64_t slots, int K, int64_t chunk, int nwarps,
-                             int* table) {
+template <int SYNC, bool PACK>
+__global__ void __launch_bounds__(kMaxWarps * 32, 1) route_kernel(const RouteArgs a) {
   extern __shared__ int sm[];
-  const int K1 = K + 1, warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < warps * K1; i += blockDim.x) sm[i] = 0;
+  __shared__ int red[96];
+  __shared__ int part[2][32][33];
+  const int K = a.K, K1 = K + 1, warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nblocks = SYNC == kOneBlock ? 1 : (int)gridDim.x, block = blockIdx.x;
+  const int words = Counters<PACK>::words(K1);
+  int* base = sm;                 // [K1] totals of the block, then where its slots of each label go
+  int* counters = sm + K1;        // [warps][words]
+  int* size = a.keep ? counters + warps * words : nullptr;  // [K1] slots per group ...
+  int* first = size + K1;         // ... and the scans of the tiles
+  int* first2 = first + K1;
+  for (int i = threadIdx.x; i < warps * words; i += blockDim.x) counters[i] = 0;
   __syncthreads();
-  const int64_t w = (int64_t)blockIdx.x * warps + warp;
-  const int64_t begin = min(slots, w * chunk), end = min(slots, begin + chunk);
-  walk<true>(labels, wide, begin, end, K, sm + warp * K1, nullptr);
+  const Counters<PACK> mine{counters + warp * words};
+  const int64_t from = ((int64_t)block * warps + warp) * a.chunk;
+  const int begin = (int)min((int64_t)a.slots, from), end = (int)min((int64_t)a.slots, from + a.chunk);
+  walk<PACK, true>(a, begin, end, mine, nullptr);
   __syncthreads();
-  const int rows = min(warps, nwarps - (int)blockIdx.x * warps);
-  int* out = table + (int64_t)blockIdx.x * warps * K1;
-  for (int i = threadIdx.x; i < rows * K1; i += blockDim.x) out[i] = sm[i];
-}
-
-// Columns of the table scanned over the warps: 32 columns per block, 32
-// segments of warps; total[k] gets the column sums.
-__global__ void __launch_bounds__(1024) columns_kernel(int* table, int nwarps, int K1, int* total) {
-  __shared__ int part[32][33];
-  const int lane = threadIdx.x & 31, seg = threadIdx.x >> 5;
-  const int k = blockIdx.x * 32 + lane;
-  const int per = (nwarps + 31) / 32, w0 = min(nwarps, seg * per), w1 = min(nwarps, w0 + per);
-  int sum = 0;
-  if (k < K1)
-    for (int w = w0; w < w1; ++w) sum += table[(int64_t)w * K1 + k];
-  part[seg][lane] = sum;
-  __syncthreads();
-  int run = 0;
-  for (int s = 0; s < seg; ++s) run += part[s][lane];
-  if (k < K1) {
-    if (seg == 31) total[k] = run + sum;
-    for (int w = w0; w < w1; ++w) {
-      const int c = table[(int64_t)w * K1 + k];
-      table[(int64_t)w * K1 + k] = run;
-      run += c;
+  // counts -> exclusive prefixes over the block's warps; the block's totals
+  for (int i = threadIdx.x; i < words; i += blockDim.x) {
+    if (PACK) {
+      int lo = 0, hi = 0;
+      for (int w = 0; w < warps; ++w) {
+        const int c = counters[w * words + i];
+        counters[w * words + i] = lo | (hi << 16);
+        lo += c & 0xffff;
+        hi += (c >> 16) & 0xffff;
+      }
+      base[2 * i] = lo;
+      if (2 * i + 1 < K1) base[2 * i + 1] = hi;
+    } else {
+      int run = 0;
+      for (int w = 0; w < warps; ++w) {
+        const int c = counters[w * words + i];
+        counters[w * words + i] = run;
+        run += c;
+      }
+      base[i] = run;
     }
   }
-}
-
-__global__ void __launch_bounds__(1024) totals_kernel(const int* total, int K, int* start, int* first,
-                                                      int* first2, int32_t* offsets, int32_t* tiles) {
-  __shared__ int red[32];
-  scan_groups(K, [&](int k) { return total[k]; }, start, first, first2, offsets, tiles, red);
-}
-
-__global__ void place_kernel(const void* labels, int wide, int64_t slots, int K, int64_t chunk, int nwarps,
-                             const int* table, const int* start, const int* first, const int* first2, int32_t* order,
-                             int32_t* tiles, int64_t pairs) {
-  extern __shared__ int sm[];
-  const int K1 = K + 1, warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
-  const int rows = min(warps, nwarps - (int)blockIdx.x * warps);
-  const int* in = table + (int64_t)blockIdx.x * warps * K1;
-  for (int i = threadIdx.x; i < rows * K1; i += blockDim.x) sm[i] = in[i] + start[i % K1];
   __syncthreads();
-  const int64_t w = (int64_t)blockIdx.x * warps + warp;
-  const int64_t begin = min(slots, w * chunk), end = min(slots, begin + chunk);
-  walk<false>(labels, wide, begin, end, K, sm + warp * K1, order);
-  fill_tables(K, first, first2, start, (int)slots, tiles, pairs, (int64_t)blockIdx.x * blockDim.x + threadIdx.x,
-              (int64_t)gridDim.x * blockDim.x);
+  const bool direct = a.direct != 0;
+  int* row = a.table + (int64_t)block * K1;
+  if (SYNC != kOneBlock) {
+    for (int k = threadIdx.x; k < K1; k += blockDim.x) row[k] = base[k];
+    if (!barrier<SYNC>(a, 1)) return;
+    // 32 columns at a time, the rows cut over the warps
+    const int per = (nblocks + warps - 1) / warps, b0 = min(nblocks, warp * per), b1 = min(nblocks, b0 + per);
+    for (int k0 = direct ? 0 : block * 32; k0 < K1; k0 += direct ? 32 : nblocks * 32) {
+      const int k = k0 + lane;
+      int all = 0, before = 0;
+      if (k < K1) {
+#pragma unroll 4
+        for (int b = b0; b < b1; ++b) {
+          const int c = __ldcg(a.table + (int64_t)b * K1 + k);
+          all += c;
+          before += b < block ? c : 0;
+        }
+      }
+      part[0][warp][lane] = all;
+      part[1][warp][lane] = before;
+      __syncthreads();
+      if (direct) {  // this block's start and the total of its columns
+        if (warp == 0 && k < K1) {
+          int t = 0, f = 0;
+          for (int w = 0; w < warps; ++w) {
+            t += part[0][w][lane];
+            f += part[1][w][lane];
+          }
+          base[k] = f;
+          size[k] = t;
+        }
+      } else {  // every block's start, in place
+        int run = 0;
+        for (int w = 0; w < warp; ++w) run += part[0][w][lane];
+        if (k < K1) {
+          if (warp == warps - 1) a.total[k] = run + all;
+          for (int b = b0; b < b1; ++b) {
+            int* p = a.table + (int64_t)b * K1 + k;
+            const int c = __ldcg(p);
+            *p = run;
+            run += c;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (!direct) {
+      if (!barrier<SYNC>(a, 2)) return;
+      for (int k = threadIdx.x; k < K1; k += blockDim.x) base[k] = __ldcg(row + k);
+    }
+  } else {
+    for (int k = threadIdx.x; k < K1; k += blockDim.x) {
+      if (direct) size[k] = base[k];
+      else a.total[k] = base[k];
+      base[k] = 0;
+    }
+  }
+  __syncthreads();
+  auto size_of = [&](int k) { return direct ? size[k] : __ldcg(a.total + k); };
+  const Three all = scan_groups(K, red, size_of, [&](int k, int r, int t, int p) {
+    base[k] += r;
+    if (a.keep) {
+      size[k] = r;  // from here on: starts
+      first[k] = t;
+      first2[k] = p;
+    }
+    if (block == 0) a.offsets[k] = r;  // offsets[K]: end of the last group, start of the unassigned slots
+  });
+  if (block == 0 && threadIdx.x == 0) {
+    a.tiles[0] = all.b;
+    a.tiles[1] = all.c;
+  }
+  __syncthreads();
+  walk<PACK, false>(a, begin, end, mine, base);
+  if (!a.keep) {  // base and counters are done with: the scans again, in their place
+    __syncthreads();
+    size = sm;
+    first = size + K1;
+    first2 = first + K1;
+    scan_groups(K, red, size_of, [&](int k, int r, int t, int p) {
+      size[k] = r;
+      first[k] = t;
+      first2[k] = p;
+    });
+    __syncthreads();
+  }
+  const int t0 = block * blockDim.x + threadIdx.x, step = nblocks * blockDim.x;
+  for (int t = t0; t < all.b; t += step) fill_tile(K, first, size, a.slots, kTileRows, a.tiles + kTileHeader, t);
+  for (int t = t0; t < all.c; t += step) fill_tile(K, first2, size, a.slots, kPairRows, a.tiles + kTileHeader + a.pairs, t);
 }
 
 struct Plan {
-  bool small;
-  int smem;             // dynamic shared memory of the walking kernels
-  int warps, blocks;    // per block, grid
-  int nwarps;           // rows of the table
-  int64_t chunk;
-  int64_t table, total, start, first, first2, bytes;  // workspace offsets (large path)
+  bool pack, keep, direct;
+  int warps, blocks, chunk, smem;
+  int64_t table, total, barrier, bytes;  // workspace offsets
 };
 
-Plan make_plan(int64_t slots, int64_t K) {
+Plan make_plan(int64_t slots, int64_t K, int sms) {
   Plan p{};
   const int64_t K1 = K + 1;
-  const int64_t small = (kWarps + 3) * K1 * 4;
-  p.small = slots <= kSmallSlots && small <= kSmallSmem;
-  if (p.small) {
-    p.smem = (int)small;
-    p.bytes = 256;
-    return p;
+  // base, counters, and the three scans where they fit beside 32 warps' counters
+  const int64_t fixed = K1 * 4, scans = 3 * K1 * 4;
+  p.keep = fixed + scans + kMaxWarps * K1 * 4 <= kMaxSmem;
+  p.pack = !p.keep && slots < (int64_t)sms * 65536;  // then a block's chunk stays below 2^16
+  const int64_t per_warp = p.pack ? (K1 + 1) / 2 * 4 : K1 * 4;
+  p.warps = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxWarps, (kMaxSmem - fixed) / per_warp));
+  // four steps of 32 slots per warp before another block is worth its part of the barrier
+  p.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(sms, ceil_div(slots, (int64_t)p.warps * 128)));
+  p.chunk = (int)round_up(std::max<int64_t>(1, ceil_div(slots, (int64_t)p.warps * p.blocks)), 32);
+  if (p.pack && (int64_t)p.warps * p.chunk > 65535) {
+    p.pack = false;
+    p.warps = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxWarps, (kMaxSmem - fixed) / (K1 * 4)));
+    p.blocks = sms;
+    p.chunk = (int)round_up(ceil_div(slots, (int64_t)p.warps * p.blocks), 32);
   }
-  p.warps = (int)std::min<int64_t>(kWarps, std::max<int64_t>(1, kTableSmem / (K1 * 4)));
-  const int64_t most = std::min<int64_t>(kMaxWarps, (int64_t)148 * p.warps);
-  p.chunk = round_up(std::max<int64_t>(kChunk, ceil_div(slots, most)), 128);
-  p.nwarps = (int)std::max<int64_t>(1, ceil_div(slots, p.chunk));
-  p.blocks = (int)ceil_div(p.nwarps, p.warps);
-  p.smem = (int)(p.warps * K1 * 4);
+  const int64_t counters = p.warps * (p.pack ? (K1 + 1) / 2 * 4 : K1 * 4);
+  p.smem = (int)(p.keep ? fixed + counters + scans : std::max(fixed + counters, scans));
+  p.direct = p.keep && (p.blocks <= 8 || p.blocks * K1 <= kDirectTable);
   int64_t off = 0;
-  p.table = off; off += round_up((int64_t)p.nwarps * K1 * 4, 256);
+  p.table = off; off += round_up((int64_t)p.blocks * K1 * 4, 256);
   p.total = off; off += round_up(K1 * 4, 256);
-  p.start = off; off += round_up(K1 * 4, 256);
-  p.first = off; off += round_up(K1 * 4, 256);
-  p.first2 = off; off += round_up(K1 * 4, 256);
-  p.bytes = off;
+  p.barrier = off; off += 256;
+  p.bytes = p.blocks == 1 && p.direct ? 256 : off;
   return p;
 }
 
+template <int SYNC, bool PACK>
+int launch_route(const RouteArgs& a, const Plan& p, cudaStream_t st) {
+  const auto kern = route_kernel<SYNC, PACK>;
+  static SmemGrants grants;
+  if (int rc = allow_smem((const void*)kern, kMaxSmem, grants)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  if (SYNC == kCluster) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.blocks;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+  } else {
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+  }
+  cfg.gridDim = dim3(p.blocks);
+  cfg.blockDim = dim3(p.warps * 32);
+  cfg.dynamicSmemBytes = p.smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = SYNC == kOneBlock ? 0 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
+  if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "route_kernel launch: %s", cudaGetErrorString(e));
+  return GMMXX_OK;
+}
+
+// The plan must not depend on a device query where the workspace is sized
+// without one: B200's SM count.  A device with fewer SMs could not hold the
+// cooperative grid at once and would refuse the launch.
+constexpr int kSms = 148;
+
 }  // namespace
+
+int route_status(int* flag, cudaStream_t st) { return take_flag((const void*)&g_route_status, flag, st); }
 
 int64_t tiles_len(int64_t slots, int64_t K) {
   return kTileHeader + kTileInts * (most_tiles(slots, K, kTileRows) + most_tiles(slots, K, kPairRows));
 }
 
-size_t group_rows_ws(int64_t slots, int64_t K) { return (size_t)make_plan(slots, K).bytes; }
+size_t group_rows_ws(int64_t slots, int64_t K) { return (size_t)make_plan(slots, K, kSms).bytes; }
 
 int launch_group_rows(const void* labels, int wide, int64_t slots, int64_t K, int32_t* order, int32_t* offsets,
                       int32_t* tiles, char* ws, cudaStream_t st) {
-  const Plan p = make_plan(slots, K);
-  const int64_t pairs = kTileInts * most_tiles(slots, K, kTileRows);
-  if (p.small) {
-    static SmemGrants grants;
-    if (int rc = allow_smem((const void*)group_rows_small_kernel, kSmallSmem, grants)) return rc;
-    group_rows_small_kernel<<<1, 1024, p.smem, st>>>(labels, wide, (int)slots, (int)K, order, offsets, tiles, pairs);
-    return check_launch("group_rows_small_kernel");
-  }
-  int* table = reinterpret_cast<int*>(ws + p.table);
-  int* total = reinterpret_cast<int*>(ws + p.total);
-  int* start = reinterpret_cast<int*>(ws + p.start);
-  int* first = reinterpret_cast<int*>(ws + p.first);
-  int* first2 = reinterpret_cast<int*>(ws + p.first2);
-  static SmemGrants count_grants, place_grants;
-  if (int rc = allow_smem((const void*)count_kernel, kTableSmem, count_grants)) return rc;
-  if (int rc = allow_smem((const void*)place_kernel, kTableSmem, place_grants)) return rc;
-  count_kernel<<<p.blocks, p.warps * 32, p.smem, st>>>(labels, wide, slots, (int)K, p.chunk, p.nwarps, table);
-  if (int rc = check_launch("count_kernel")) return rc;
-  columns_kernel<<<(unsigned)ceil_div(K + 1, 32), 1024, 0, st>>>(table, p.nwarps, (int)K + 1, total);
-  if (int rc = check_launch("columns_kernel")) return rc;
-  totals_kernel<<<1, 1024, 0, st>>>(total, (int)K, start, first, first2, offsets, tiles);
-  if (int rc = check_launch("totals_kernel")) return rc;
-  place_kernel<<<p.blocks, p.warps * 32, p.smem, st>>>(labels, wide, slots, (int)K, p.chunk, p.nwarps, table, start,
-                                                       first, first2, order, tiles, pairs);
-  return check_launch("place_kernel");
+  const Plan p = make_plan(slots, K, kSms);
+  RouteArgs a{};
+  a.labels = labels;
+  a.wide = wide;
+  a.slots = (int)slots;
+  a.K = (int)K;
+  a.chunk = p.chunk;
+  a.table = reinterpret_cast<int*>(ws + p.table);
+  a.total = reinterpret_cast<int*>(ws + p.total);
+  a.barrier = reinterpret_cast<int*>(ws + p.barrier);
+  a.order = order;
+  a.offsets = offsets;
+  a.tiles = tiles;
+  a.pairs = kTileInts * most_tiles(slots, K, kTileRows);
+  a.keep = p.keep;
+  a.direct = p.direct;
+  if (p.blocks == 1) return p.pack ? launch_route<kOneBlock, true>(a, p, st) : launch_route<kOneBlock, false>(a, p, st);
+  if (p.blocks <= 8) return p.pack ? launch_route<kCluster, true>(a, p, st) : launch_route<kCluster, false>(a, p, st);
+  const cudaError_t e = cudaMemsetAsync(a.barrier, 0, sizeof(int), st);
+  if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "memset: %s", cudaGetErrorString(e));
+  return p.pack ? launch_route<kGrid, true>(a, p, st) : launch_route<kGrid, false>(a, p, st);
 }
 
 }  // namespace experts

@@ -286,7 +286,7 @@ GMMXX_API int gmmxx_label_stats(int x_dtype, const void* x, int64_t B, int64_t N
  *   sorted by label, equal labels in slot order, unassigned slots last.
  *   offsets_out (K + 1): group k is order[offsets[k] .. offsets[k + 1]).
  *   tiles_out: gmmxx_group_tiles_len(slots, K) int32, the table of row tiles
- *   that the product kernels walk (opaque).  slots < 2^31, 1 <= K <= 32768. */
+ *   that the product kernels walk (opaque).  slots < 2^31, 1 <= K <= 16384. */
 GMMXX_API int64_t gmmxx_group_tiles_len(int64_t slots, int64_t K);
 GMMXX_API size_t gmmxx_group_rows_workspace_bytes(int64_t slots, int64_t K);
 GMMXX_API int gmmxx_group_rows(const void* labels, int label_bytes, int64_t slots, int64_t K, int32_t* order_out,
@@ -318,7 +318,7 @@ GMMXX_API int gmmxx_grouped_matmul_backward(int dtype, const void* grad_out, con
                                             size_t workspace_bytes, void* stream);
 
 /* GMMXX_OK, or GMMXX_ERR_TIMEOUT when a bounded device-side wait ran out in a
- * product or orthogonalisation kernel of the current device since the last
+ * routing, product or orthogonalisation kernel of the current device since the last
  * call (those kernels' results are undefined).  Synchronises the stream. */
 GMMXX_API int gmmxx_products_status(int* status_out, void* stream);
 

@@ -55,7 +55,7 @@ def test_group_rows_arguments(host_checks):
     with pytest.raises(ValueError, match="choice"):
         gm.group_rows(torch.zeros(4, 0, dtype=torch.int64), 3)
     with pytest.raises(nat.UnsupportedShape, match="routing window"):
-        gm.group_rows(torch.zeros(4, dtype=torch.int64), 32769)
+        gm.group_rows(torch.zeros(4, dtype=torch.int64), 16385)
 
 
 def test_product_arguments(host_checks):

@@ -117,7 +117,8 @@ def _check_groups(labels, k, groups):
 
 
 @pytest.mark.parametrize("n,top,k", [(1, 1, 1), (31, 1, 3), (129, 2, 16), (4097, 8, 64), (32768, 1, 1500),
-                                     (32769, 1, 7), (100003, 1, 8192), (70001, 2, 32768), (300000, 1, 1)])
+                                     (32769, 1, 7), (100003, 1, 8192), (70001, 2, 16384), (300000, 1, 1),
+                                     (1000, 1, 16384), (900001, 1, 300), (1500007, 1, 3000), (2, 1, 9000)])
 @pytest.mark.parametrize("kind", ["even", "dropped", "skewed"])
 @pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
 def test_group_rows(cuda_device, n, top, k, kind, dtype):
