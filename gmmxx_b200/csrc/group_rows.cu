@@ -264,10 +264,15 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) route_kernel(const RouteArg
       if (2 * i + 1 < K1) base[2 * i + 1] = hi;
     } else {
       int run = 0;
-      for (int w = 0; w < warps; ++w) {
-        const int c = counters[w * words + i];
-        counters[w * words + i] = run;
-        run += c;
+      for (int w0 = 0; w0 < warps; w0 += 8) {  // eight loads at a time: each would wait for the store before it
+        int c[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) c[u] = w0 + u < warps ? counters[(w0 + u) * words + i] : 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          if (w0 + u < warps) counters[(w0 + u) * words + i] = run;
+          run += c[u];
+        }
       }
       base[i] = run;
     }
@@ -278,46 +283,60 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) route_kernel(const RouteArg
   if (SYNC != kOneBlock) {
     for (int k = threadIdx.x; k < K1; k += blockDim.x) row[k] = base[k];
     if (!barrier<SYNC>(a, 1)) return;
-    // 32 columns at a time, the rows cut over the warps
-    const int per = (nblocks + warps - 1) / warps, b0 = min(nblocks, warp * per), b1 = min(nblocks, b0 + per);
-    for (int k0 = direct ? 0 : block * 32; k0 < K1; k0 += direct ? 32 : nblocks * 32) {
-      const int k = k0 + lane;
-      int all = 0, before = 0;
-      if (k < K1) {
-#pragma unroll 4
-        for (int b = b0; b < b1; ++b) {
+    if (direct && nblocks <= 16) {  // few rows: a thread per column
+      for (int k = threadIdx.x; k < K1; k += blockDim.x) {
+        int all = 0, before = 0;
+#pragma unroll 8
+        for (int b = 0; b < nblocks; ++b) {
           const int c = __ldcg(a.table + (int64_t)b * K1 + k);
           all += c;
           before += b < block ? c : 0;
         }
+        base[k] = before;
+        size[k] = all;
       }
-      part[0][warp][lane] = all;
-      part[1][warp][lane] = before;
-      __syncthreads();
-      if (direct) {  // this block's start and the total of its columns
-        if (warp == 0 && k < K1) {
-          int t = 0, f = 0;
-          for (int w = 0; w < warps; ++w) {
-            t += part[0][w][lane];
-            f += part[1][w][lane];
-          }
-          base[k] = f;
-          size[k] = t;
-        }
-      } else {  // every block's start, in place
-        int run = 0;
-        for (int w = 0; w < warp; ++w) run += part[0][w][lane];
+    } else {
+      // 32 columns at a time, the rows cut over the warps
+      const int per = (nblocks + warps - 1) / warps, b0 = min(nblocks, warp * per), b1 = min(nblocks, b0 + per);
+      for (int k0 = direct ? 0 : block * 32; k0 < K1; k0 += direct ? 32 : nblocks * 32) {
+        const int k = k0 + lane;
+        int all = 0, before = 0;
         if (k < K1) {
-          if (warp == warps - 1) a.total[k] = run + all;
+#pragma unroll 4
           for (int b = b0; b < b1; ++b) {
-            int* p = a.table + (int64_t)b * K1 + k;
-            const int c = __ldcg(p);
-            *p = run;
-            run += c;
+            const int c = __ldcg(a.table + (int64_t)b * K1 + k);
+            all += c;
+            before += b < block ? c : 0;
           }
         }
+        part[0][warp][lane] = all;
+        part[1][warp][lane] = before;
+        __syncthreads();
+        if (direct) {  // this block's start and the total of its columns
+          if (warp == 0 && k < K1) {
+            int t = 0, f = 0;
+            for (int w = 0; w < warps; ++w) {
+              t += part[0][w][lane];
+              f += part[1][w][lane];
+            }
+            base[k] = f;
+            size[k] = t;
+          }
+        } else {  // every block's start, in place
+          int run = 0;
+          for (int w = 0; w < warp; ++w) run += part[0][w][lane];
+          if (k < K1) {
+            if (warp == warps - 1) a.total[k] = run + all;
+            for (int b = b0; b < b1; ++b) {
+              int* p = a.table + (int64_t)b * K1 + k;
+              const int c = __ldcg(p);
+              *p = run;
+              run += c;
+            }
+          }
+        }
+        __syncthreads();
       }
-      __syncthreads();
     }
     if (!direct) {
       if (!barrier<SYNC>(a, 2)) return;
@@ -379,6 +398,9 @@ Plan make_plan(int64_t slots, int64_t K, int sms) {
   p.pack = !p.keep && slots < (int64_t)sms * 65536;  // then a block's chunk stays below 2^16
   const int64_t per_warp = p.pack ? (K1 + 1) / 2 * 4 : K1 * 4;
   p.warps = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxWarps, (kMaxSmem - fixed) / per_warp));
+  // few slots: only as many warps as they (and the scans over the components) use
+  if (slots <= kMaxWarps * 64)
+    p.warps = (int)std::min<int64_t>(p.warps, std::max<int64_t>(4, std::max(ceil_div(slots, 64), ceil_div(K1, 128))));
   // four steps of 32 slots per warp before another block is worth its part of the barrier
   p.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(sms, ceil_div(slots, (int64_t)p.warps * 128)));
   p.chunk = (int)round_up(std::max<int64_t>(1, ceil_div(slots, (int64_t)p.warps * p.blocks)), 32);
