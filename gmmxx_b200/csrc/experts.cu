@@ -175,14 +175,42 @@ int rows_product(int dt, const Planes& src, int div, const Groups& g, int64_t k_
   return launch_product(kRows, src.n, pair, maps, a, g.max_tiles(rows_per), st);
 }
 
-// gx[row] = sum over the row's slots, rounded once
-__global__ void sum_slots_kernel(const float* part, int64_t rows, int top, int n, void* out, int dt) {
-  const int64_t total = rows * n;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t row = i / n, c = i % n;
-    float s = 0.f;
-    for (int t = 0; t < top; ++t) s += part[(row * top + t) * n + c];
-    store_y(out, i, dt, s);
+// gx[row] = sum over the row's slots, rounded once: four columns per thread
+// (one where rows are no multiple of four), a block per stretch of one row
+template <int V>
+__global__ void __launch_bounds__(256) sum_slots_kernel(const float* part, int64_t rows, int top, int n, void* out,
+                                                        int dt) {
+  const int c = (blockIdx.y * 256 + threadIdx.x) * V;
+  if (c >= n) return;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const float* p = part + row * top * n + c;
+    float s[V] = {};
+    for (int t = 0; t < top; ++t, p += n) {
+      if (V == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        s[0] += v.x;
+        s[V > 1 ? 1 : 0] += v.y;
+        s[V > 2 ? 2 : 0] += v.z;
+        s[V > 3 ? 3 : 0] += v.w;
+      } else {
+        s[0] += *p;
+      }
+    }
+    const int64_t at = row * n + c;
+    if (V == 4 && dt == GMMXX_FLOAT32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = make_float4(s[0], s[1 % V], s[2 % V], s[3 % V]);
+    } else if (V == 4) {
+      uint2 q;
+      if (dt == GMMXX_BFLOAT16) {
+        q = make_uint2(ptx::pack_bf16(s[0], s[1 % V]), ptx::pack_bf16(s[2 % V], s[3 % V]));
+      } else {
+        const __half2 x = __floats2half2_rn(s[0], s[1 % V]), y = __floats2half2_rn(s[2 % V], s[3 % V]);
+        q = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+      }
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = q;
+    } else {
+      store_y(out, at, dt, s[0]);
+    }
   }
 }
 
@@ -213,47 +241,54 @@ SegPlan seg_plan(const Groups& g, int64_t m, int64_t n) {
   return p;
 }
 
-__device__ __forceinline__ int block_exclusive(int v, int* red, int* total) {
+// exclusive scans of three values per thread over a block of 1024; red: 96 ints
+__device__ __forceinline__ int3 block_exclusive3(int3 v, int* red, int3* total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int s = v;
+  int3 s = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int t = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += t;
+    const int x = __shfl_up_sync(0xffffffffu, s.x, o), y = __shfl_up_sync(0xffffffffu, s.y, o),
+              z = __shfl_up_sync(0xffffffffu, s.z, o);
+    if (lane >= o) s = make_int3(s.x + x, s.y + y, s.z + z);
   }
   __syncthreads();
-  if (lane == 31) red[w] = s;
+  if (lane == 31) {
+    red[w] = s.x;
+    red[32 + w] = s.y;
+    red[64 + w] = s.z;
+  }
   __syncthreads();
-  int before = 0, all = 0;
+  int3 before = make_int3(0, 0, 0), all = before;
+#pragma unroll 8
   for (int i = 0; i < 32; ++i) {
-    if (i < w) before += red[i];
-    all += red[i];
+    const int x = red[i], y = red[32 + i], z = red[64 + i];
+    if (i < w) before = make_int3(before.x + x, before.y + y, before.z + z);
+    all = make_int3(all.x + x, all.y + y, all.z + z);
   }
   *total = all;
-  return before + s - v;
+  return make_int3(before.x + s.x - v.x, before.y + s.y - v.y, before.z + s.z - v.z);
 }
 
 // table: [0] segments, [1] split groups; per segment {group, first position,
 // rows, partial slot or -1}; split[i] = {group, first slot, segments, 0}
 __global__ void __launch_bounds__(1024) segments_kernel(const int32_t* offsets, int K, int seg, int32_t* table,
                                                         int4* split) {
-  __shared__ int red[32];
+  __shared__ int red[96];
   int seg0 = 0, slot0 = 0, split0 = 0;
   for (int k0 = 0; k0 < K; k0 += 1024) {
     const int k = k0 + threadIdx.x;
     const int pos = k < K ? offsets[k] : 0, c = k < K ? offsets[k + 1] - pos : 0;
     const int ns = k < K ? max(1, (int)(((int64_t)c + seg - 1) / seg)) : 0;
-    int n_segs, n_slots, n_split;
-    const int s = seg0 + block_exclusive(ns, red, &n_segs);
-    const int sl = slot0 + block_exclusive(ns > 1 ? ns : 0, red, &n_slots);
-    const int sp = split0 + block_exclusive(ns > 1 ? 1 : 0, red, &n_split);
+    int3 all;
+    const int3 at = block_exclusive3(make_int3(ns, ns > 1 ? ns : 0, ns > 1 ? 1 : 0), red, &all);
+    const int s = seg0 + at.x, sl = slot0 + at.y, sp = split0 + at.z;
     for (int i = 0; i < ns; ++i)
       reinterpret_cast<int4*>(table + kSegHeader)[s + i] =
           make_int4(k, pos + i * seg, min(seg, c - i * seg), ns > 1 ? sl + i : -1);
     if (ns > 1) split[sp] = make_int4(k, sl, ns, 0);
-    seg0 += n_segs;
-    slot0 += n_slots;
-    split0 += n_split;
+    seg0 += all.x;
+    slot0 += all.y;
+    split0 += all.z;
   }
   if (threadIdx.x == 0) {
     table[0] = seg0;
@@ -288,7 +323,7 @@ __global__ void __launch_bounds__(256) bias_kernel(const int32_t* table, const i
     const int4 s = reinterpret_cast<const int4*>(table + kSegHeader)[it];
     float acc[8] = {};
     if (c < n) {
-#pragma unroll 2
+#pragma unroll 8
       for (int r = rl; r < s.z; r += 16) {
         const int64_t at = (int64_t)order[s.y + r] * n + c;
         if (vec && dt != GMMXX_FLOAT32) {
@@ -328,38 +363,100 @@ __global__ void __launch_bounds__(256) bias_kernel(const int32_t* table, const i
 // Newton-Schulz
 // ---------------------------------------------------------------------------
 
-constexpr int kNormBlocks = 64;  // per matrix, at most
+constexpr int kNormBlocks = 256;  // per matrix, at most
 
-__global__ void __launch_bounds__(256) square_sum_kernel(int dt, const void* g, int64_t n, double* part) {
+// eight consecutive values as fp32 (the caller checks alignment), or one by one
+__device__ __forceinline__ void load8(const void* p, int64_t i, int dt, float* v) {
+  if (dt == GMMXX_FLOAT32) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const float4 x = q[0], y = q[1];
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+  } else {
+    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float2 f;
+      if (dt == GMMXX_BFLOAT16) f = make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u));
+      else f = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  }
+}
+
+// sums of squares: a matrix's elements in order over gridDim.x blocks; pieces
+// of eight where they are aligned (whole: n is a multiple of eight)
+__global__ void __launch_bounds__(256) square_sum_kernel(int dt, const void* g, int64_t n, int whole, double* part) {
   __shared__ double red[8];
-  const int64_t base = (int64_t)blockIdx.y * n;
+  const int64_t base = (int64_t)blockIdx.y * n, step = (int64_t)gridDim.x * 256;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   double s = 0.0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const double v = load_x(g, base + i, dt);
-    s += v * v;
+  if (whole) {
+#pragma unroll 4
+    for (int64_t i = t; i < n / 8; i += step) {
+      float v[8];
+      load8(g, base + i * 8, dt, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += (double)v[j] * v[j];
+    }
+  } else {
+#pragma unroll 8
+    for (int64_t i = t; i < n; i += step) {
+      const double v = load_x(g, base + i, dt);
+      s += v * v;
+    }
   }
   s = block_sum(s, red);
   if (threadIdx.x == 0) part[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = s;
 }
 
-// x = g / (|g| + eps) as fp16 planes of x * kPlaneScale, or (q) rounded to the result
-__global__ void __launch_bounds__(256) scale_kernel(int dt, const void* g, int64_t m, int n, int ld, float eps,
-                                                    const double* part, int nparts, __half* hi, __half* lo, void* q) {
-  const int64_t z = blockIdx.y, total = m * n;
-  double s = 0.0;
-  for (int i = 0; i < nparts; ++i) s += part[z * nparts + i];
-  const double inv = 1.0 / (sqrt(s) + (double)eps);
+// x = g / (|g| + eps) as fp16 planes of x * kPlaneScale, or (q) rounded to the
+// result; a thread takes eight columns of a row
+__global__ void __launch_bounds__(256) scale_kernel(int dt, const void* g, int64_t m, int n, int ld, int whole,
+                                                    float eps, const double* part, int nparts, __half* hi, __half* lo,
+                                                    void* q) {
+  __shared__ double inv_s;
+  const int64_t z = blockIdx.y;
+  if (threadIdx.x < 32) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < nparts; i += 32) s += part[z * nparts + i];
+    s = warp_sum_d(s);
+    if (threadIdx.x == 0) inv_s = 1.0 / (sqrt(s) + (double)eps);
+  }
+  __syncthreads();
+  const double inv = inv_s;
+  const int per = ld / 8;
+  const int64_t total = m * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const double v = load_x(g, z * total + i, dt) * inv;
+    const int64_t r = i / per;
+    const int c = (int)(i - r * per) * 8, left = n - c;
+    const int64_t at = (z * m + r) * n + c;
+    float v[8];
+    if (whole) {
+      load8(g, at, dt, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < left ? load_x(g, at + j, dt) : 0.f;
+    }
     if (q != nullptr) {
-      store_y(q, z * total + i, dt, (float)v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < left) store_y(q, at + j, dt, (float)(v[j] * inv));
       continue;
     }
-    const int64_t at = (z * m + i / n) * ld + i % n;
-    const float f = (float)(v * kPlaneScale);
-    const __half h = __float2half_rn(f);
-    hi[at] = h;
-    if (lo != nullptr) lo[at] = __float2half_rn(f - __half2float(h));
+    uint4 h, l;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = (float)(v[2 * j] * inv * kPlaneScale), y = (float)(v[2 * j + 1] * inv * kPlaneScale);
+      const __half2 p = __floats2half2_rn(x, y);
+      const float2 f = __half22float2(p);
+      reinterpret_cast<__half2*>(&h)[j] = p;
+      reinterpret_cast<__half2*>(&l)[j] = __floats2half2_rn(x - f.x, y - f.y);
+    }
+    const int64_t o = (z * m + r) * ld + c;
+    *reinterpret_cast<uint4*>(hi + o) = h;
+    if (lo != nullptr) *reinterpret_cast<uint4*>(lo + o) = l;
   }
 }
 
@@ -382,7 +479,7 @@ NsPlan ns_plan(int dt, int64_t batch, int64_t m, int64_t n) {
   s.ldp = pad8(s.lo);
   s.x_plane = al256(batch * m * s.ldx * 2);
   s.p_plane = al256(batch * s.lo * s.ldp * 2);
-  s.nparts = (int)std::min<int64_t>(kNormBlocks, ceil_div(m * n, 4096));
+  s.nparts = (int)std::min<int64_t>(kNormBlocks, ceil_div(m * n, 8192));
   int64_t off = 0;
   s.x = off; off += s.x_plane * s.planes;
   s.y = off; off += s.x_plane * s.planes;
@@ -446,8 +543,10 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
                               g.top > 1 ? GMMXX_FLOAT32 : dt, st))
       return rc;
     if (g.top > 1) {
-      const int64_t blocks = std::min<int64_t>(148 * 16, ceil_div(g.rows * n_in, 256));
-      sum_slots_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const float*>(to), g.rows, g.top, (int)n_in, gx, dt);
+      const int per = vec_ok(gx, dt, n_in) ? 4 : 1;
+      const dim3 grid((unsigned)std::min<int64_t>(g.rows, 148 * 64), (unsigned)ceil_div(n_in, 256 * per));
+      if (per == 4) sum_slots_kernel<4><<<grid, 256, 0, st>>>(static_cast<const float*>(to), g.rows, g.top, (int)n_in, gx, dt);
+      else sum_slots_kernel<1><<<grid, 256, 0, st>>>(static_cast<const float*>(to), g.rows, g.top, (int)n_in, gx, dt);
       if (int rc = check_launch("sum_slots_kernel")) return rc;
     }
   }
@@ -549,12 +648,13 @@ int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_
     const unsigned nz = (unsigned)std::min<int64_t>(65535, batch - z0);
     const char* gz = static_cast<const char*>(g) + z0 * size * elem_bytes(dt);
     double* pz = part + z0 * s.nparts;
-    square_sum_kernel<<<dim3((unsigned)s.nparts, nz), 256, 0, st>>>(dt, gz, size, pz);
+    const int aligned = (reinterpret_cast<uintptr_t>(gz) & 15) == 0;
+    square_sum_kernel<<<dim3((unsigned)s.nparts, nz), 256, 0, st>>>(dt, gz, size, aligned && size % 8 == 0, pz);
     if (int rc = check_launch("square_sum_kernel")) return rc;
     __half* hi = reinterpret_cast<__half*>(ws + s.x) + z0 * m * s.ldx;
     __half* lo = s.planes > 1 ? reinterpret_cast<__half*>(ws + s.x + s.x_plane) + z0 * m * s.ldx : nullptr;
-    scale_kernel<<<dim3((unsigned)std::min<int64_t>(256, ceil_div(size, 1024)), nz), 256, 0, st>>>(
-        dt, gz, m, (int)n, (int)s.ldx, eps, pz, s.nparts, hi, lo,
+    scale_kernel<<<dim3((unsigned)std::min<int64_t>(1024, ceil_div(m * s.ldx, 2048)), nz), 256, 0, st>>>(
+        dt, gz, m, (int)n, (int)s.ldx, aligned && n % 8 == 0, eps, pz, s.nparts, hi, lo,
         steps == 0 ? static_cast<char*>(q) + z0 * size * elem_bytes(dt) : nullptr);
     if (int rc = check_launch("scale_kernel")) return rc;
   }

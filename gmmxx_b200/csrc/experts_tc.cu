@@ -57,7 +57,7 @@ static __device__ int g_status = 0;  // sticky: 1 when a bounded wait ran out (g
 namespace {
 
 constexpr int kBM = 128;
-constexpr int kGatherWarp0 = 12, kGatherThreads = 128;
+constexpr int kGatherWarp0 = 12;
 constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
 constexpr int kABytes = kBM * 128;  // one plane of A per stage
 constexpr int kMaxStages = 8;
@@ -276,7 +276,9 @@ template <int KIND, int PLANES, int CG>
 struct Roles {
   static constexpr bool kGather = KIND != kBatch && PLANES == 1;      // rows by cp.async
   static constexpr bool kTma = !(KIND == kWeights && PLANES == 1);    // something by TMA
-  static constexpr int kThreads = kGather ? 512 : 384;
+  // kWeights fetches both operands: the copies' address arithmetic held four warps at 1250 cycles a stage
+  static constexpr int kGatherThreads = KIND == kWeights ? 256 : 128;
+  static constexpr int kThreads = 384 + (kGather ? kGatherThreads : 0);
   static constexpr bool kRelay = kGather || CG > 1;                   // stages reach the products through `ready`
   static constexpr int kFullCount = (kGather ? kGatherThreads : 0) + (kTma ? 1 : 0);
 };
@@ -538,8 +540,26 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
     const int c_lo = (w >> 2) * (a.bn / 2), c_hi = c_lo + a.bn / 2;
     Ring sums;
     bool ok = true;
-    for (int64_t it = first; ok && it < total; it += stride) {
-      const Tile t = decode<KIND, CG>(a, it, rank);
+    // Rows in store order: lane takes rows r8 + 4 i, four columns each (8 lanes per row).  Where the rows are
+    // routed, the next tile's place is fetched while this one's products run: table, then order.
+    const int row0 = (w & 3) * 32, r8 = lane >> 3, c4 = (lane & 7) * 4;
+    int slot_of[KIND == kRows ? 8 : 1];
+    auto fetch_rows = [&](const Tile& u) {
+      if (KIND != kRows) return;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = row0 + r8 + 4 * i;
+        slot_of[i] = r < u.rows ? __ldg(a.order + u.pos + r) : -1;
+      }
+    };
+    Tile t{};
+    if (first < total) {
+      t = decode<KIND, CG>(a, first, rank);
+      fetch_rows(t);
+    }
+    Tile u = t;
+    for (int64_t it = first; ok && it < total; it += stride, t = u) {
+      u = decode<KIND, CG>(a, it + stride < total ? it + stride : it, rank);
       float held[PLANES > 1 ? 64 : 1];  // sums of the finished accumulations (bn <= 128: 64 columns at most)
       if (PLANES > 1) {
 #pragma unroll
@@ -574,10 +594,8 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
       }
       const int buf = sums.i;
       if (PLANES == 1 && t.kb > 0) sums.step(2);
-      // Rows in store order: lane takes rows r8 + 4 i, four columns each (8 lanes per row)
       const int n_left = a.n - t.n0;
       const int valid_rows = KIND == kWeights ? min(kBM, a.m - t.m0) : t.rows;
-      const int row0 = (w & 3) * 32, r8 = lane >> 3, c4 = (lane & 7) * 4;
       void* out = a.out;
       int dt = a.out_dt, vec = a.vec;
       if (KIND == kWeights && t.slot >= 0) {
@@ -585,18 +603,17 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
         dt = GMMXX_FLOAT32;
         vec = (a.n & 3) == 0;
       }
-      // first element of tile row r
-      auto row_at = [&](int r) -> int64_t {
-        if (KIND == kRows) return (int64_t)__ldg(a.order + t.pos + r) * a.ldo;
-        if (KIND == kWeights && t.slot >= 0) return ((int64_t)t.slot * a.m + t.m0 + r) * a.n;
-        return t.g * a.out_stride + (int64_t)(t.m0 + r) * a.ldo;
-      };
+      // first element of this lane's rows
       int64_t at[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = row0 + r8 + 4 * i;
-        at[i] = r < valid_rows ? row_at(r) : -1;
+        if (KIND == kRows) at[i] = slot_of[i] < 0 ? -1 : (int64_t)slot_of[i] * a.ldo;
+        else if (r >= valid_rows) at[i] = -1;
+        else if (KIND == kWeights && t.slot >= 0) at[i] = ((int64_t)t.slot * a.m + t.m0 + r) * a.n;
+        else at[i] = t.g * a.out_stride + (int64_t)(t.m0 + r) * a.ldo;
       }
+      fetch_rows(u);
 #pragma unroll
       for (int j = 0; j < (PLANES > 1 ? 2 : 4); ++j) {
         const int c = c_lo + 32 * j;
@@ -701,12 +718,13 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
     }
   }
   if (R::kGather && warp >= kGatherWarp0) {
-    // ---- gathered rows: thread = 16-byte piece `q` of every 16th row ----
+    // ---- gathered rows: thread = 16-byte piece `q` of every kStep'th row ----
+    constexpr int kStep = R::kGatherThreads / 8, kSkip = kStep * 128;
     const int tid = threadIdx.x - kGatherWarp0 * 32, q = tid & 7, r0 = tid >> 3;
-    const uint32_t at = (uint32_t)(r0 * 128 + ((q ^ (r0 & 7)) << 4));  // 128-byte swizzle; rows r0 + 16 i: + 2048 i
+    const uint32_t at = (uint32_t)(r0 * 128 + ((q ^ (r0 & 7)) << 4));  // 128-byte swizzle; rows r0 + kStep i: + kSkip i
     Ring ring;
     bool ok = true;
-    constexpr int kR = KIND == kRows ? 8 : 4;  // rows of a stage per thread
+    constexpr int kR = (KIND == kRows ? kBM : kBlockK) / kStep;  // rows of a stage per thread
     // The next tile's place and rows are fetched while this tile's stages are
     // in flight: each of these loads waits for the one before.
     Tile t{};
@@ -715,7 +733,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
     auto first_rows = [&](const Tile& u) {
 #pragma unroll
       for (int i = 0; i < kR; ++i) {
-        const int r = r0 + 16 * i;
+        const int r = r0 + kStep * i;
         next[i] = u.kb > 0 && r < u.rows ? __ldg(a.order + u.pos + r) : 0;
       }
     };
@@ -728,7 +746,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
         first_rows(t);
         continue;
       }
-      const char* src[8];
+      const char* src[KIND == kRows ? kR : 2 * kR];
       if (KIND == kRows) {
 #pragma unroll
         for (int i = 0; i < kR; ++i) src[i] = a.src_a + ((int64_t)(next[i] / a.div_a) * a.ld_a + q * 8) * 2;
@@ -738,10 +756,10 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
         const int s = ring.i, nb = t.n0 + rank * bcols;
         if (KIND == kWeights) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < kR; ++i) {
             src[i] = a.src_a + ((int64_t)(next[i] / a.div_a) * a.ld_a + q * 8 + t.m0) * 2;
-            src[4 + i] = a.src_b + ((int64_t)(next[i] / a.div_b) * a.ld_b + q * 8 + nb) * 2;
-            if (!last) next[i] = __ldg(a.order + t.pos + min((kb + 1) * kBlockK + r0 + 16 * i, t.rows - 1));
+            src[kR + i] = a.src_b + ((int64_t)(next[i] / a.div_b) * a.ld_b + q * 8 + nb) * 2;
+            if (!last) next[i] = __ldg(a.order + t.pos + min((kb + 1) * kBlockK + r0 + kStep * i, t.rows - 1));
           }
         }
         ok = wait_phase_warp(&bars.empty[s], ring.phase ^ 1, abort);
@@ -751,17 +769,17 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
           const bool live = kb * kBlockK + q * 8 < a.k;
           const int64_t k0 = live ? (int64_t)kb * (kBlockK * 2) : 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) copy16(sa + 2048 * i, src[i] + k0, live && r0 + 16 * i < t.rows);
+          for (int i = 0; i < kR; ++i) copy16(sa + kSkip * i, src[i] + k0, live && r0 + kStep * i < t.rows);
         } else {
           const uint32_t sb = sa + kABytes;
-          const int left = t.rows - kb * kBlockK - r0;  // rows r0 + 16 i < left are the segment's
+          const int left = t.rows - kb * kBlockK - r0;  // rows r0 + kStep i < left are the segment's
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             const bool in = t.m0 + g * 64 + q * 8 < a.m;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool live = in && 16 * i < left;
-              copy16(sa + g * 8192 + 2048 * i, live ? src[i] + g * 128 : a.src_a, live);
+            for (int i = 0; i < kR; ++i) {
+              const bool live = in && kStep * i < left;
+              copy16(sa + g * 8192 + kSkip * i, live ? src[i] + g * 128 : a.src_a, live);
             }
           }
 #pragma unroll
@@ -769,9 +787,9 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
             if (g >= bcols / 64) break;
             const bool in = nb + g * 64 + q * 8 < a.n;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool live = in && 16 * i < left;
-              copy16(sb + g * 8192 + 2048 * i, live ? src[4 + i] + g * 128 : a.src_b, live);
+            for (int i = 0; i < kR; ++i) {
+              const bool live = in && kStep * i < left;
+              copy16(sb + g * 8192 + kSkip * i, live ? src[kR + i] + g * 128 : a.src_b, live);
             }
           }
         }
