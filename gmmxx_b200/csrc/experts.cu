@@ -134,6 +134,10 @@ bool vec_ok(const void* p, int dt, int64_t ld) {
   return (reinterpret_cast<uintptr_t>(p) & (4 * elem_size(dt) - 1)) == 0 && ld % 4 == 0;
 }
 
+bool packed_ok(const void* p, int dt, int64_t ld) {
+  return dt != GMMXX_FLOAT32 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0;
+}
+
 // ---------------------------------------------------------------------------
 // rows x their group's matrix
 // ---------------------------------------------------------------------------
@@ -170,6 +174,7 @@ int rows_product(int dt, const Planes& src, int div, const Groups& g, int64_t k_
   a.out_dt = out_dt;
   a.ldo = n;
   a.vec = vec_ok(out, out_dt, n);
+  a.packed = packed_ok(out, out_dt, n) && (reinterpret_cast<uintptr_t>(bias) & 15) == 0;
   a.bias = bias;
   a.bias_dt = dt;
   return launch_product(kRows, src.n, pair, maps, a, g.max_tiles(rows_per), st);
@@ -605,6 +610,7 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
     a.ldo = n;
     a.out_stride = m * n;
     a.vec = vec_ok(gw, dt, n);
+    a.packed = packed_ok(gw, dt, n);
     a.part = part;
     if (int rc = launch_product(kWeights, planes, pair, maps, a, p.max_segs, st)) return rc;
     if (p.max_split > 0) {
@@ -680,7 +686,7 @@ int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_
     t.a_mn = a_mn;
     t.b_mn = b_mn;
     t.idesc = product_idesc(1, bn, a_mn, b_mn, pair);
-    t.items = batch;
+    t.items = (int)batch;
     t.alpha = alpha / kPlaneScale;
     t.beta = beta;
     for (int i = 0; i < s.planes; ++i) {

@@ -195,19 +195,18 @@ struct Tile {
 };
 
 template <int KIND>
-__device__ __forceinline__ int64_t tile_count(const ProductArgs& a) {
-  const int64_t items = KIND == kBatch ? a.items : (int64_t)__ldg(a.count);
-  return items * a.mt * a.nt;
+__device__ __forceinline__ int tile_count(const ProductArgs& a) {  // below 2^31: checked before the launch
+  return (KIND == kBatch ? a.items : __ldg(a.count)) * a.mt * a.nt;
 }
 
 // this block's part (its 128 rows) of tile `it` of CG * 128 rows
 template <int KIND, int CG>
-__device__ __forceinline__ Tile decode(const ProductArgs& a, int64_t it, int rank) {
+__device__ __forceinline__ Tile decode(const ProductArgs& a, int it, int rank) {
   Tile t;
-  t.n0 = (int)(it % a.nt) * a.bn;
+  t.n0 = it % a.nt * a.bn;
   it /= a.nt;
   if (KIND == kRows) {
-    const int32_t* e = a.table + it * kTileInts;
+    const int32_t* e = a.table + (int64_t)it * kTileInts;
     t.g = __ldg(e);
     t.pos = __ldg(e + 1) + rank * kBM;
     t.rows = max(0, min(kBM, __ldg(e + 2) - rank * kBM));
@@ -216,17 +215,17 @@ __device__ __forceinline__ Tile decode(const ProductArgs& a, int64_t it, int ran
     t.kb = t.g < a.groups ? (a.k + kBlockK - 1) / kBlockK : 0;
     return t;
   }
-  t.m0 = ((int)(it % a.mt) * CG + rank) * kBM;
+  t.m0 = (it % a.mt * CG + rank) * kBM;
   it /= a.mt;
   if (KIND == kWeights) {
-    const int32_t* e = a.table + it * kSegInts;
+    const int32_t* e = a.table + (int64_t)it * kSegInts;
     t.g = __ldg(e);
     t.pos = __ldg(e + 1);
     t.rows = __ldg(e + 2);
     t.slot = __ldg(e + 3);
     t.kb = (t.rows + kBlockK - 1) / kBlockK;
   } else {
-    t.g = (int)it;
+    t.g = it;
     t.pos = 0;
     t.rows = min(kBM, a.m - t.m0);
     t.slot = -1;
@@ -294,7 +293,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
   const int rank = CG == 1 ? 0 : (int)cluster_rank();
   const int bcols = a.bn / CG;     // columns of B that this block loads
   const int bbytes = bcols * 128;  // one plane of B per stage
-  const int64_t first = blockIdx.x / CG, stride = gridDim.x / CG;
+  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
   const int stage_bytes = PLANES * (kABytes + bbytes);
   volatile int* abort = &bars.abort;
   // two buffers of one accumulator, or of two (leading products, others)
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
   block_or_pair_sync<CG>();
   tmem_fence_after();
   const uint32_t tmem = bars.tmem_base;
-  const int64_t total = tile_count<KIND>(a);
+  const int total = tile_count<KIND>(a);
 
   if (R::kTma && warp == 0) {
     // ---- tiled loads: kRows' matrices, sorted planes, stacks ----
@@ -330,7 +329,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
     int64_t filled = 0;
     bool ok = true;
     const uint32_t bytes = (uint32_t)(R::kGather ? bbytes : stage_bytes);
-    for (int64_t it = first; ok && it < total; it += stride) {
+    for (int it = first; ok && it < total; it += stride) {
       const Tile t = decode<KIND, CG>(a, it, rank);
       for (int kb = 0; kb < t.kb; ++kb, ring.step(a.stages), ++filled) {
         const int s = ring.i;
@@ -386,8 +385,8 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
       uint64_t* there = R::kRelay ? bars.ready : bars.full;
       Tile t{};
       if (first < total) t = decode<KIND, CG>(a, first, rank);
-      for (int64_t it = first; ok && it < total; it += stride) {
-        const int64_t ahead = it + stride < total ? it + stride : it;
+      for (int it = first; ok && it < total; it += stride) {
+        const int ahead = it + stride < total ? it + stride : it;
         if (t.kb == 0) {
           t = decode<KIND, CG>(a, ahead, rank);
           continue;
@@ -445,7 +444,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
     // thread that issues the products ----
     Ring ring;
     bool ok = true;
-    for (int64_t it = first; ok && it < total; it += stride) {
+    for (int it = first; ok && it < total; it += stride) {
       const int n = decode<KIND, CG>(a, it, rank).kb;
       for (int kb = 0; kb < n; ++kb, ring.step(a.stages)) {
         ok = wait_phase_warp(&bars.full[ring.i], ring.phase, abort);
@@ -468,7 +467,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
     const uint64_t desc_b = a.b_mn ? desc_mnmajor(sb0, 8192) : desc_kmajor(sb0);
     const uint32_t stage_units = (uint32_t)stage_bytes >> 4, b_units = (uint32_t)bbytes >> 4;
     const uint32_t idesc = a.idesc;
-    for (int64_t it = first; ok && it < total; it += stride) {
+    for (int it = first; ok && it < total; it += stride) {
       const Tile t = decode<KIND, CG>(a, it, rank);
       int buf = 0;
       uint32_t d = 0;
@@ -543,13 +542,16 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
     // Rows in store order: lane takes rows r8 + 4 i, four columns each (8 lanes per row).  Where the rows are
     // routed, the next tile's place is fetched while this one's products run: table, then order.
     const int row0 = (w & 3) * 32, r8 = lane >> 3, c4 = (lane & 7) * 4;
+    // 16-bit results go 16 bytes per lane: rows lane / 4 + 8 i, four lanes per row.
+    const bool packed = PLANES == 1 && KIND != kBatch && a.packed;
+    const int r4 = lane >> 2;
     int slot_of[KIND == kRows ? 8 : 1];
     auto fetch_rows = [&](const Tile& u) {
       if (KIND != kRows) return;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int r = row0 + r8 + 4 * i;
-        slot_of[i] = r < u.rows ? __ldg(a.order + u.pos + r) : -1;
+        const int r = row0 + (packed ? r4 + 8 * i : r8 + 4 * i);
+        if (i < 4 || !packed) slot_of[i] = r < u.rows ? __ldg(a.order + u.pos + r) : -1;
       }
     };
     Tile t{};
@@ -558,7 +560,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
       fetch_rows(t);
     }
     Tile u = t;
-    for (int64_t it = first; ok && it < total; it += stride, t = u) {
+    for (int it = first; ok && it < total; it += stride, t = u) {
       u = decode<KIND, CG>(a, it + stride < total ? it + stride : it, rank);
       float held[PLANES > 1 ? 64 : 1];  // sums of the finished accumulations (bn <= 128: 64 columns at most)
       if (PLANES > 1) {
@@ -598,6 +600,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
       const int valid_rows = KIND == kWeights ? min(kBM, a.m - t.m0) : t.rows;
       void* out = a.out;
       int dt = a.out_dt, vec = a.vec;
+      const bool wide = packed && t.slot < 0;
       if (KIND == kWeights && t.slot >= 0) {
         out = a.part;
         dt = GMMXX_FLOAT32;
@@ -607,7 +610,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
       int64_t at[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int r = row0 + r8 + 4 * i;
+        const int r = row0 + (wide ? r4 + 8 * i : r8 + 4 * i);
         if (KIND == kRows) at[i] = slot_of[i] < 0 ? -1 : (int64_t)slot_of[i] * a.ldo;
         else if (r >= valid_rows) at[i] = -1;
         else if (KIND == kWeights && t.slot >= 0) at[i] = ((int64_t)t.slot * a.m + t.m0 + r) * a.n;
@@ -651,6 +654,46 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
           for (int i = 0; i < 32; ++i) v[i] = 0.f;
         }
         if (nv <= 0) continue;
+        if (PLANES == 1 && KIND != kBatch && wide) {  // a.n is a multiple of 8
+          const bool biased = KIND == kRows && a.bias != nullptr && t.kb > 0;
+          const uint16_t* bias = static_cast<const uint16_t*>(a.bias) + (int64_t)t.g * a.n + t.n0 + c;
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            float* x = v + 8 * p;
+            if (biased && 8 * p < nv) {
+              const uint4 q = __ldg(reinterpret_cast<const uint4*>(bias + 8 * p));
+              const uint32_t u4[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+              for (int h = 0; h < 4; ++h) {
+                const float2 f = dt == GMMXX_BFLOAT16
+                                     ? make_float2(bf16lo_to_f32(u4[h]), bf16hi_to_f32(u4[h]))
+                                     : __half22float2(*reinterpret_cast<const __half2*>(&u4[h]));
+                x[2 * h] += f.x;
+                x[2 * h + 1] += f.y;
+              }
+            }
+            uint4 q;
+            if (dt == GMMXX_BFLOAT16) {
+              q = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+            } else {
+              const uint2 lo = half4(make_float4(x[0], x[1], x[2], x[3])), hi = half4(make_float4(x[4], x[5], x[6], x[7]));
+              q = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            }
+            // 64-byte rows: piece p of row r at piece p ^ (r / 2 % 4), free of bank conflicts both ways
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((p ^ ((lane >> 1) & 3)) << 4)) = q;
+          }
+          __syncwarp();
+          const int p = lane & 3;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = r4 + 8 * i;
+            const uint4 q = *reinterpret_cast<const uint4*>(stage + r * 64 + ((p ^ ((r >> 1) & 3)) << 4));
+            if (at[i] >= 0 && 8 * p < nv)
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at[i] + t.n0 + c + 8 * p) = q;
+          }
+          __syncwarp();
+          continue;
+        }
         stage_row(stage, lane, v);
         if (KIND == kBatch && PLANES > 1) fetch();  // later: the sums hold the registers
         __syncwarp();
@@ -729,17 +772,21 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
     // in flight: each of these loads waits for the one before.
     Tile t{};
     if (first < total) t = decode<KIND, CG>(a, first, rank);
-    int next[kR];
-    auto first_rows = [&](const Tile& u) {
+    int next[kR], after[KIND == kWeights ? kR : 1];  // kWeights: the stage after the next as well
+    auto rows_of = [&](const Tile& u, int kb, int* to) {
 #pragma unroll
       for (int i = 0; i < kR; ++i) {
-        const int r = r0 + kStep * i;
-        next[i] = u.kb > 0 && r < u.rows ? __ldg(a.order + u.pos + r) : 0;
+        const int r = kb * kBlockK + r0 + kStep * i;
+        to[i] = u.kb > 0 && r < u.rows ? __ldg(a.order + u.pos + r) : 0;
       }
     };
+    auto first_rows = [&](const Tile& u) {
+      rows_of(u, 0, next);
+      if (KIND == kWeights) rows_of(u, 1, after);
+    };
     first_rows(t);
-    for (int64_t it = first; ok && it < total; it += stride) {
-      const int64_t ahead = it + stride < total ? it + stride : it;
+    for (int it = first; ok && it < total; it += stride) {
+      const int ahead = it + stride < total ? it + stride : it;
       Tile u = t;
       if (t.kb == 0) {
         t = decode<KIND, CG>(a, ahead, rank);
@@ -759,8 +806,9 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
           for (int i = 0; i < kR; ++i) {
             src[i] = a.src_a + ((int64_t)(next[i] / a.div_a) * a.ld_a + q * 8 + t.m0) * 2;
             src[kR + i] = a.src_b + ((int64_t)(next[i] / a.div_b) * a.ld_b + q * 8 + nb) * 2;
-            if (!last) next[i] = __ldg(a.order + t.pos + min((kb + 1) * kBlockK + r0 + kStep * i, t.rows - 1));
+            next[i] = after[KIND == kWeights ? i : 0];
           }
+          rows_of(t, kb + 2, after);
         }
         ok = wait_phase_warp(&bars.empty[s], ring.phase ^ 1, abort);
         if (!ok) break;
@@ -894,6 +942,8 @@ int launch_product(Kind kind, int planes, int pair, const ProductMaps& maps, con
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
   const int64_t tiles = std::max<int64_t>(1, max_items * a.mt * a.nt);
+  if (tiles >= (1ll << 31) - 1024)
+    return set_error(GMMXX_ERR_UNSUPPORTED, "%lld output tiles: their numbers are 32-bit", (long long)tiles);
   const unsigned grid = (unsigned)(std::min<int64_t>(sms / pair, tiles) * pair);
   if (pair == 2) {
     if (kind == kRows) return launch_one<kRows, 1, 2>(maps, a, grid, st);

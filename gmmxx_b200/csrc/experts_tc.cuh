@@ -28,7 +28,7 @@ struct ProductArgs {
   int mt, nt;      // tiles along m and n
   int a_mn, b_mn;  // operand contiguous along M / N instead of K
   uint32_t idesc;  // tcgen05 instruction descriptor (types, majors, M = 128, N = bn)
-  int64_t items;   // kBatch: matrices; otherwise read from the tables
+  int items;       // kBatch: matrices; otherwise read from the tables
   // routing
   const int32_t* order;
   const char *src_a, *src_b;  // 16-bit rows fetched by cp.async (one plane): 16-byte aligned,
@@ -42,7 +42,8 @@ struct ProductArgs {
   int out_dt;
   int64_t ldo;           // elements between rows of out
   int64_t out_stride;    // elements between matrices of out (kWeights, kBatch)
-  int vec;               // 16-byte stores allowed
+  int vec;               // stores of four elements allowed
+  int packed;            // 16-bit results (and bias) whose rows are multiples of 16 bytes: 16-byte stores
   const void* bias;
   int bias_dt;
   float* part;           // kWeights: fp32 partials of split groups
