@@ -573,6 +573,7 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
   ws += al256(p.max_slots * n_out * 4);
   segments_kernel<<<1, 1024, 0, st>>>(g.offsets, g.K, (int)p.seg, table, split);
   if (int rc = check_launch("segments_kernel")) return rc;
+  bool summed = false;
   if (gw != nullptr) {
     if (int rc = routed(dt, x, g.rows, n_in, g, g.top, ws, &px, st)) return rc;
     // (n_in x n_out) = x^T gy; for a transposed weight (n_out x n_in) = gy^T x
@@ -589,7 +590,13 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
     a.m = (int)m;
     a.n = (int)n;
     a.bn = bn;
-    a.stages = product_stages(planes, bn, pair);
+    // Columns of at most 128: the rows' memory bounds the launch and the tensor core is idle, so that the bias's
+    // gradient comes with it (500,009 x 128: 66 us less than reading the gathered rows once more)
+    if (gb != nullptr && !wt && planes == 1 && pair == 1 && bn <= 128) {
+      a.gb = gb;
+      a.part_b = part_b;
+    }
+    a.stages = product_stages(planes, bn, pair, a.gb != nullptr);
     a.mt = (int)ceil_div(m, 128 * pair);
     a.nt = (int)ceil_div(n, bn);
     a.a_mn = a.b_mn = 1;
@@ -617,11 +624,14 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
       join_kernel<<<148 * 8, 256, 0, st>>>(table, split, part, m * n, gw, dt);
       if (int rc = check_launch("join_kernel")) return rc;
     }
+    summed = a.gb != nullptr;
   }
   if (gb != nullptr) {
-    const dim3 grid((unsigned)ceil_div(n_out, 128), (unsigned)std::min<int64_t>(65535, p.max_segs));
-    bias_kernel<<<grid, 256, 0, st>>>(table, g.order, gy, dt, (int)n_out, n_out % 8 == 0, part_b, gb);
-    if (int rc = check_launch("bias_kernel")) return rc;
+    if (!summed) {
+      const dim3 grid((unsigned)ceil_div(n_out, 128), (unsigned)std::min<int64_t>(65535, p.max_segs));
+      bias_kernel<<<grid, 256, 0, st>>>(table, g.order, gy, dt, (int)n_out, n_out % 8 == 0, part_b, gb);
+      if (int rc = check_launch("bias_kernel")) return rc;
+    }
     if (p.max_split > 0) {
       join_kernel<<<148, 256, 0, st>>>(table, split, part_b, n_out, gb, dt);
       if (int rc = check_launch("join_kernel")) return rc;

@@ -298,7 +298,11 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
   volatile int* abort = &bars.abort;
   // two buffers of one accumulator, or of two (leading products, others)
   constexpr int kAccs = PLANES > 1 ? 2 : 1;
-  const uint32_t tmem_cols = 2 * kAccs * a.bn;  // a power of two of at least 32
+  // kWeights with the bias's gradient: two more for the column sums of B, products with an A of ones
+  constexpr bool kSums = KIND == kWeights && PLANES == 1 && CG == 1;
+  const bool sums_too = kSums && a.gb != nullptr;
+  char* ones = sm + a.stages * stage_bytes + kEpiWarps * kStageEpi;
+  const uint32_t tmem_cols = (sums_too ? 4 : 2 * kAccs) * a.bn;  // a power of two of at least 32
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
@@ -314,6 +318,12 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
     fence_barrier_init();
   }
   if (warp == 2) tmem_take<CG>(&bars.tmem_base, tmem_cols);
+  if (sums_too) {
+    const uint32_t one = a.out_dt == GMMXX_BFLOAT16 ? 0x3f803f80u : 0x3c003c00u;
+    for (int i = threadIdx.x; i < kABytes / 16; i += R::kThreads)
+      *reinterpret_cast<uint4*>(ones + i * 16) = make_uint4(one, one, one, one);
+    fence_proxy_async();
+  }
   block_or_pair_sync<CG>();
   tmem_fence_after();
   const uint32_t tmem = bars.tmem_base;
@@ -382,6 +392,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
       const uint64_t desc_b = a.b_mn ? desc_mnmajor(sb0, 8192) : desc_kmajor(sb0);
       const uint32_t stage_units = (uint32_t)stage_bytes >> 4;
       const uint32_t idesc = a.idesc;
+      const uint64_t desc_ones = kSums ? desc_mnmajor(smem_u32(ones), 8192) : 0;
       uint64_t* there = R::kRelay ? bars.ready : bars.full;
       Tile t{};
       if (first < total) t = decode<KIND, CG>(a, first, rank);
@@ -394,7 +405,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
         ok = wait_phase_warp(&bars.accempty[sums.i], sums.phase ^ 1, abort);
         if (!ok) break;
         tmem_fence_after();
-        const uint32_t d = tmem + sums.i * a.bn;
+        const uint32_t d = tmem + sums.i * a.bn, d_sums = tmem + (2 + sums.i) * a.bn;
         Tile u = t;
         for (int kb = 0; kb < t.kb; ++kb, ++use) {
           if (!peeked) ok = wait_phase_warp(&there[ring.i], ring.phase, abort);
@@ -418,12 +429,17 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
             if (elect_one()) {
               mma_16<CG>(d, da + 2 * step_a, db + 2 * step_b, idesc, 1);
               mma_16<CG>(d, da + 3 * step_a, db + 3 * step_b, idesc, 1);
+              if (kSums && sums_too && t.m0 == 0)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mma_16<CG>(d_sums, desc_ones, db + k * step_b, idesc, (kb | k) != 0);
               commit<CG>(done);
               if (last) commit<CG>(&bars.accfull[sums.i]);
             }
           } else {
             if (elect_one()) {
               for (int k = 0; k < steps; ++k) mma_16<CG>(d, da + k * step_a, db + k * step_b, idesc, (kb | k) != 0);
+              if (kSums && sums_too && t.m0 == 0)
+                for (int k = 0; k < steps; ++k) mma_16<CG>(d_sums, desc_ones, db + k * step_b, idesc, (kb | k) != 0);
               commit<CG>(done);
               if (last) commit<CG>(&bars.accfull[sums.i]);
             }
@@ -506,19 +522,21 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
         }
         tmem_fence_after();
         if (elect_one()) {
-          constexpr int kPairs = PLANES == 1 ? 1 : PLANES == 2 ? 3 : 6;
+          // A's leading plane takes B's first two at once: they lie one behind the other, as do the two
+          // accumulators, and a product of 2 x 128 columns takes hardly longer than one of 128 (128 cycles to ~114)
+          constexpr int kPairs = PLANES == 2 ? 2 : 5;
 #pragma unroll
           for (int c = 0; c < kPairs; ++c) {
-            constexpr int pa[6] = {0, 0, 1, 1, 0, 2}, pb[6] = {0, 1, 0, 1, 2, 0};
+            constexpr int pa[5] = {0, 1, 1, 0, 2}, pb[5] = {0, 0, 1, 2, 0};
             const uint64_t da = desc_a + (uint32_t)s * stage_units + pa[c] * (kABytes >> 4);
             const uint64_t db = desc_b + (uint32_t)s * stage_units + pb[c] * b_units;
-            const uint32_t dc = c == 0 ? d : d + a.bn;
-            const bool add = in_sum != 0 || c > 1;
+            const uint32_t dc = c == 0 ? d : d + a.bn, shape = c == 0 ? idesc + ((uint32_t)(a.bn >> 3) << 17) : idesc;
+            const bool add = in_sum != 0 || c > 0;
             if (steps == 4) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) mma_16<CG>(dc, da + k * step_a, db + k * step_b, idesc, k != 0 || add);
+              for (int k = 0; k < 4; ++k) mma_16<CG>(dc, da + k * step_a, db + k * step_b, shape, k != 0 || add);
             } else {
-              for (int k = 0; k < steps; ++k) mma_16<CG>(dc, da + k * step_a, db + k * step_b, idesc, k != 0 || add);
+              for (int k = 0; k < steps; ++k) mma_16<CG>(dc, da + k * step_a, db + k * step_b, shape, k != 0 || add);
             }
           }
           mma_commit(&bars.empty[s]);
@@ -554,10 +572,19 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
         if (i < 4 || !packed) slot_of[i] = r < u.rows ? __ldg(a.order + u.pos + r) : -1;
       }
     };
+    // a tile's bias into L1 while the tile before it is stored
+    auto fetch_bias = [&](const Tile& u) {
+      if (KIND != kRows || a.bias == nullptr || u.g >= a.groups) return;
+      const int c = u.n0 + lane * 32;  // a lane per 64 or 128 bytes
+      if (lane * 32 >= a.bn || c >= a.n) return;
+      const char* p = static_cast<const char*>(a.bias) + ((int64_t)u.g * a.n + c) * (a.bias_dt == GMMXX_FLOAT32 ? 4 : 2);
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
+    };
     Tile t{};
     if (first < total) {
       t = decode<KIND, CG>(a, first, rank);
       fetch_rows(t);
+      fetch_bias(t);
     }
     Tile u = t;
     for (int it = first; ok && it < total; it += stride, t = u) {
@@ -617,6 +644,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
         else at[i] = t.g * a.out_stride + (int64_t)(t.m0 + r) * a.ldo;
       }
       fetch_rows(u);
+      fetch_bias(u);
 #pragma unroll
       for (int j = 0; j < (PLANES > 1 ? 2 : 4); ++j) {
         const int c = c_lo + 32 * j;
@@ -636,6 +664,22 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
                                               : make_uint2(0, 0);
         };
         if (KIND == kBatch && PLANES == 1) fetch();
+        if (kSums && sums_too && t.m0 == 0 && (w & 3) == 0) {  // every row of the column sums is the same: one column per lane
+          float x = 0.f;
+          __syncwarp();
+          if (t.kb > 0) {
+            float v[32];
+            tmem_ld32(tmem + (2 + buf) * a.bn + c, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x = lane == i ? v[i] : x;
+          }
+          if (lane < nv) {
+            const int col = t.n0 + c + lane;
+            if (t.slot >= 0) a.part_b[(int64_t)t.slot * a.n + col] = x;
+            else store_y(a.gb, (int64_t)t.g * a.n + col, a.out_dt, x);
+          }
+        }
         float v[32];
         __syncwarp();
         if (PLANES > 1) {
@@ -886,7 +930,8 @@ int encode(CUtensorMap* map, const void* base, int fp16, int rank, const cuuint6
 template <int KIND, int PLANES, int CG>
 int launch_one(const ProductMaps& maps, const ProductArgs& a, unsigned grid, cudaStream_t st) {
   using R = Roles<KIND, PLANES, CG>;
-  const int smem = a.stages * PLANES * (kABytes + a.bn / CG * 128) + kEpiWarps * kStageEpi + 1024;
+  const int smem = a.stages * PLANES * (kABytes + a.bn / CG * 128) + kEpiWarps * kStageEpi + 1024 +
+                   (a.gb != nullptr ? kABytes : 0);
   const auto kern = product_kernel<KIND, PLANES, CG>;
   static SmemGrants grants;
   if (int rc = allow_smem((const void*)kern, kSmemLimit - 1024, grants)) return rc;
@@ -922,8 +967,9 @@ int encode_stack(CUtensorMap* map, const void* base, int fp16, int64_t cols, int
   return encode(map, base, fp16, 3, dims, strides, box);
 }
 
-int product_stages(int planes, int bn, int pair) {
-  return std::min(kMaxStages, (kSmemLimit - 2048 - kEpiWarps * kStageEpi) / (planes * (kABytes + bn / pair * 128)));
+int product_stages(int planes, int bn, int pair, int sums) {
+  const int fixed = 2048 + kEpiWarps * kStageEpi + (sums ? kABytes : 0);
+  return std::min(kMaxStages, (kSmemLimit - fixed) / (planes * (kABytes + bn / pair * 128)));
 }
 
 int device_sms(int* sms) {

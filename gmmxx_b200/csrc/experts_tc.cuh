@@ -47,6 +47,8 @@ struct ProductArgs {
   const void* bias;
   int bias_dt;
   float* part;           // kWeights: fp32 partials of split groups
+  void* gb;              // kWeights, one plane, no pair, bn <= 128: column sums of B as well (or NULL) ...
+  float* part_b;         // ... and their partials
   // kBatch epilogue: v = beta * e + alpha * acc / kPlaneScale, to planes o or (out != NULL) to out / kPlaneScale
   const __half* e[2];
   __half* o[2];
@@ -109,7 +111,7 @@ __host__ __device__ inline uint32_t product_idesc(int fp16, int bn, int a_mn, in
   return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
          ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(128 * pair >> 4) << 24);
 }
-int product_stages(int planes, int bn, int pair);
+int product_stages(int planes, int bn, int pair, int sums = 0);
 int launch_product(Kind kind, int planes, int pair, const ProductMaps& maps, const ProductArgs& a, int64_t max_items,
                    cudaStream_t st);
 int device_sms(int* sms);
