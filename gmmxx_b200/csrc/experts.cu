@@ -679,7 +679,7 @@ int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_
   const bool wide = m <= n;
   const int max_bn = s.planes == 1 ? 256 : 128;
   auto product = [&](const Stack& A, bool a_mn, const Stack& B, bool b_mn, int64_t rows, int64_t cols, int64_t k,
-                     float alpha, float beta, const Stack* E, const Stack& O, void* out) {
+                     float alpha, float beta, const Stack* E, const Stack& O, bool sym, void* out) {
     const int bn = tile_columns(batch * ceil_div(rows, 128), cols, s.planes, max_bn);
     const int pair = rows > 128 ? pair_of(s.planes, bn, batch * ceil_div(rows, 256) * ceil_div(cols, bn)) : 1;
     ProductMaps maps;
@@ -697,6 +697,12 @@ int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_
     t.b_mn = b_mn;
     t.idesc = product_idesc(1, bn, a_mn, b_mn, pair);
     t.items = (int)batch;
+    t.sym = sym;
+    t.per = t.mt * t.nt;
+    if (sym) {
+      t.per = 0;
+      for (int mi = 0; mi < t.mt; ++mi) t.per += t.nt - mi * pair * 128 / bn;
+    }
     t.alpha = alpha / kPlaneScale;
     t.beta = beta;
     for (int i = 0; i < s.planes; ++i) {
@@ -709,18 +715,19 @@ int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_
     t.out_dt = dt;
     t.ldo = cols;
     t.out_stride = rows * cols;
-    t.vec = vec_ok(out, dt, cols) && vec_ok(out, dt, rows * cols);
+    t.vec = vec_ok(out, dt, cols);
+    t.packed = packed_ok(out, dt, cols);
     return launch_product(kBatch, s.planes, pair, maps, t, batch, st);
   };
   for (int i = 0; i < steps; ++i) {
     void* out = i == steps - 1 ? q : nullptr;
-    if (int rc = wide ? product(X, false, X, false, s.lo, s.lo, s.hi, 1.f, 0.f, nullptr, P, nullptr)
-                      : product(X, true, X, true, s.lo, s.lo, s.hi, 1.f, 0.f, nullptr, P, nullptr))
+    if (int rc = wide ? product(X, false, X, false, s.lo, s.lo, s.hi, 1.f, 0.f, nullptr, P, true, nullptr)
+                      : product(X, true, X, true, s.lo, s.lo, s.hi, 1.f, 0.f, nullptr, P, true, nullptr))
       return rc;
     // P is symmetric: its rows serve as the columns of the second factor
-    if (int rc = product(P, false, P, false, s.lo, s.lo, s.lo, c, b, &P, Q, nullptr)) return rc;
-    if (int rc = wide ? product(Q, false, X, true, m, n, s.lo, 1.f, a, &X, Y, out)
-                      : product(X, false, Q, false, m, n, s.lo, 1.f, a, &X, Y, out))
+    if (int rc = product(P, false, P, false, s.lo, s.lo, s.lo, c, b, &P, Q, true, nullptr)) return rc;
+    if (int rc = wide ? product(Q, false, X, true, m, n, s.lo, 1.f, a, &X, Y, false, out)
+                      : product(X, false, Q, false, m, n, s.lo, 1.f, a, &X, Y, false, out))
       return rc;
     std::swap(X, Y);
   }

@@ -191,18 +191,37 @@ struct Tile {
   int rows;    // kRows: rows of the tile; kWeights: rows of the segment; kBatch: rows of the tile
   int m0, n0;
   int slot;    // kWeights: partial slot or -1
+  bool mirror; // kBatch, symmetric result: the tile's transpose is stored too
   int kb;      // contraction stages; 0: the result is zero
 };
 
 template <int KIND>
 __device__ __forceinline__ int tile_count(const ProductArgs& a) {  // below 2^31: checked before the launch
-  return (KIND == kBatch ? a.items : __ldg(a.count)) * a.mt * a.nt;
+  return KIND == kBatch ? a.items * a.per : __ldg(a.count) * a.mt * a.nt;
 }
 
 // this block's part (its 128 rows) of tile `it` of CG * 128 rows
 template <int KIND, int CG>
 __device__ __forceinline__ Tile decode(const ProductArgs& a, int it, int rank) {
   Tile t;
+  t.mirror = false;
+  if (KIND == kBatch && a.sym) {  // rows of tiles that start at the diagonal's
+    t.g = it / a.per;
+    it -= t.g * a.per;
+    int mi = 0, lo = 0;
+    while (it >= a.nt - lo) {
+      it -= a.nt - lo;
+      lo = ++mi * CG * kBM / a.bn;
+    }
+    t.n0 = (lo + it) * a.bn;
+    t.mirror = t.n0 >= (mi + 1) * CG * kBM;
+    t.m0 = (mi * CG + rank) * kBM;
+    t.pos = 0;
+    t.rows = min(kBM, a.m - t.m0);
+    t.slot = -1;
+    t.kb = (a.k + kBlockK - 1) / kBlockK;
+    return t;
+  }
   t.n0 = it % a.nt * a.bn;
   it /= a.nt;
   if (KIND == kRows) {
@@ -251,14 +270,17 @@ __device__ __forceinline__ float staged1(const char* st, int row, int c) {
   return *reinterpret_cast<const float*>(st + row * 128 + (((c >> 2) ^ (row & 7)) << 4) + (c & 3) * 4);
 }
 
+// The same of 16-bit values, 64-byte rows: piece p (8 values) of row r at piece p ^ (r / 2 % 4)
+__device__ __forceinline__ void put_piece(char* st, int r, int p, uint4 q) {
+  *reinterpret_cast<uint4*>(st + r * 64 + ((p ^ ((r >> 1) & 3)) << 4)) = q;
+}
+__device__ __forceinline__ uint4 get_piece(const char* st, int r, int p) {
+  return *reinterpret_cast<const uint4*>(st + r * 64 + ((p ^ ((r >> 1) & 3)) << 4));
+}
+
 __device__ __forceinline__ uint2 half4(float4 v) {
   const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
   return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-}
-__device__ __forceinline__ float4 float4_of(uint2 q) {
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&q.x));
-  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&q.y));
-  return make_float4(a.x, a.y, b.x, b.y);
 }
 
 // 4 values to out[at ..], aligned to 4 elements
@@ -561,15 +583,16 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
     // routed, the next tile's place is fetched while this one's products run: table, then order.
     const int row0 = (w & 3) * 32, r8 = lane >> 3, c4 = (lane & 7) * 4;
     // 16-bit results go 16 bytes per lane: rows lane / 4 + 8 i, four lanes per row.
-    const bool packed = PLANES == 1 && KIND != kBatch && a.packed;
-    const int r4 = lane >> 2;
+    const bool packed = PLANES == 1 && a.packed;
+    const int r4 = lane >> 2, p4 = lane & 3;
     int slot_of[KIND == kRows ? 8 : 1];
     auto fetch_rows = [&](const Tile& u) {
-      if (KIND != kRows) return;
+      if constexpr (KIND == kRows) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = row0 + (packed ? r4 + 8 * i : r8 + 4 * i);
-        if (i < 4 || !packed) slot_of[i] = r < u.rows ? __ldg(a.order + u.pos + r) : -1;
+        for (int i = 0; i < 8; ++i) {
+          const int r = row0 + (packed ? r4 + 8 * i : r8 + 4 * i);
+          if (i < 4 || !packed) slot_of[i] = r < u.rows ? __ldg(a.order + u.pos + r) : -1;
+        }
       }
     };
     // a tile's bias into L1 while the tile before it is stored
@@ -650,20 +673,19 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
         const int c = c_lo + 32 * j;
         if (c >= c_hi) break;
         const int nv = n_left - c;  // columns left from c
-        // the planes to add, fetched while the accumulator is read
-        uint2 e[KIND == kBatch ? PLANES : 1][KIND == kBatch ? 8 : 1];
-        int64_t pat = 0;
-        auto fetch = [&]() {
-          pat = t.g * a.p_stride + (int64_t)(t.m0 + row0 + r8) * a.ldp + t.n0 + c + c4;
-          if (a.e[0] == nullptr) return;
+        // kBatch: the planes to add, 16 bytes per lane (rows r4 + 8 i, four lanes per row), fetched while the
+        // accumulator is read
+        uint4 e[KIND == kBatch ? PLANES : 1][KIND == kBatch ? 4 : 1];
+        const int64_t pat = KIND != kBatch ? 0 : t.g * a.p_stride + (int64_t)(t.m0 + row0 + r4) * a.ldp + t.n0 + c + p4 * 8;
+        if (KIND == kBatch && a.e[0] != nullptr && nv > 0) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int p = 0; p < PLANES; ++p)  // ldp is a multiple of 8: whole pieces, their tail is not used
-              e[p][i] = at[i] >= 0 && c4 < nv ? *reinterpret_cast<const uint2*>(a.e[p] + pat + 4 * i * a.ldp)
-                                              : make_uint2(0, 0);
-        };
-        if (KIND == kBatch && PLANES == 1) fetch();
+              e[p][i] = row0 + r4 + 8 * i < t.rows && 8 * p4 < nv
+                            ? *reinterpret_cast<const uint4*>(a.e[p] + pat + 8 * i * a.ldp)
+                            : make_uint4(0, 0, 0, 0);
+        }
         if (kSums && sums_too && t.m0 == 0 && (w & 3) == 0) {  // every row of the column sums is the same: one column per lane
           float x = 0.f;
           __syncwarp();
@@ -698,7 +720,72 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
           for (int i = 0; i < 32; ++i) v[i] = 0.f;
         }
         if (nv <= 0) continue;
-        if (PLANES == 1 && KIND != kBatch && wide) {  // a.n is a multiple of 8
+        if (KIND == kBatch) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] *= a.alpha;
+          if (a.e[0] != nullptr) {
+#pragma unroll
+            for (int p = PLANES - 1; p >= 0; --p) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) put_piece(stage, r4 + 8 * i, p4, e[p][i]);
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint4 q = get_piece(stage, lane, i);
+                const uint32_t u4[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u4[h]));
+                  v[8 * i + 2 * h] = fmaf(a.beta, f.x, v[8 * i + 2 * h]);
+                  v[8 * i + 2 * h + 1] = fmaf(a.beta, f.y, v[8 * i + 2 * h + 1]);
+                }
+              }
+              __syncwarp();
+            }
+          }
+          if (a.out == nullptr) {  // planes
+#pragma unroll
+            for (int p = 0; p < PLANES; ++p) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint32_t u4[4];
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                  float& x = v[8 * i + 2 * h];
+                  float& y = v[8 * i + 2 * h + 1];
+                  const __half2 q = __floats2half2_rn(x, y);
+                  u4[h] = *reinterpret_cast<const uint32_t*>(&q);
+                  if (t.mirror) {
+                    // lanes are rows of one column: neighbours swap, so that each has two rows of one column,
+                    // and half a warp writes 64 bytes along a row of the transpose
+                    const uint32_t other = __shfl_xor_sync(0xffffffffu, u4[h], 1);
+                    const uint32_t pair = lane & 1 ? (other >> 16) | (u4[h] & 0xffff0000u)
+                                                   : (u4[h] & 0xffffu) | (other << 16);
+                    const int cc = 8 * i + 2 * h + (lane & 1), r = row0 + (lane & ~1);
+                    if (cc < nv && r < t.rows)
+                      *reinterpret_cast<uint32_t*>(a.o[p] + t.g * a.p_stride + (int64_t)(t.n0 + c + cc) * a.ldp + t.m0 + r) = pair;
+                  }
+                  if (PLANES > 1) {
+                    const float2 f = __half22float2(q);
+                    x -= f.x;
+                    y -= f.y;
+                  }
+                }
+                put_piece(stage, lane, i, make_uint4(u4[0], u4[1], u4[2], u4[3]));
+              }
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (row0 + r4 + 8 * i < t.rows && 8 * p4 < nv)
+                  *reinterpret_cast<uint4*>(a.o[p] + pat + 8 * i * a.ldp) = get_piece(stage, r4 + 8 * i, p4);
+              __syncwarp();
+            }
+            continue;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] *= 1.f / kPlaneScale;
+        }
+        if (PLANES == 1 && wide) {  // a.n is a multiple of 8
           const bool biased = KIND == kRows && a.bias != nullptr && t.kb > 0;
           const uint16_t* bias = static_cast<const uint16_t*>(a.bias) + (int64_t)t.g * a.n + t.n0 + c;
 #pragma unroll
@@ -723,81 +810,39 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
               const uint2 lo = half4(make_float4(x[0], x[1], x[2], x[3])), hi = half4(make_float4(x[4], x[5], x[6], x[7]));
               q = make_uint4(lo.x, lo.y, hi.x, hi.y);
             }
-            // 64-byte rows: piece p of row r at piece p ^ (r / 2 % 4), free of bank conflicts both ways
-            *reinterpret_cast<uint4*>(stage + lane * 64 + ((p ^ ((lane >> 1) & 3)) << 4)) = q;
+            put_piece(stage, lane, p, q);
           }
           __syncwarp();
-          const int p = lane & 3;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int r = r4 + 8 * i;
-            const uint4 q = *reinterpret_cast<const uint4*>(stage + r * 64 + ((p ^ ((r >> 1) & 3)) << 4));
-            if (at[i] >= 0 && 8 * p < nv)
-              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at[i] + t.n0 + c + 8 * p) = q;
+            const uint4 q = get_piece(stage, r4 + 8 * i, p4);
+            if (at[i] >= 0 && 8 * p4 < nv)
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at[i] + t.n0 + c + 8 * p4) = q;
           }
           __syncwarp();
           continue;
         }
         stage_row(stage, lane, v);
-        if (KIND == kBatch && PLANES > 1) fetch();  // later: the sums hold the registers
         __syncwarp();
-        if (KIND == kBatch) {
+        const bool biased = KIND == kRows && a.bias != nullptr && t.kb > 0;
+        const int64_t b0 = (int64_t)t.g * a.n + t.n0 + c;
+        if (vec) {  // a.n is a multiple of 4: a piece of four columns is whole or absent
+          float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (biased && c4 < nv)
+            b = make_float4(load_x(a.bias, b0 + c4, a.bias_dt), load_x(a.bias, b0 + c4 + 1, a.bias_dt),
+                            load_x(a.bias, b0 + c4 + 2, a.bias_dt), load_x(a.bias, b0 + c4 + 3, a.bias_dt));
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            float4 x = staged4(stage, r8 + 4 * i, lane & 7);
-            x = make_float4(x.x * a.alpha, x.y * a.alpha, x.z * a.alpha, x.w * a.alpha);
-            if (a.e[0] != nullptr) {
-#pragma unroll
-              for (int p = PLANES - 1; p >= 0; --p) {
-                const float4 f = float4_of(e[p][i]);
-                x = make_float4(fmaf(a.beta, f.x, x.x), fmaf(a.beta, f.y, x.y), fmaf(a.beta, f.z, x.z),
-                                fmaf(a.beta, f.w, x.w));
-              }
-            }
-            if (at[i] < 0 || c4 >= nv) continue;
-            if (a.out != nullptr) {
-              constexpr float down = 1.f / kPlaneScale;
-              x = make_float4(x.x * down, x.y * down, x.z * down, x.w * down);
-              const int64_t o = at[i] + t.n0 + c + c4;
-              if (vec) {
-                store4(out, dt, o, x);
-              } else {
-                store_y(out, o, dt, x.x);
-                if (c4 + 1 < nv) store_y(out, o + 1, dt, x.y);
-                if (c4 + 2 < nv) store_y(out, o + 2, dt, x.z);
-                if (c4 + 3 < nv) store_y(out, o + 3, dt, x.w);
-              }
-            } else {
-              const uint2 hi = half4(x);
-              *reinterpret_cast<uint2*>(a.o[0] + pat + 4 * i * a.ldp) = hi;
-              if (PLANES > 1) {
-                const float4 f = float4_of(hi);
-                *reinterpret_cast<uint2*>(a.o[1] + pat + 4 * i * a.ldp) =
-                    half4(make_float4(x.x - f.x, x.y - f.y, x.z - f.z, x.w - f.w));
-              }
-            }
+            const float4 x = staged4(stage, r8 + 4 * i, lane & 7);
+            if (at[i] >= 0 && c4 < nv)
+              store4(out, dt, at[i] + t.n0 + c + c4, make_float4(x.x + b.x, x.y + b.y, x.z + b.z, x.w + b.w));
           }
-        } else {
-          const bool biased = KIND == kRows && a.bias != nullptr && t.kb > 0;
-          const int64_t b0 = (int64_t)t.g * a.n + t.n0 + c;
-          if (vec) {  // a.n is a multiple of 4: a piece of four columns is whole or absent
-            float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (biased && c4 < nv)
-              b = make_float4(load_x(a.bias, b0 + c4, a.bias_dt), load_x(a.bias, b0 + c4 + 1, a.bias_dt),
-                              load_x(a.bias, b0 + c4 + 2, a.bias_dt), load_x(a.bias, b0 + c4 + 3, a.bias_dt));
+        } else {  // a lane per column: whole lines although no row is aligned
+          const float b = biased && lane < nv ? load_x(a.bias, b0 + lane, a.bias_dt) : 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 x = staged4(stage, r8 + 4 * i, lane & 7);
-              if (at[i] >= 0 && c4 < nv)
-                store4(out, dt, at[i] + t.n0 + c + c4, make_float4(x.x + b.x, x.y + b.y, x.z + b.z, x.w + b.w));
-            }
-          } else {  // a lane per column: whole lines although no row is aligned
-            const float b = biased && lane < nv ? load_x(a.bias, b0 + lane, a.bias_dt) : 0.f;
-#pragma unroll
-            for (int r = 0; r < 32; ++r) {
-              const int64_t base = __shfl_sync(0xffffffffu, at[r >> 2], (r & 3) * 8);
-              if (base >= 0 && lane < nv) store_y(out, base + t.n0 + c + lane, dt, staged1(stage, r, lane) + b);
-            }
+          for (int r = 0; r < 32; ++r) {
+            const int64_t base = __shfl_sync(0xffffffffu, at[r >> 2], (r & 3) * 8);
+            if (base >= 0 && lane < nv) store_y(out, base + t.n0 + c + lane, dt, staged1(stage, r, lane) + b);
           }
         }
         __syncwarp();
@@ -987,7 +1032,7 @@ int launch_product(Kind kind, int planes, int pair, const ProductMaps& maps, con
                    cudaStream_t st) {
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
-  const int64_t tiles = std::max<int64_t>(1, max_items * a.mt * a.nt);
+  const int64_t tiles = std::max<int64_t>(1, max_items * (kind == kBatch ? a.per : (int64_t)a.mt * a.nt));
   if (tiles >= (1ll << 31) - 1024)
     return set_error(GMMXX_ERR_UNSUPPORTED, "%lld output tiles: their numbers are 32-bit", (long long)tiles);
   const unsigned grid = (unsigned)(std::min<int64_t>(sms / pair, tiles) * pair);

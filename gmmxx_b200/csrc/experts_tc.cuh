@@ -49,6 +49,8 @@ struct ProductArgs {
   float* part;           // kWeights: fp32 partials of split groups
   void* gb;              // kWeights, one plane, no pair, bn <= 128: column sums of B as well (or NULL) ...
   float* part_b;         // ... and their partials
+  // kBatch: tiles per matrix; sym: the result is symmetric, only the tiles on and above the diagonal are computed
+  int per, sym;
   // kBatch epilogue: v = beta * e + alpha * acc / kPlaneScale, to planes o or (out != NULL) to out / kPlaneScale
   const __half* e[2];
   __half* o[2];
