@@ -465,11 +465,61 @@ __global__ void __launch_bounds__(256) scale_kernel(int dt, const void* g, int64
   }
 }
 
+// Planes of the symmetric P = sum of its partial products (fp32, of value), in
+// order: 32 x 32 pieces on and above the diagonal (the tiles of 128 rows cover
+// them), each written to its own place and to its mirror image's.
+__global__ void __launch_bounds__(256) join_planes_kernel(const float* part, int shares, int64_t share, int lo, int ld,
+                                                          __half* hi, __half* low) {
+  __shared__ float tile[32][33];
+  const int64_t base = (int64_t)blockIdx.y * lo * ld;
+  int tr = 0, left = blockIdx.x, n = (lo + 31) / 32;
+  while (left >= n - tr) left -= n - tr++;
+  const int tc = tr + left, row = threadIdx.x >> 3, col = (threadIdx.x & 7) * 4;
+  auto store = [&](int r, int c, const float* v) {  // ld is a multiple of 8: a piece of four starts inside the row
+    if (r >= lo || c >= lo) return;
+    uint2 h, l;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const __half2 q = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+      const float2 f = __half22float2(q);
+      reinterpret_cast<__half2*>(&h)[j] = q;
+      reinterpret_cast<__half2*>(&l)[j] = __floats2half2_rn(v[2 * j] - f.x, v[2 * j + 1] - f.y);
+    }
+    const int64_t at = base + (int64_t)r * ld + c;
+    *reinterpret_cast<uint2*>(hi + at) = h;
+    if (low != nullptr) *reinterpret_cast<uint2*>(low + at) = l;
+  };
+  float v[4] = {};
+  const int r = tr * 32 + row, c = tc * 32 + col;
+  if (r < lo && c < lo) {
+    const float* p = part + base + (int64_t)r * ld + c;
+#pragma unroll 4
+    for (int s = 0; s < shares; ++s) {
+      const float4 x = *reinterpret_cast<const float4*>(p + s * share);
+      v[0] += x.x;
+      v[1] += x.y;
+      v[2] += x.z;
+      v[3] += x.w;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = c + j < lo ? v[j] * kPlaneScale : 0.f;  // behind the last column: not written
+  store(r, c, v);
+  if (tr == tc) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) tile[row][col + j] = v[j];
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = tile[col + j][row];
+  store(tc * 32 + row, tr * 32 + col, v);
+}
+
 struct NsPlan {
   int planes;
   int64_t lo, hi, ldx, ldp, x_plane, p_plane;  // bytes per plane
-  int64_t x, y, p, q, part, bytes;
+  int64_t x, y, p, q, part, shares, bytes;
   int nparts;
+  int ksplit, ksteps;  // shares of the long contraction of P = X X^T, where its tiles are few
 };
 
 // One fp16 plane per iterate where the result is rounded to bf16 and the short
@@ -491,6 +541,16 @@ NsPlan ns_plan(int dt, int64_t batch, int64_t m, int64_t n) {
   s.p = off; off += s.p_plane * s.planes;
   s.q = off; off += s.p_plane * s.planes;
   s.part = off; off += al256(batch * s.nparts * 8);
+  // a symmetric product of few tiles leaves SMs idle: as many shares of its contraction as fill them, of at least
+  // four stages (a share costs its partial's 4 bytes per element twice)
+  const int64_t steps = ceil_div(s.hi, kBlockK), mt = ceil_div(s.lo, 128), tiles = batch * mt * (mt + 1) / 2;
+  s.ksplit = 1;
+  s.ksteps = (int)steps;
+  if (tiles * 2 <= 148 && steps >= 8) {
+    s.ksteps = (int)std::max<int64_t>(4, ceil_div(steps, 148 / tiles));
+    s.ksplit = (int)ceil_div(steps, s.ksteps);
+  }
+  s.shares = off; off += s.ksplit > 1 ? al256(s.ksplit * batch * s.lo * s.ldp * 4) : 0;
   s.bytes = off;
   return s;
 }
@@ -677,11 +737,13 @@ int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_
   Stack X{ws + s.x, s.x_plane, m, n, s.ldx}, Y{ws + s.y, s.x_plane, m, n, s.ldx};
   const Stack P{ws + s.p, s.p_plane, s.lo, s.lo, s.ldp}, Q{ws + s.q, s.p_plane, s.lo, s.lo, s.ldp};
   const bool wide = m <= n;
-  const int max_bn = s.planes == 1 ? 256 : 128;
+  const int max_bn = s.planes == 1 ? 256 : 128, share_bn = s.lo <= 64 ? 64 : 128;
   auto product = [&](const Stack& A, bool a_mn, const Stack& B, bool b_mn, int64_t rows, int64_t cols, int64_t k,
-                     float alpha, float beta, const Stack* E, const Stack& O, bool sym, void* out) {
-    const int bn = tile_columns(batch * ceil_div(rows, 128), cols, s.planes, max_bn);
-    const int pair = rows > 128 ? pair_of(s.planes, bn, batch * ceil_div(rows, 256) * ceil_div(cols, bn)) : 1;
+                     float alpha, float beta, const Stack* E, const Stack& O, bool sym, void* out,
+                     int out_dt, bool shares) {
+    // shares: tiles of 128 x 128, each share of the contraction to its own fp32 result
+    const int bn = shares ? share_bn : tile_columns(batch * ceil_div(rows, 128), cols, s.planes, max_bn);
+    const int pair = rows > 128 && !shares ? pair_of(s.planes, bn, batch * ceil_div(rows, 256) * ceil_div(cols, bn)) : 1;
     ProductMaps maps;
     if (int rc = stack_operand(A, s.planes, batch, a_mn ? kBlockK : 128, maps.a)) return rc;
     if (int rc = stack_operand(B, s.planes, batch, b_mn ? kBlockK : bn / pair, maps.b)) return rc;
@@ -703,6 +765,8 @@ int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_
       t.per = 0;
       for (int mi = 0; mi < t.mt; ++mi) t.per += t.nt - mi * pair * 128 / bn;
     }
+    t.ksplit = shares ? s.ksplit : 1;
+    t.ksteps = shares ? s.ksteps : (int)ceil_div(k, kBlockK);
     t.alpha = alpha / kPlaneScale;
     t.beta = beta;
     for (int i = 0; i < s.planes; ++i) {
@@ -712,22 +776,31 @@ int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_
     t.ldp = O.ld;
     t.p_stride = O.rows * O.ld;
     t.out = out;
-    t.out_dt = dt;
-    t.ldo = cols;
-    t.out_stride = rows * cols;
-    t.vec = vec_ok(out, dt, cols);
-    t.packed = packed_ok(out, dt, cols);
+    t.out_dt = out_dt;
+    t.ldo = shares ? O.ld : cols;
+    t.out_stride = rows * t.ldo;
+    t.vec = vec_ok(out, out_dt, t.ldo);
+    t.packed = packed_ok(out, out_dt, t.ldo);
     return launch_product(kBatch, s.planes, pair, maps, t, batch, st);
   };
   for (int i = 0; i < steps; ++i) {
     void* out = i == steps - 1 ? q : nullptr;
-    if (int rc = wide ? product(X, false, X, false, s.lo, s.lo, s.hi, 1.f, 0.f, nullptr, P, true, nullptr)
-                      : product(X, true, X, true, s.lo, s.lo, s.hi, 1.f, 0.f, nullptr, P, true, nullptr))
+    const bool shares = s.ksplit > 1;
+    if (int rc = product(X, !wide, X, !wide, s.lo, s.lo, s.hi, 1.f, 0.f, nullptr, P, true,
+                         shares ? ws + s.shares : nullptr, shares ? GMMXX_FLOAT32 : dt, shares))
       return rc;
+    if (shares) {
+      const int64_t n32 = ceil_div(s.lo, 32);
+      join_planes_kernel<<<dim3((unsigned)(n32 * (n32 + 1) / 2), (unsigned)batch), 256, 0, st>>>(
+          reinterpret_cast<const float*>(ws + s.shares), s.ksplit, batch * s.lo * s.ldp, (int)s.lo, (int)s.ldp,
+          reinterpret_cast<__half*>(P.base),
+          s.planes > 1 ? reinterpret_cast<__half*>(P.base + P.plane) : nullptr);
+      if (int rc = check_launch("join_planes_kernel")) return rc;
+    }
     // P is symmetric: its rows serve as the columns of the second factor
-    if (int rc = product(P, false, P, false, s.lo, s.lo, s.lo, c, b, &P, Q, true, nullptr)) return rc;
-    if (int rc = wide ? product(Q, false, X, true, m, n, s.lo, 1.f, a, &X, Y, false, out)
-                      : product(X, false, Q, false, m, n, s.lo, 1.f, a, &X, Y, false, out))
+    if (int rc = product(P, false, P, false, s.lo, s.lo, s.lo, c, b, &P, Q, true, nullptr, dt, false)) return rc;
+    if (int rc = wide ? product(Q, false, X, true, m, n, s.lo, 1.f, a, &X, Y, false, out, dt, false)
+                      : product(X, false, Q, false, m, n, s.lo, 1.f, a, &X, Y, false, out, dt, false))
       return rc;
     std::swap(X, Y);
   }

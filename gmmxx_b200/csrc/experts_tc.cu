@@ -190,14 +190,14 @@ struct Tile {
   int pos;     // first position (routed)
   int rows;    // kRows: rows of the tile; kWeights: rows of the segment; kBatch: rows of the tile
   int m0, n0;
-  int slot;    // kWeights: partial slot or -1
+  int slot;    // kWeights: partial slot or -1; kBatch: share of the contraction, which starts at stage `pos`
   bool mirror; // kBatch, symmetric result: the tile's transpose is stored too
   int kb;      // contraction stages; 0: the result is zero
 };
 
 template <int KIND>
 __device__ __forceinline__ int tile_count(const ProductArgs& a) {  // below 2^31: checked before the launch
-  return KIND == kBatch ? a.items * a.per : __ldg(a.count) * a.mt * a.nt;
+  return KIND == kBatch ? a.items * a.per * a.ksplit : __ldg(a.count) * a.mt * a.nt;
 }
 
 // this block's part (its 128 rows) of tile `it` of CG * 128 rows
@@ -205,6 +205,13 @@ template <int KIND, int CG>
 __device__ __forceinline__ Tile decode(const ProductArgs& a, int it, int rank) {
   Tile t;
   t.mirror = false;
+  if (KIND == kBatch) {  // this tile's share of the contraction
+    const int ks = it % a.ksplit;
+    it /= a.ksplit;
+    t.slot = ks;
+    t.pos = ks * a.ksteps;
+    t.kb = min(a.ksteps, (a.k + kBlockK - 1) / kBlockK - t.pos);
+  }
   if (KIND == kBatch && a.sym) {  // rows of tiles that start at the diagonal's
     t.g = it / a.per;
     it -= t.g * a.per;
@@ -214,12 +221,9 @@ __device__ __forceinline__ Tile decode(const ProductArgs& a, int it, int rank) {
       lo = ++mi * CG * kBM / a.bn;
     }
     t.n0 = (lo + it) * a.bn;
-    t.mirror = t.n0 >= (mi + 1) * CG * kBM;
+    t.mirror = a.ksplit == 1 && t.n0 >= (mi + 1) * CG * kBM;
     t.m0 = (mi * CG + rank) * kBM;
-    t.pos = 0;
     t.rows = min(kBM, a.m - t.m0);
-    t.slot = -1;
-    t.kb = (a.k + kBlockK - 1) / kBlockK;
     return t;
   }
   t.n0 = it % a.nt * a.bn;
@@ -245,10 +249,7 @@ __device__ __forceinline__ Tile decode(const ProductArgs& a, int it, int rank) {
     t.kb = (t.rows + kBlockK - 1) / kBlockK;
   } else {
     t.g = it;
-    t.pos = 0;
     t.rows = min(kBM, a.m - t.m0);
-    t.slot = -1;
-    t.kb = (a.k + kBlockK - 1) / kBlockK;
   }
   return t;
 }
@@ -349,6 +350,12 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
   block_or_pair_sync<CG>();
   tmem_fence_after();
   const uint32_t tmem = bars.tmem_base;
+  if (KIND == kBatch) {
+    // A chain of short launches: let the next one set itself up on the SMs that this one leaves free, and wait
+    // here for all that the one before has written.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+  }
   const int total = tile_count<KIND>(a);
 
   if (R::kTma && warp == 0) {
@@ -372,7 +379,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
         uint64_t* bar = &bars.full[s];
         if (lane == 0) mbar_expect_tx(bar, bytes);
         __syncwarp();
-        const int k0 = kb * kBlockK, nb = t.n0 + rank * bcols;
+        const int k0 = (KIND == kBatch ? t.pos + kb : kb) * kBlockK, nb = t.n0 + rank * bcols;
 #pragma unroll
         for (int p = 0; p < PLANES; ++p) {
           char* pa = sa + p * kABytes;
@@ -650,7 +657,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
       const int valid_rows = KIND == kWeights ? min(kBM, a.m - t.m0) : t.rows;
       void* out = a.out;
       int dt = a.out_dt, vec = a.vec;
-      const bool wide = packed && t.slot < 0;
+      const bool wide = packed && (KIND == kBatch || t.slot < 0);
       if (KIND == kWeights && t.slot >= 0) {
         out = a.part;
         dt = GMMXX_FLOAT32;
@@ -664,7 +671,7 @@ __global__ void __launch_bounds__(Roles<KIND, PLANES, CG>::kThreads, 1)
         if (KIND == kRows) at[i] = slot_of[i] < 0 ? -1 : (int64_t)slot_of[i] * a.ldo;
         else if (r >= valid_rows) at[i] = -1;
         else if (KIND == kWeights && t.slot >= 0) at[i] = ((int64_t)t.slot * a.m + t.m0 + r) * a.n;
-        else at[i] = t.g * a.out_stride + (int64_t)(t.m0 + r) * a.ldo;
+        else at[i] = (KIND == kBatch ? t.g + (int64_t)t.slot * a.items : t.g) * a.out_stride + (int64_t)(t.m0 + r) * a.ldo;
       }
       fetch_rows(u);
       fetch_bias(u);
@@ -980,22 +987,29 @@ int launch_one(const ProductMaps& maps, const ProductArgs& a, unsigned grid, cud
   const auto kern = product_kernel<KIND, PLANES, CG>;
   static SmemGrants grants;
   if (int rc = allow_smem((const void*)kern, kSmemLimit - 1024, grants)) return rc;
-  if (CG == 1) {
+  if (CG == 1 && KIND != kBatch) {
     kern<<<grid, R::kThreads, smem, st>>>(maps, a);
     return check_launch("product_kernel");
   }
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (CG > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = CG;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  if (KIND == kBatch) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(R::kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = n;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, maps, a);
   if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "product_kernel launch: %s", cudaGetErrorString(e));
   return GMMXX_OK;
@@ -1032,7 +1046,7 @@ int launch_product(Kind kind, int planes, int pair, const ProductMaps& maps, con
                    cudaStream_t st) {
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
-  const int64_t tiles = std::max<int64_t>(1, max_items * (kind == kBatch ? a.per : (int64_t)a.mt * a.nt));
+  const int64_t tiles = std::max<int64_t>(1, max_items * (kind == kBatch ? (int64_t)a.per * a.ksplit : (int64_t)a.mt * a.nt));
   if (tiles >= (1ll << 31) - 1024)
     return set_error(GMMXX_ERR_UNSUPPORTED, "%lld output tiles: their numbers are 32-bit", (long long)tiles);
   const unsigned grid = (unsigned)(std::min<int64_t>(sms / pair, tiles) * pair);

@@ -51,6 +51,8 @@ struct ProductArgs {
   float* part_b;         // ... and their partials
   // kBatch: tiles per matrix; sym: the result is symmetric, only the tiles on and above the diagonal are computed
   int per, sym;
+  // and the contraction in ksplit shares of ksteps stages, share s of matrix z to out's matrix s * items + z
+  int ksplit, ksteps;
   // kBatch epilogue: v = beta * e + alpha * acc / kPlaneScale, to planes o or (out != NULL) to out / kPlaneScale
   const __half* e[2];
   __half* o[2];

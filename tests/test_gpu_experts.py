@@ -369,7 +369,7 @@ def _ns_check(q, g, steps=5, coef=(3.4445, -4.7750, 2.0315), eps=1e-7):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", [(1, 1, 1), (3, 1, 9), (2, 5, 3), (4, 64, 64), (3, 33, 100), (2, 130, 64),
                                    (1, 128, 128), (2, 129, 200), (1, 300, 257), (2, 256, 520), (1, 520, 256),
-                                   (24, 520, 776), (20, 1000, 536), (3, 60, 500), (2, 90, 250), (2, 250, 100),
+                                   (24, 520, 776), (20, 1000, 536), (1, 135, 1500), (2, 2000, 140), (1, 259, 900), (3, 60, 500), (2, 90, 250), (2, 250, 100),
                                    (260, 16, 16), (2, 3, 24, 40)])
 def test_orthogonalize(cuda_device, shape, dtype):
     import gmmxx_b200 as gm
