@@ -701,11 +701,10 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
 }
 
 int read_status(int* out, cudaStream_t st) {
-  int a = 0, b = 0, c = 0;
+  int a = 0, b = 0;
   if (int rc = product_status(&a, st)) return rc;
   if (int rc = orth_small_status(&b, st)) return rc;
-  if (int rc = route_status(&c, st)) return rc;
-  *out = a != 0 || b != 0 || c != 0 ? GMMXX_ERR_TIMEOUT : GMMXX_OK;
+  *out = a != 0 || b != 0 ? GMMXX_ERR_TIMEOUT : GMMXX_OK;
   return GMMXX_OK;
 }
 

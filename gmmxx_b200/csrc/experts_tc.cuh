@@ -123,7 +123,6 @@ int device_sms(int* sms);
 int take_flag(const void* symbol, int* flag, cudaStream_t st);
 int product_status(int* flag, cudaStream_t st);
 int orth_small_status(int* flag, cudaStream_t st);
-int route_status(int* flag, cudaStream_t st);
 
 // stacks of small matrices in one launch (orth_small.cu)
 bool orth_small_fits(int64_t m, int64_t n);

@@ -1,21 +1,23 @@
 // group_rows.cu -- routing: slots sorted by the component they are assigned to
 // (gmmxx_group_rows), and the tables of row tiles that the grouped products walk.
 //
-// A stable counting sort in one launch.  The slots are cut into one contiguous
-// chunk per warp.  Every warp counts its chunk's labels in shared memory (column
-// K: unassigned slots); the warps' counts become their exclusive prefixes within
-// the block, the blocks' totals go to a [blocks][K + 1] table; after a barrier
-// every block knows what comes before it and how many slots each component has;
-// every warp walks its chunk again and places each slot at (group start) +
-// (earlier blocks') + (earlier warps') + (its rank in the warp).  Equal labels
-// keep their slot order and nothing depends on the order in which warps run, so
-// the result is the same in every run.
+// A stable counting sort.  The slots are cut into one contiguous chunk per
+// warp.  Every warp counts its chunk's labels in shared memory (column K:
+// unassigned slots); the warps' counts become their exclusive prefixes within
+// the block, the blocks' totals go to a [blocks][K + 1] table; once that is
+// complete every block knows what comes before it and how many slots each
+// component has; every warp walks its chunk again and places each slot at (group
+// start) + (earlier blocks') + (earlier warps') + (its rank in the warp).  Equal
+// labels keep their slot order and nothing depends on the order in which warps
+// run, so the result is the same in every run.
 //
-// The barrier is none for one block, a cluster's for up to 8 blocks, and for
-// more a counter in the workspace of a cooperative launch (bounded waits).  With
-// a small table every block sums the rows it needs; a large one (blocks x
-// components) is scanned by columns, one block a share of the columns, between
-// two barriers.
+// One block needs no table, up to 8 blocks are a cluster and meet at its
+// barrier: one launch.  More blocks take a launch to count and one to place,
+// which counts again (from L2) rather than keep every warp's counts; a small
+// table is summed by every block itself, a large one (blocks x components) is
+// scanned by columns in a launch between.  The later launches set themselves up,
+// and count, while the one before them ends.  (A cooperative launch with barriers
+// over the grid takes 15 to 35 us longer outside a graph: the host's part of it.)
 //
 // A rank in a warp takes a match over the warp only where a label occurs twice:
 // each lane reads its label's counter and then adds to it, and if every lane's
@@ -38,18 +40,17 @@ constexpr int kMaxSmem = 216 * 1024;
 constexpr int kMaxWarps = 32;
 constexpr int kDirectTable = 32768;  // table entries up to which every block reads the rows it needs itself
 
-static __device__ int g_route_status = 0;  // sticky: 1 when the bounded barrier ran out
-
-enum Sync { kOneBlock = 0, kCluster = 1, kGrid = 2 };
+// the whole sort in one block or one cluster, or the two launches around a table
+enum Part { kOneBlock = 0, kCluster = 1, kCount = 2, kPlace = 3 };
 
 struct RouteArgs {
   const void* labels;
   int wide;       // int64 labels
   int slots, K;
-  int chunk;      // slots per warp, a multiple of 32
+  int warps;      // walking warps per block
+  int chunk;      // slots per walking warp, a multiple of 32
   int* table;     // [blocks][K + 1]
   int* total;     // [K + 1]
-  int* barrier;   // kGrid: zero at launch
   int32_t* order;
   int32_t* offsets;
   int32_t* tiles;
@@ -147,33 +148,52 @@ __device__ __forceinline__ Three block_exclusive3(Three v, int* red, Three* tota
     red[64 + w] = s.c;
   }
   __syncthreads();
-  Three before = {0, 0, 0}, all = {0, 0, 0};
-  for (int i = 0; i < nw; ++i) {
-    const int x = red[i], y = red[32 + i], z = red[64 + i];
-    if (i < w) {
-      before.a += x;
-      before.b += y;
-      before.c += z;
+  // every warp scans the warps' sums itself
+  Three t = {0, 0, 0};
+  if (lane < nw) t = {red[lane], red[32 + lane], red[64 + lane]};
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, t.a, o), y = __shfl_up_sync(0xffffffffu, t.b, o),
+              z = __shfl_up_sync(0xffffffffu, t.c, o);
+    if (lane >= o) {
+      t.a += x;
+      t.b += y;
+      t.c += z;
     }
-    all.a += x;
-    all.b += y;
-    all.c += z;
   }
-  *total = all;
-  return {before.a + s.a - v.a, before.b + s.b - v.b, before.c + s.c - v.c};
+  *total = {__shfl_sync(0xffffffffu, t.a, 31), __shfl_sync(0xffffffffu, t.b, 31), __shfl_sync(0xffffffffu, t.c, 31)};
+  const int p = w > 0 ? w - 1 : 0;
+  const Three before = {__shfl_sync(0xffffffffu, t.a, p), __shfl_sync(0xffffffffu, t.b, p),
+                        __shfl_sync(0xffffffffu, t.c, p)};
+  return {(w ? before.a : 0) + s.a - v.a, (w ? before.b : 0) + s.b - v.b, (w ? before.c : 0) + s.c - v.c};
 }
 
 // Starts of the groups' rows, 128-row tiles and 256-row tiles from the sizes:
 // out(k, rows, tiles, pairs) for k = 0 .. K.  Returns the totals.
 template <typename Size, typename Out>
 __device__ __forceinline__ Three scan_groups(int K, int* red, Size size, Out out) {
+  constexpr int kEach = 4;  // consecutive groups per thread
   Three at = {0, 0, 0};
-  for (int k0 = 0; k0 <= K; k0 += blockDim.x) {
-    const int k = k0 + threadIdx.x;
-    const int c = k <= K ? size(k) : 0;
-    Three all;
-    const Three v = block_exclusive3({c, (c + kTileRows - 1) / kTileRows, (c + kPairRows - 1) / kPairRows}, red, &all);
-    if (k <= K) out(k, at.a + v.a, at.b + v.b, at.c + v.c);
+  for (int k0 = 0; k0 <= K; k0 += kEach * blockDim.x) {
+    const int k = k0 + kEach * threadIdx.x;
+    int c[kEach];
+    Three sum = {0, 0, 0}, all;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) c[j] = k + j <= K ? size(k + j) : 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      sum.a += c[j];
+      sum.b += (c[j] + kTileRows - 1) / kTileRows;
+      sum.c += (c[j] + kPairRows - 1) / kPairRows;
+    }
+    Three v = block_exclusive3(sum, red, &all);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      if (k + j <= K) out(k + j, at.a + v.a, at.b + v.b, at.c + v.c);
+      v.a += c[j];
+      v.b += (c[j] + kTileRows - 1) / kTileRows;
+      v.c += (c[j] + kPairRows - 1) / kPairRows;
+    }
     at.a += all.a;
     at.b += all.b;
     at.c += all.c;
@@ -198,45 +218,46 @@ __device__ __forceinline__ void fill_tile(int K, const int* first, const int* st
   e[2] = min(per, end - pos);
 }
 
-// All blocks' writes before it are visible after it.  False when the bounded
-// wait ran out (kGrid).
-template <int SYNC>
-__device__ __forceinline__ bool barrier(const RouteArgs& a, int round) {
-  if (SYNC == kOneBlock) {
-    __syncthreads();
-    return true;
+__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// columns of the table scanned over the blocks: 32 columns per block, its 32
+// warps take a share of the rows each; total[k] gets the column's sum
+__global__ void __launch_bounds__(1024) columns_kernel(int* table, int nblocks, int K1, int* total) {
+  __shared__ int part[32][33];
+  dependents_may_start();
+  wait_for_launch_before();
+  const int lane = threadIdx.x & 31, seg = threadIdx.x >> 5, k = blockIdx.x * 32 + lane;
+  const int per = (nblocks + 31) / 32, b0 = min(nblocks, seg * per), b1 = min(nblocks, b0 + per);
+  constexpr int kHeld = 8;  // of nblocks <= 148: at most 5 rows per warp
+  int held[kHeld], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    held[i] = b0 + i < b1 && k < K1 ? __ldcg(table + (int64_t)(b0 + i) * K1 + k) : 0;
+    sum += held[i];
   }
-  if (SYNC == kCluster) {
-    __syncthreads();
-    ptx::cluster_sync();
-    return true;
-  }
+  part[seg][lane] = sum;
   __syncthreads();
-  int ok = 1;
-  if (threadIdx.x == 0) {
-    __threadfence();
-    atomicAdd(a.barrier, 1);
-    const int want = (int)gridDim.x * round;
-    const long long t0 = clock64();
-    while (*(volatile int*)a.barrier < want) {
-      if (clock64() - t0 > kWaitCycles) {
-        ok = 0;
-        atomicOr(&g_route_status, 1);
-        break;
-      }
-    }
-    __threadfence();
+  int run = 0;
+  for (int s = 0; s < seg; ++s) run += part[s][lane];
+  if (k >= K1) return;
+  if (seg == 31) total[k] = run + sum;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    if (b0 + i < b1) table[(int64_t)(b0 + i) * K1 + k] = run;
+    run += held[i];
   }
-  return __syncthreads_and(ok) != 0;
 }
 
-template <int SYNC, bool PACK>
+template <int PART, bool PACK>
 __global__ void __launch_bounds__(kMaxWarps * 32, 1) route_kernel(const RouteArgs a) {
   extern __shared__ int sm[];
   __shared__ int red[96];
   __shared__ int part[2][32][33];
-  const int K = a.K, K1 = K + 1, warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int nblocks = SYNC == kOneBlock ? 1 : (int)gridDim.x, block = blockIdx.x;
+  if (PART == kCount) dependents_may_start();
+  // `warps` of the block walk the slots; where their counters leave room for few, the block has more for the rest
+  const int K = a.K, K1 = K + 1, warps = a.warps, all_warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nblocks = PART == kOneBlock ? 1 : (int)gridDim.x, block = blockIdx.x;
   const int words = Counters<PACK>::words(K1);
   int* base = sm;                 // [K1] totals of the block, then where its slots of each label go
   int* counters = sm + K1;        // [warps][words]
@@ -245,9 +266,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) route_kernel(const RouteArg
   int* first2 = first + K1;
   for (int i = threadIdx.x; i < warps * words; i += blockDim.x) counters[i] = 0;
   __syncthreads();
-  const Counters<PACK> mine{counters + warp * words};
+  const Counters<PACK> mine{counters + min(warp, warps - 1) * words};
   const int64_t from = ((int64_t)block * warps + warp) * a.chunk;
-  const int begin = (int)min((int64_t)a.slots, from), end = (int)min((int64_t)a.slots, from + a.chunk);
+  const int begin = warp < warps ? (int)min((int64_t)a.slots, from) : 0;
+  const int end = warp < warps ? (int)min((int64_t)a.slots, from + a.chunk) : 0;
   walk<PACK, true>(a, begin, end, mine, nullptr);
   __syncthreads();
   // counts -> exclusive prefixes over the block's warps; the block's totals
@@ -280,10 +302,22 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) route_kernel(const RouteArg
   __syncthreads();
   const bool direct = a.direct != 0;
   int* row = a.table + (int64_t)block * K1;
-  if (SYNC != kOneBlock) {
+  if (PART == kCluster || PART == kCount)
     for (int k = threadIdx.x; k < K1; k += blockDim.x) row[k] = base[k];
-    if (!barrier<SYNC>(a, 1)) return;
-    if (direct && nblocks <= 16) {  // few rows: a thread per column
+  if (PART == kCount) return;
+  if (PART == kPlace) wait_for_launch_before();
+  if (PART == kOneBlock) {
+    for (int k = threadIdx.x; k < K1; k += blockDim.x) {
+      if (direct) size[k] = base[k];
+      else a.total[k] = base[k];
+      base[k] = 0;
+    }
+  } else {
+    __syncthreads();
+    if (PART == kCluster) ptx::cluster_sync();
+    if (!direct && PART == kPlace) {  // scanned by columns_kernel
+      for (int k = threadIdx.x; k < K1; k += blockDim.x) base[k] = __ldcg(row + k);
+    } else if (nblocks <= 16) {  // few rows: a thread per column
       for (int k = threadIdx.x; k < K1; k += blockDim.x) {
         int all = 0, before = 0;
 #pragma unroll 8
@@ -293,12 +327,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) route_kernel(const RouteArg
           before += b < block ? c : 0;
         }
         base[k] = before;
-        size[k] = all;
+        if (direct) size[k] = all;
+        else if (block == 0) a.total[k] = all;
       }
-    } else {
-      // 32 columns at a time, the rows cut over the warps
-      const int per = (nblocks + warps - 1) / warps, b0 = min(nblocks, warp * per), b1 = min(nblocks, b0 + per);
-      for (int k0 = direct ? 0 : block * 32; k0 < K1; k0 += direct ? 32 : nblocks * 32) {
+      if (!direct) ptx::cluster_sync();  // kCluster: the totals
+    } else {  // 32 columns at a time, the rows cut over the warps
+      const int per = (nblocks + all_warps - 1) / all_warps, b0 = min(nblocks, warp * per), b1 = min(nblocks, b0 + per);
+      for (int k0 = 0; k0 < K1; k0 += 32) {
         const int k = k0 + lane;
         int all = 0, before = 0;
         if (k < K1) {
@@ -312,41 +347,17 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) route_kernel(const RouteArg
         part[0][warp][lane] = all;
         part[1][warp][lane] = before;
         __syncthreads();
-        if (direct) {  // this block's start and the total of its columns
-          if (warp == 0 && k < K1) {
-            int t = 0, f = 0;
-            for (int w = 0; w < warps; ++w) {
-              t += part[0][w][lane];
-              f += part[1][w][lane];
-            }
-            base[k] = f;
-            size[k] = t;
+        if (warp == 0 && k < K1) {
+          int t = 0, f = 0;
+          for (int w = 0; w < all_warps; ++w) {
+            t += part[0][w][lane];
+            f += part[1][w][lane];
           }
-        } else {  // every block's start, in place
-          int run = 0;
-          for (int w = 0; w < warp; ++w) run += part[0][w][lane];
-          if (k < K1) {
-            if (warp == warps - 1) a.total[k] = run + all;
-            for (int b = b0; b < b1; ++b) {
-              int* p = a.table + (int64_t)b * K1 + k;
-              const int c = __ldcg(p);
-              *p = run;
-              run += c;
-            }
-          }
+          base[k] = f;
+          size[k] = t;
         }
         __syncthreads();
       }
-    }
-    if (!direct) {
-      if (!barrier<SYNC>(a, 2)) return;
-      for (int k = threadIdx.x; k < K1; k += blockDim.x) base[k] = __ldcg(row + k);
-    }
-  } else {
-    for (int k = threadIdx.x; k < K1; k += blockDim.x) {
-      if (direct) size[k] = base[k];
-      else a.total[k] = base[k];
-      base[k] = 0;
     }
   }
   __syncthreads();
@@ -385,8 +396,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) route_kernel(const RouteArg
 
 struct Plan {
   bool pack, keep, direct;
-  int warps, blocks, chunk, smem;
-  int64_t table, total, barrier, bytes;  // workspace offsets
+  int warps, threads, blocks, chunk, smem;
+  int64_t table, total, bytes;  // workspace offsets
 };
 
 Plan make_plan(int64_t slots, int64_t K, int sms) {
@@ -410,52 +421,70 @@ Plan make_plan(int64_t slots, int64_t K, int sms) {
     p.blocks = sms;
     p.chunk = (int)round_up(ceil_div(slots, (int64_t)p.warps * p.blocks), 32);
   }
+  p.threads = p.keep ? p.warps * 32 : kMaxWarps * 32;
   const int64_t counters = p.warps * (p.pack ? (K1 + 1) / 2 * 4 : K1 * 4);
   p.smem = (int)(p.keep ? fixed + counters + scans : std::max(fixed + counters, scans));
   p.direct = p.keep && (p.blocks <= 8 || p.blocks * K1 <= kDirectTable);
   int64_t off = 0;
   p.table = off; off += round_up((int64_t)p.blocks * K1 * 4, 256);
   p.total = off; off += round_up(K1 * 4, 256);
-  p.barrier = off; off += 256;
   p.bytes = p.blocks == 1 && p.direct ? 256 : off;
   return p;
 }
 
-template <int SYNC, bool PACK>
+template <int PART, bool PACK>
 int launch_route(const RouteArgs& a, const Plan& p, cudaStream_t st) {
-  const auto kern = route_kernel<SYNC, PACK>;
+  const auto kern = route_kernel<PART, PACK>;
   static SmemGrants grants;
   if (int rc = allow_smem((const void*)kern, kMaxSmem, grants)) return rc;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  if (SYNC == kCluster) {
+  if (PART == kCluster) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = p.blocks;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
   } else {
-    attr[0].id = cudaLaunchAttributeCooperative;
-    attr[0].val.cooperative = 1;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
   }
   cfg.gridDim = dim3(p.blocks);
-  cfg.blockDim = dim3(p.warps * 32);
+  cfg.blockDim = dim3(p.threads);
   cfg.dynamicSmemBytes = p.smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = SYNC == kOneBlock ? 0 : 1;
+  cfg.numAttrs = PART == kCluster || PART == kPlace ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "route_kernel launch: %s", cudaGetErrorString(e));
   return GMMXX_OK;
 }
 
-// The plan must not depend on a device query where the workspace is sized
-// without one: B200's SM count.  A device with fewer SMs could not hold the
-// cooperative grid at once and would refuse the launch.
+template <bool PACK>
+int launch_parts(const RouteArgs& a, const Plan& p, cudaStream_t st) {
+  if (p.blocks == 1) return launch_route<kOneBlock, PACK>(a, p, st);
+  if (p.blocks <= 8) return launch_route<kCluster, PACK>(a, p, st);
+  if (int rc = launch_route<kCount, PACK>(a, p, st)) return rc;
+  if (!p.direct) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)ceil_div(a.K + 1, 32));
+    cfg.blockDim = dim3(1024);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, columns_kernel, a.table, p.blocks, a.K + 1, a.total);
+    if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "columns_kernel launch: %s", cudaGetErrorString(e));
+  }
+  return launch_route<kPlace, PACK>(a, p, st);
+}
+
+// The plan must not depend on a device query, since the workspace is sized
+// without one: B200's SM count.
 constexpr int kSms = 148;
 
 }  // namespace
-
-int route_status(int* flag, cudaStream_t st) { return take_flag((const void*)&g_route_status, flag, st); }
 
 int64_t tiles_len(int64_t slots, int64_t K) {
   return kTileHeader + kTileInts * (most_tiles(slots, K, kTileRows) + most_tiles(slots, K, kPairRows));
@@ -471,21 +500,17 @@ int launch_group_rows(const void* labels, int wide, int64_t slots, int64_t K, in
   a.wide = wide;
   a.slots = (int)slots;
   a.K = (int)K;
+  a.warps = p.warps;
   a.chunk = p.chunk;
   a.table = reinterpret_cast<int*>(ws + p.table);
   a.total = reinterpret_cast<int*>(ws + p.total);
-  a.barrier = reinterpret_cast<int*>(ws + p.barrier);
   a.order = order;
   a.offsets = offsets;
   a.tiles = tiles;
   a.pairs = kTileInts * most_tiles(slots, K, kTileRows);
   a.keep = p.keep;
   a.direct = p.direct;
-  if (p.blocks == 1) return p.pack ? launch_route<kOneBlock, true>(a, p, st) : launch_route<kOneBlock, false>(a, p, st);
-  if (p.blocks <= 8) return p.pack ? launch_route<kCluster, true>(a, p, st) : launch_route<kCluster, false>(a, p, st);
-  const cudaError_t e = cudaMemsetAsync(a.barrier, 0, sizeof(int), st);
-  if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "memset: %s", cudaGetErrorString(e));
-  return p.pack ? launch_route<kGrid, true>(a, p, st) : launch_route<kGrid, false>(a, p, st);
+  return p.pack ? launch_parts<true>(a, p, st) : launch_parts<false>(a, p, st);
 }
 
 }  // namespace experts

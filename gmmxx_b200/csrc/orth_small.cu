@@ -32,8 +32,6 @@ using namespace ptx;
 
 namespace {
 
-constexpr int kOrthThreads = 256;
-
 static __device__ int g_orth_status = 0;  // sticky: 1 when a bounded wait ran out
 
 struct OrthArgs {
@@ -53,9 +51,14 @@ struct OrthArgs {
   float a, b, c, eps;
 };
 
-__device__ __forceinline__ void load16(uint32_t addr, float* v) {
-  tmem_ld16(addr, v);
+// the sum of two accumulators' 16 columns
+__device__ __forceinline__ void load_sum16(uint32_t lead, uint32_t rest, float* v) {
+  float u[16];
+  tmem_ld16(lead, u);
+  tmem_ld16(rest, v);
   tmem_wait_ld();
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] += u[j];
 }
 
 // 8 values of a row to / from the planes
@@ -82,11 +85,15 @@ __device__ __forceinline__ void add8(const char* hi, const char* lo, uint32_t of
   }
 }
 
-__global__ void __launch_bounds__(kOrthThreads) orth_small_kernel(const OrthArgs a) {
+// THREADS: 256 where four blocks share an SM, else 512 (the epilogues, which the
+// chain of products waits for, take half the time)
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) orth_small_kernel(const OrthArgs a) {
+  constexpr int kParts = THREADS / 128;  // warps per quarter of the accumulators' lanes: shares of the columns
   extern __shared__ __align__(1024) char smem_raw[];
   __shared__ uint64_t bar;
   __shared__ uint32_t tmem_base;
-  __shared__ double red[kOrthThreads / 32];
+  __shared__ double red[THREADS / 32];
   char* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rb = a.rows * 128;  // bytes of a block of 64 columns
@@ -102,7 +109,7 @@ __global__ void __launch_bounds__(kOrthThreads) orth_small_kernel(const OrthArgs
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = tmem_base;
-  // this thread's row of the accumulators and its half of their columns
+  // this thread's row of the accumulators and its share of their columns
   const int row = (warp & 3) * 32 + lane, part = warp >> 2;
   const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
   const bool active = (warp & 3) * 32 < a.rows;  // blocks of 64 rows: half of the warps have none
@@ -115,20 +122,20 @@ __global__ void __launch_bounds__(kOrthThreads) orth_small_kernel(const OrthArgs
   for (int64_t z = blockIdx.x; ok && z < a.batch; z += gridDim.x) {
     const int64_t size = (int64_t)a.m * a.n, base = z * size;
     double s = 0.0;
-    for (int64_t i = tid; i < size; i += kOrthThreads) {
+    for (int64_t i = tid; i < size; i += THREADS) {
       const double v = load_x(a.g, base + i, a.dt);
       s += v * v;
     }
     s = block_sum(s, red);
     const double inv = 1.0 / (sqrt(s) + (double)a.eps);
     if (a.steps == 0) {
-      for (int64_t i = tid; i < size; i += kOrthThreads)
+      for (int64_t i = tid; i < size; i += THREADS)
         store_y(a.q, base + i, a.dt, (float)(load_x(a.g, base + i, a.dt) * inv));
       continue;
     }
     // X, zero outside lo x hi: the products then keep every padding zero
     const int pieces = a.xb * 8;
-    for (int i = tid; i < a.rows * pieces; i += kOrthThreads) {
+    for (int i = tid; i < a.rows * pieces; i += THREADS) {
       const int r = a.tall ? i % a.rows : i / pieces, c = (a.tall ? i / a.rows : i % pieces) * 8;
       float v[8];
 #pragma unroll
@@ -161,11 +168,13 @@ __global__ void __launch_bounds__(kOrthThreads) orth_small_kernel(const OrthArgs
       phase ^= 1;
       tmem_fence_after();
       if (active)
-        for (int c = part * (a.np / 2); c < (part + 1) * (a.np / 2); c += 16) {
-          float v[16], u[16];
-          load16(corr_p + c + lanes, v);
-          for (int i = 0; i < a.chunks; ++i) {
-            load16(tmem + i * a.np + c + lanes, u);
+        for (int c = part * (a.np / kParts); c < (part + 1) * (a.np / kParts); c += 16) {
+          float v[16];
+          load_sum16(tmem + c + lanes, corr_p + c + lanes, v);
+          for (int i = 1; i < a.chunks; ++i) {
+            float u[16];
+            tmem_ld16(tmem + i * a.np + c + lanes, u);
+            tmem_wait_ld();
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] += u[j];
           }
@@ -194,12 +203,11 @@ __global__ void __launch_bounds__(kOrthThreads) orth_small_kernel(const OrthArgs
       phase ^= 1;
       tmem_fence_after();
       if (active)
-        for (int c = part * (a.np / 2); c < (part + 1) * (a.np / 2); c += 16) {
-          float v[16], u[16];
-          load16(tmem + a.np + c + lanes, v);
-          load16(tmem + c + lanes, u);
+        for (int c = part * (a.np / kParts); c < (part + 1) * (a.np / kParts); c += 16) {
+          float v[16];
+          load_sum16(tmem + c + lanes, tmem + a.np + c + lanes, v);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = (v[j] + u[j]) * (a.c * down);
+          for (int j = 0; j < 16; ++j) v[j] *= a.c * down;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t off = (c >> 6) * rb + sw128(row, (c & 63) + 8 * h);
@@ -229,14 +237,13 @@ __global__ void __launch_bounds__(kOrthThreads) orth_small_kernel(const OrthArgs
         phase ^= 1;
         tmem_fence_after();
         if (active)
-          for (int c = part * (a.xn / 2); c < (part + 1) * (a.xn / 2); c += 16) {
+          for (int c = part * (a.xn / kParts); c < (part + 1) * (a.xn / kParts); c += 16) {
             const int col = ch * 128 + c;
             if (col >= a.xb * 64) break;
-            float v[16], u[16];
-            load16(tmem + a.xn + c + lanes, v);
-            load16(tmem + c + lanes, u);
+            float v[16];
+            load_sum16(tmem + c + lanes, tmem + a.xn + c + lanes, v);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = (v[j] + u[j]) * down;
+            for (int j = 0; j < 16; ++j) v[j] *= down;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint32_t off = (col >> 6) * rb + sw128(row, (col & 63) + 8 * h);
@@ -306,13 +313,16 @@ int launch_orth_small(int dt, const void* g, int64_t batch, int64_t m, int64_t n
   int smem = 2 * (t.xb + t.pb) * t.rows * 128 + 8192 + 1024;
   // as many blocks per SM as tensor memory serves (an SM that held more would let them wait for it)
   const int per_sm = std::min(512 / t.tmem, std::max(1, (232448 - 4096) / (smem + 2048)));
-  smem = std::max(smem, 226 * 1024 / per_sm - 3072);
-  static SmemGrants grants;
-  if (int rc = allow_smem((const void*)orth_small_kernel, 231424, grants)) return rc;
+  smem = std::max(smem, 225 * 1024 / per_sm - 3072);
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
+  // four blocks of 64 x 64 per SM only where there are matrices for them
+  const bool shared = per_sm > 2 && batch > 2 * sms;
   const unsigned grid = (unsigned)std::min<int64_t>(batch, (int64_t)sms * per_sm);
-  orth_small_kernel<<<grid, kOrthThreads, smem, st>>>(t);
+  static SmemGrants grants256, grants512;
+  const auto kern = shared ? orth_small_kernel<256> : orth_small_kernel<512>;
+  if (int rc = allow_smem((const void*)kern, 230000, shared ? grants256 : grants512)) return rc;
+  kern<<<grid, shared ? 256 : 512, smem, st>>>(t);
   return check_launch("orth_small_kernel");
 }
 

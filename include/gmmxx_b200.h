@@ -318,7 +318,7 @@ GMMXX_API int gmmxx_grouped_matmul_backward(int dtype, const void* grad_out, con
                                             size_t workspace_bytes, void* stream);
 
 /* GMMXX_OK, or GMMXX_ERR_TIMEOUT when a bounded device-side wait ran out in a
- * routing, product or orthogonalisation kernel of the current device since the last
+ * product or orthogonalisation kernel of the current device since the last
  * call (those kernels' results are undefined).  Synchronises the stream. */
 GMMXX_API int gmmxx_products_status(int* status_out, void* stream);
 
