@@ -570,6 +570,7 @@ int stack_operand(const Stack& s, int planes, int64_t batch, int box_rows, CUten
 }  // namespace
 
 size_t grouped_matmul_ws(int dt, const Groups& g, int64_t n_in, int64_t n_out) {
+  // (what the thin form does not use stays unused: the size must not depend on the weight's order)
   // the weight's inner length is n_out or (transposed) n_in: room for either
   const int64_t w = std::max(pack_bytes(dt, g.K * n_in, n_out), pack_bytes(dt, g.K * n_out, n_in));
   return (size_t)(256 + routed_bytes(dt, g.rows, n_in, g) + w);
@@ -577,6 +578,9 @@ size_t grouped_matmul_ws(int dt, const Groups& g, int64_t n_in, int64_t n_out) {
 
 int launch_grouped_matmul(int dt, const void* x, const Groups& g, int64_t n_in, int64_t n_out, const void* w, int wt,
                           const void* bias, void* out, char* ws, cudaStream_t st) {
+  if (thin_rows_fit(dt, g, wt ? n_in : n_out))
+    return launch_thin_rows(static_cast<const float*>(x), g.top, g, n_in, n_out, static_cast<const float*>(w), wt,
+                            static_cast<const float*>(bias), static_cast<float*>(out), st);
   Planes px, pw;
   if (int rc = routed(dt, x, g.rows, n_in, g, g.top, ws, &px, st)) return rc;
   if (int rc = operand(dt, w, g.K * (wt ? n_out : n_in), wt ? n_in : n_out, nullptr, 1, ws, &pw, st)) return rc;
@@ -595,18 +599,24 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
                             const void* w, int wt, void* gx, void* gw, void* gb, char* ws, cudaStream_t st) {
   Planes pg, pw, px;
   const int64_t slots = g.slots();
-  if (slots > 0 && (gx != nullptr || gw != nullptr))
+  const bool thin = thin_rows_fit(dt, g, wt ? n_in : n_out);
+  if (slots > 0 && ((gx != nullptr && !thin) || gw != nullptr))
     if (int rc = routed(dt, gy, slots, n_out, g, 1, ws, &pg, st)) return rc;
   if (slots > 0 && gx != nullptr) {
-    if (int rc = operand(dt, w, g.K * (wt ? n_out : n_in), wt ? n_in : n_out, nullptr, 1, ws, &pw, st)) return rc;
     void* to = gx;
     if (g.top > 1) {
       to = ws;
       ws += al256(slots * n_in * 4);
     }
-    if (int rc = rows_product(dt, pg, 1, g, n_out, n_in, pw, wt == 0, nullptr, to,
-                              g.top > 1 ? GMMXX_FLOAT32 : dt, st))
-      return rc;
+    const int to_dt = g.top > 1 ? GMMXX_FLOAT32 : dt;
+    if (thin) {
+      if (int rc = launch_thin_rows(static_cast<const float*>(gy), 1, g, n_out, n_in, static_cast<const float*>(w), !wt,
+                                    nullptr, static_cast<float*>(to), st))
+        return rc;
+    } else {
+      if (int rc = operand(dt, w, g.K * (wt ? n_out : n_in), wt ? n_in : n_out, nullptr, 1, ws, &pw, st)) return rc;
+      if (int rc = rows_product(dt, pg, 1, g, n_out, n_in, pw, wt == 0, nullptr, to, to_dt, st)) return rc;
+    }
     if (g.top > 1) {
       const int per = vec_ok(gx, dt, n_in) ? 4 : 1;
       const dim3 grid((unsigned)std::min<int64_t>(g.rows, 148 * 64), (unsigned)ceil_div(n_in, 256 * per));

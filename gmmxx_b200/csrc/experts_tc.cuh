@@ -129,5 +129,10 @@ bool orth_small_fits(int64_t m, int64_t n);
 int launch_orth_small(int dt, const void* g, int64_t batch, int64_t m, int64_t n, int steps, float a, float b, float c,
                       float eps, void* q, cudaStream_t st);
 
+// fp32 rows times matrices where groups have few rows (thin_rows.cu); inner: length of the weights' contiguous rows
+bool thin_rows_fit(int dt, const Groups& g, int64_t inner);
+int launch_thin_rows(const float* x, int div, const Groups& g, int64_t k, int64_t n, const float* w, int kmajor,
+                     const float* bias, float* out, cudaStream_t st);
+
 }  // namespace experts
 }  // namespace gmmxx

@@ -1,0 +1,200 @@
+// thin_rows.cu -- fp32 rows times their group's matrix where a group has few
+// rows: the weights are read once, as they lie, and multiplied on the CUDA cores.
+//
+// With r rows per group every weight serves r products: with few of them the
+// launch is bound by the weights' bytes, and the tensor-core kernel's laying out
+// of fp32 weights as three planes (6 bytes written and read per weight of 4) is
+// what it spends its time on.  Measured against it, 1 / 4 / 8 rows per group:
+// 58 x (320 x 1728) 32 / 56 / 83 us to 108 / 126 / 128, 16 x (2048 x 1024) 64 /
+// 101 / 162 to 134 / 137 / 137, 200 x (128 x 192) 10 / 19 / 26 to 23 / 27 / 28;
+// the transposed product less at 4 rows (127 to 125 at the first), more at 1.
+// 16-bit weights lose to it at any number of rows but one.  Here a block takes one
+// tile of the row-tile table, 128 columns and eight rows at a time (the weights
+// come from L2 for the second eight), the rows staged in shared memory:
+//
+//   columns contiguous (x W):   a warp takes every eighth group of four
+//     contraction elements, a lane four columns; the eight warps' sums are added
+//     in warp order;
+//   contraction contiguous (x W^T): a warp takes four columns at a time, a lane
+//     four contraction elements of every 128; the 32 sums of eight rows and four
+//     columns are added over the lanes by halving (31 shuffles).
+//
+// fp32 products and sums, in an order that depends on nothing but the sizes.
+#include "experts_api.cuh"
+#include "experts_tc.cuh"
+
+#include <algorithm>
+
+namespace gmmxx {
+namespace experts {
+namespace {
+
+constexpr int kRowsAt = 8;      // rows of one pass over the weights
+constexpr int kCols = 128;      // columns of a block
+constexpr int kPiece = 1024;    // contraction elements staged at a time
+constexpr int kWarpsThin = 8;
+
+struct ThinArgs {
+  const float* x;
+  int div;
+  Groups g;
+  int k, n;
+  const float* w;  // rows of multiples of four elements, 16-byte aligned
+  const float* bias;
+  float* out;
+};
+
+// four consecutive weights, or zeros behind the end of the row (of a multiple of four)
+__device__ __forceinline__ float4 four(const float* w, int64_t i, bool in) {
+  return in ? __ldg(reinterpret_cast<const float4*>(w + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+// KMAJOR: w (K, n, k), else (K, k, n)
+template <bool KMAJOR>
+__global__ void __launch_bounds__(kWarpsThin * 32) thin_kernel(const ThinArgs a) {
+  __shared__ __align__(16) float xs[kRowsAt][kPiece];       // also the warps' sums
+  __shared__ int slot[kRowsAt];
+  if ((int)blockIdx.y >= a.g.tiles[0]) return;
+  const int32_t* e = a.g.tiles + kTileHeader + (int64_t)blockIdx.y * kTileInts;
+  const int g = e[0], pos = e[1], rows = e[2];
+  const int c0 = blockIdx.x * kCols, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (g >= a.g.K) {  // unassigned slots
+    for (int i = threadIdx.x; i < rows * kCols; i += kWarpsThin * 32) {
+      const int c = c0 + i % kCols;
+      if (c < a.n) a.out[(int64_t)a.g.order[pos + i / kCols] * a.n + c] = 0.f;
+    }
+    return;
+  }
+  const int64_t wg = (int64_t)g * a.k * a.n;
+  for (int r0 = 0; r0 < rows; r0 += kRowsAt) {
+    const int nr = min(kRowsAt, rows - r0);
+    if (threadIdx.x < kRowsAt) slot[threadIdx.x] = (int)threadIdx.x < nr ? a.g.order[pos + r0 + threadIdx.x] : -1;
+    float acc[kRowsAt][4];  // column form: rows x this lane's columns; dot form: used per four columns
+#pragma unroll
+    for (int r = 0; r < kRowsAt; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[r][j] = 0.f;
+    float dots[kCols / (4 * kWarpsThin)];  // dot form: this lane's (row, column) of each group of four columns
+#pragma unroll
+    for (int i = 0; i < kCols / (4 * kWarpsThin); ++i) dots[i] = 0.f;
+    for (int k0 = 0; k0 < a.k; k0 += kPiece) {
+      const int kn = min(kPiece, a.k - k0), k4 = (kn + 3) & ~3;
+      __syncthreads();
+      for (int i = threadIdx.x; i < kRowsAt * k4; i += kWarpsThin * 32) {
+        const int r = i / k4, k = i - r * k4;
+        xs[r][k] = r < nr && k < kn ? a.x[(int64_t)(slot[r] / a.div) * a.k + k0 + k] : 0.f;
+      }
+      __syncthreads();
+      if (!KMAJOR) {
+        const int c = c0 + lane * 4;
+#pragma unroll 2
+        for (int k = warp * 4; k < kn; k += kWarpsThin * 4) {
+          float4 w[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            w[u] = four(a.w, wg + (int64_t)(k0 + k + u) * a.n + c, c < a.n && k + u < kn);
+#pragma unroll
+          for (int r = 0; r < kRowsAt; ++r) {
+            const float4 x = *reinterpret_cast<const float4*>(&xs[r][k]);
+            acc[r][0] = fmaf(x.w, w[3].x, fmaf(x.z, w[2].x, fmaf(x.y, w[1].x, fmaf(x.x, w[0].x, acc[r][0]))));
+            acc[r][1] = fmaf(x.w, w[3].y, fmaf(x.z, w[2].y, fmaf(x.y, w[1].y, fmaf(x.x, w[0].y, acc[r][1]))));
+            acc[r][2] = fmaf(x.w, w[3].z, fmaf(x.z, w[2].z, fmaf(x.y, w[1].z, fmaf(x.x, w[0].z, acc[r][2]))));
+            acc[r][3] = fmaf(x.w, w[3].w, fmaf(x.z, w[2].w, fmaf(x.y, w[1].w, fmaf(x.x, w[0].w, acc[r][3]))));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kCols / (4 * kWarpsThin); ++i) {
+          const int c = c0 + (i * kWarpsThin + warp) * 4;
+          if (c >= a.n) break;
+          float s[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) s[j] = 0.f;
+#pragma unroll 2
+          for (int k = lane * 4; k < kn; k += 128) {
+            float4 w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              w[j] = four(a.w, wg + (int64_t)(c + j) * a.k + k0 + k, c + j < a.n);
+#pragma unroll
+            for (int r = 0; r < kRowsAt; ++r) {
+              const float4 x = *reinterpret_cast<const float4*>(&xs[r][k]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                s[r * 4 + j] = fmaf(x.w, w[j].w, fmaf(x.z, w[j].z, fmaf(x.y, w[j].y, fmaf(x.x, w[j].x, s[r * 4 + j]))));
+            }
+          }
+          // lane l ends with the sum of s[l] over the lanes
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            const bool up = (lane & o) != 0;
+#pragma unroll
+            for (int j = 0; j < o; ++j) {
+              const float give = up ? s[j] : s[j + o], keep = up ? s[j + o] : s[j];
+              s[j] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            }
+          }
+          dots[i] += s[0];
+        }
+      }
+    }
+    if (KMAJOR) {
+      const int r = lane >> 2;
+#pragma unroll
+      for (int i = 0; i < kCols / (4 * kWarpsThin); ++i) {
+        const int c = c0 + (i * kWarpsThin + warp) * 4 + (lane & 3);
+        if (r >= nr || c >= a.n) continue;
+        float v = dots[i];
+        if (a.bias != nullptr) v += a.bias[(int64_t)g * a.n + c];
+        a.out[(int64_t)slot[r] * a.n + c] = v;
+      }
+      __syncthreads();  // slot
+    } else {
+      __syncthreads();
+      float* sums = &xs[0][0];  // [warps][rows][columns]
+#pragma unroll
+      for (int r = 0; r < kRowsAt; ++r)
+        *reinterpret_cast<float4*>(sums + (warp * kRowsAt + r) * kCols + lane * 4) =
+            make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+      __syncthreads();
+      for (int i = threadIdx.x; i < nr * kCols; i += kWarpsThin * 32) {
+        const int r = i / kCols, c = c0 + i % kCols;
+        if (c >= a.n) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarpsThin; ++w) v += sums[(w * kRowsAt + r) * kCols + i % kCols];
+        if (a.bias != nullptr) v += a.bias[(int64_t)g * a.n + c];
+        a.out[(int64_t)slot[r] * a.n + c] = v;
+      }
+      __syncthreads();
+    }
+  }
+}
+static_assert(kWarpsThin * kRowsAt * kCols <= kRowsAt * kPiece, "the warps' sums share the rows' memory");
+
+}  // namespace
+
+// Up to four rows per group on average (see above); the grid's second dimension takes the tiles
+bool thin_rows_fit(int dt, const Groups& g, int64_t inner) {
+  return dt == GMMXX_FLOAT32 && inner % 4 == 0 && g.slots() <= 4 * (int64_t)g.K && g.max_tiles() <= 65535;
+}
+
+int launch_thin_rows(const float* x, int div, const Groups& g, int64_t k, int64_t n, const float* w, int kmajor,
+                     const float* bias, float* out, cudaStream_t st) {
+  ThinArgs a{};
+  a.x = x;
+  a.div = div;
+  a.g = g;
+  a.k = (int)k;
+  a.n = (int)n;
+  a.w = w;
+  a.bias = bias;
+  a.out = out;
+  const dim3 grid((unsigned)ceil_div(n, kCols), (unsigned)g.max_tiles());
+  if (kmajor) thin_kernel<true><<<grid, kWarpsThin * 32, 0, st>>>(a);
+  else thin_kernel<false><<<grid, kWarpsThin * 32, 0, st>>>(a);
+  return check_launch("thin_kernel");
+}
+
+}  // namespace experts
+}  // namespace gmmxx

@@ -214,6 +214,29 @@ def test_pairs_of_blocks(cuda_device, n, top, k, n_in, n_out, kind, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,top,k,n_in,n_out,kind", [(30, 1, 9, 1100, 132, "even"), (37, 2, 20, 2051, 36, "dropped"),
+                                                     (20, 2, 11, 2052, 37, "dropped"),
+                                                     (140, 1, 36, 70, 1028, "skewed"), (50, 1, 16, 4, 300, "one")])
+def test_few_rows_per_group(cuda_device, n, top, k, n_in, n_out, kind, dtype):
+    """Groups of a few rows (and one of many), contractions longer than what is
+    staged at a time, both orders of the weights."""
+    import gmmxx_b200 as gm
+
+    labels, x, w, b, gy = _case(cuda_device, n, top, k, n_in, n_out, dtype, kind)
+    groups = gm.group_rows(labels, k)
+    wt = w.transpose(1, 2).contiguous().transpose(1, 2)
+    ref, mag = _reference(x, w, b, labels.cpu(), gy)
+    most = max(1, int((groups.offsets[1:] - groups.offsets[:-1]).max()))
+    for weight in (w, wt):
+        y = gm.grouped_matmul(x, weight, groups, bias=b)
+        gx, gw, gb = gm.grouped_matmul_backward(gy, x, weight, groups, bias=True)
+        _close(y.reshape(n, top, n_out), ref["y"], mag["y"], n_in + 1, dtype)
+        _close(gx, ref["gx"], mag["gx"], n_out + top, dtype)
+        _close(gw, ref["gw"], mag["gw"], most, dtype)
+        _close(gb, ref["gb"], mag["gb"], most, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_long_groups(cuda_device, dtype):
     """Groups of tens of thousands of rows: the weight gradient's sum is split and joined."""
     import gmmxx_b200 as gm
