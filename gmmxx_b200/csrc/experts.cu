@@ -630,7 +630,7 @@ int launch_grouped_backward(int dt, const void* gy, const void* x, const Groups&
     cudaError_t e = cudaSuccess;
     if (gw != nullptr) e = cudaMemsetAsync(gw, 0, (size_t)(g.K * n_in * n_out * elem_bytes(dt)), st);
     if (e == cudaSuccess && gb != nullptr) e = cudaMemsetAsync(gb, 0, (size_t)(g.K * n_out * elem_bytes(dt)), st);
-    return e == cudaSuccess ? GMMXX_OK : set_error(GMMXX_ERR_CUDA, "memset: %s", cudaGetErrorString(e));
+    return e == cudaSuccess ? GMMXX_OK : cuda_failed(e, "memset");
   }
   const SegPlan p = seg_plan(g, n_in, n_out);
   int32_t* table = reinterpret_cast<int32_t*>(ws);

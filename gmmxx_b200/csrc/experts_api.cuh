@@ -47,6 +47,12 @@ __device__ __forceinline__ void store_y(void* p, int64_t i, int dt, float v) {
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+// a failed runtime call's error, taken from the runtime too: the next launch's check must not find it
+inline int cuda_failed(cudaError_t e, const char* what) {
+  cudaGetLastError();
+  return set_error(GMMXX_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
 // Lets `kern` have `bytes` of dynamic shared memory on the current device.
 // `done` (one per kernel) holds the largest size granted so far per device: the
 // call costs more than a launch's other host work.
@@ -59,7 +65,7 @@ inline int allow_smem(const void* kern, int bytes, SmemGrants& done) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && dev < kMaxDevices && done.bytes[dev].load(std::memory_order_relaxed) >= bytes) return GMMXX_OK;
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "kernel attributes: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) return cuda_failed(e, "kernel attributes");
   if (dev < kMaxDevices) {  // only ever grows: a smaller grant must not replace a larger one
     int seen = done.bytes[dev].load(std::memory_order_relaxed);
     while (seen < bytes && !done.bytes[dev].compare_exchange_weak(seen, bytes)) {

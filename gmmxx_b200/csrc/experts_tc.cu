@@ -1011,7 +1011,7 @@ int launch_one(const ProductMaps& maps, const ProductArgs& a, unsigned grid, cud
   cfg.attrs = attr;
   cfg.numAttrs = n;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, maps, a);
-  if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "product_kernel launch: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) return cuda_failed(e, "product_kernel launch");
   return GMMXX_OK;
 }
 
@@ -1037,7 +1037,7 @@ int device_sms(int* sms) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && dev < kMaxDevices && (*sms = known[dev].load(std::memory_order_relaxed)) > 0) return GMMXX_OK;
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "device query: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) return cuda_failed(e, "device query");
   if (dev < kMaxDevices) known[dev].store(*sms, std::memory_order_relaxed);
   return GMMXX_OK;
 }
@@ -1070,7 +1070,7 @@ int take_flag(const void* symbol, int* flag, cudaStream_t st) {
     e = cudaMemcpyToSymbolAsync(symbol, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   }
-  return e == cudaSuccess ? GMMXX_OK : set_error(GMMXX_ERR_CUDA, "status read: %s", cudaGetErrorString(e));
+  return e == cudaSuccess ? GMMXX_OK : cuda_failed(e, "status read");
 }
 
 int product_status(int* flag, cudaStream_t st) { return take_flag((const void*)&g_status, flag, st); }

@@ -455,7 +455,7 @@ int launch_route(const RouteArgs& a, const Plan& p, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = PART == kCluster || PART == kPlace ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
-  if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "route_kernel launch: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) return cuda_failed(e, "route_kernel launch");
   return GMMXX_OK;
 }
 
@@ -475,7 +475,7 @@ int launch_parts(const RouteArgs& a, const Plan& p, cudaStream_t st) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, columns_kernel, a.table, p.blocks, a.K + 1, a.total);
-    if (e != cudaSuccess) return set_error(GMMXX_ERR_CUDA, "columns_kernel launch: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) return cuda_failed(e, "columns_kernel launch");
   }
   return launch_route<kPlace, PACK>(a, p, st);
 }
