@@ -25,7 +25,7 @@
 //
 // Bound by latency up to ~10^5 slots (launch, two walks, a barrier), above by
 // the scattered 4-byte stores of `order` and the walks' occupancy: counters of
-// 8192 components are held in 16 bits (a block's chunk is below 2^16 slots), 12
+// 8192 components are held in 16 bits (a block's chunk is below 2^16 slots), 11
 // warps per SM instead of 6.
 #include "experts_api.cuh"
 #include "experts_tc.cuh"

@@ -313,7 +313,7 @@ int launch_orth_small(int dt, const void* g, int64_t batch, int64_t m, int64_t n
   int smem = 2 * (t.xb + t.pb) * t.rows * 128 + 8192 + 1024;
   // as many blocks per SM as tensor memory serves (an SM that held more would let them wait for it)
   const int per_sm = std::min(512 / t.tmem, std::max(1, (232448 - 4096) / (smem + 2048)));
-  smem = std::max(smem, 225 * 1024 / per_sm - 3072);
+  smem = std::max(smem, 225 * 1024 / per_sm - 3 * 1024);
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
   // four blocks of 64 x 64 per SM only where there are matrices for them
