@@ -522,14 +522,15 @@ struct NsPlan {
   int ksplit, ksteps;  // shares of the long contraction of P = X X^T, where its tiles are few
 };
 
-// One fp16 plane per iterate where the result is rounded to bf16 and the short
-// side is long (its error, 1.0e-3 .. 1.3e-3 of the norm, stays below bf16's own
-// 1.7e-3), else two.
-NsPlan ns_plan(int dt, int64_t batch, int64_t m, int64_t n) {
+// One fp16 plane per iterate where the result is rounded to bf16, the short side
+// is long and the steps are few (with bf16's own 1.66e-3 of the norm, 5 steps end
+// at 1.9e-3 .. 2.1e-3 and 6 at 2.2e-3 .. 2.3e-3; every further step adds), else two.
+constexpr int kOnePlaneSteps = 6;
+NsPlan ns_plan(int dt, int64_t batch, int64_t m, int64_t n, int steps) {
   NsPlan s{};
   s.lo = std::min(m, n);
   s.hi = std::max(m, n);
-  s.planes = dt == GMMXX_BFLOAT16 && s.lo >= 256 ? 1 : 2;
+  s.planes = dt == GMMXX_BFLOAT16 && s.lo >= 256 && steps <= kOnePlaneSteps ? 1 : 2;
   s.ldx = pad8(n);
   s.ldp = pad8(s.lo);
   s.x_plane = al256(batch * m * s.ldx * 2);
@@ -543,12 +544,12 @@ NsPlan ns_plan(int dt, int64_t batch, int64_t m, int64_t n) {
   s.part = off; off += al256(batch * s.nparts * 8);
   // a symmetric product of few tiles leaves SMs idle: as many shares of its contraction as fill them, of at least
   // four stages (a share costs its partial's 4 bytes per element twice)
-  const int64_t steps = ceil_div(s.hi, kBlockK), mt = ceil_div(s.lo, 128), tiles = batch * mt * (mt + 1) / 2;
+  const int64_t stages = ceil_div(s.hi, kBlockK), mt = ceil_div(s.lo, 128), tiles = batch * mt * (mt + 1) / 2;
   s.ksplit = 1;
-  s.ksteps = (int)steps;
-  if (tiles * 2 <= 148 && steps >= 8) {
-    s.ksteps = (int)std::max<int64_t>(4, ceil_div(steps, 148 / tiles));
-    s.ksplit = (int)ceil_div(steps, s.ksteps);
+  s.ksteps = (int)stages;
+  if (tiles * 2 <= 148 && stages >= 8) {
+    s.ksteps = (int)std::max<int64_t>(4, ceil_div(stages, 148 / tiles));
+    s.ksplit = (int)ceil_div(stages, s.ksteps);
   }
   s.shares = off; off += s.ksplit > 1 ? al256(s.ksplit * batch * s.lo * s.ldp * 4) : 0;
   s.bytes = off;
@@ -720,13 +721,13 @@ int read_status(int* out, cudaStream_t st) {
 
 size_t orthogonalize_ws(int dt, int64_t batch, int64_t m, int64_t n) {
   if (orth_small_fits(m, n)) return 256;
-  return (size_t)(ns_plan(dt, batch, m, n).bytes + 256);
+  return (size_t)(ns_plan(dt, batch, m, n, kOnePlaneSteps + 1).bytes + 256);  // room for either
 }
 
 int launch_orthogonalize(int dt, const void* g, int64_t batch, int64_t m, int64_t n, int steps, float a, float b,
                          float c, float eps, void* q, char* ws, cudaStream_t st) {
   if (orth_small_fits(m, n)) return launch_orth_small(dt, g, batch, m, n, steps, a, b, c, eps, q, st);
-  const NsPlan s = ns_plan(dt, batch, m, n);
+  const NsPlan s = ns_plan(dt, batch, m, n, steps);
   const int64_t size = m * n;
   double* part = reinterpret_cast<double*>(ws + s.part);
   for (int64_t z0 = 0; z0 < batch; z0 += 65535) {  // grid y

@@ -8,7 +8,7 @@
 // thread issues tcgen05.mma, and eight epilogue warps drain one accumulator
 // from tensor memory while the next tile's products go to the other.
 //
-// Routed rows of 16-bit types are never copied: four warps fetch each row where
+// Routed rows of 16-bit types are never copied: four warps (eight for kWeights) fetch each row where
 // it lies with 16-byte cp.async into the swizzled stage, for kRows as the
 // K-major A operand, for kWeights -- where the rows are the contraction -- as
 // MN-major A and B operands.  (TMA's gather of four rows per instruction took
